@@ -13,7 +13,6 @@ bits; with ``own`` true through the package's entry points.
 
 from __future__ import annotations
 
-import functools
 import math
 
 import torch
@@ -98,6 +97,8 @@ def draw(rng):
     while b > 1 and b * lq * lk * h * d > 8e9:
         b -= 1
     lk = max(1, min(lk, int(8e9 / (lq * h * d))))
+    if train:       # with a single key the scores' gradient is zero, and what either side returns is rounding
+        lk = max(lk, 4)
     return _cross(b, lq, lk, h, d, hk=hk, bias=rng.choice(["none", "shared", "batch"]),
                   mask=rng.choice(["none", "tail", "holes"]), dtype=dtype, train=train)
 
@@ -161,10 +162,9 @@ def prepare(case, seed):
             state["grad"] = normal(*lead, lq, lk, case["c"]) if case["train"] else None
         else:
             state["grad"] = normal(*lead, case["c"], lq, lk) if case["train"] else None
-        if own:
-            from miniworld_engine_b200 import PositionBuckets
-            state["buckets"] = (PositionBuckets.clipped(top, segments=segments) if kind == "clip" else
-                                PositionBuckets.logarithmic(count, top, bidirectional=kind == "log", segments=segments))
+        if kind != "clip":
+            half = count // 2 if kind == "log" else count
+            state["thresholds"] = torch.tensor(_thresholds(half, half // 2, top), device="cuda")
         return state
     h, hk, d = case["h"], case["hk"], case["d"]
     state["q"], state["k"], state["v"] = normal(b, lq, h, d), normal(b, lk, hk, d), normal(b, lk, hk, d)
@@ -192,13 +192,17 @@ def run(state):
 
 
 def _own_bias(s, case):
-    from miniworld_engine_b200 import relative_position_bias_b200, relative_position_bias_backward_b200
-    seg = {"q_segment": s["q_seg"], "k_segment": s["k_seg"]} if case["chains"] > 1 else {}
-    out = relative_position_bias_b200(s["table"], s["buckets"], s["q_pos"], s["k_pos"], layout=case["layout"],
+    from miniworld_engine_b200 import (PositionBuckets, relative_position_bias_b200,
+                                       relative_position_bias_backward_b200)
+    (kind, count, top), segments = _rule(case["rule"]), case["chains"] > 1
+    buckets = (PositionBuckets.clipped(top, segments=segments) if kind == "clip" else
+               PositionBuckets.logarithmic(count, top, bidirectional=kind == "log", segments=segments))
+    seg = {"q_segment": s["q_seg"], "k_segment": s["k_seg"]} if segments else {}
+    out = relative_position_bias_b200(s["table"], buckets, s["q_pos"], s["k_pos"], layout=case["layout"],
                                       add=s.get("add"), dtype=_DTYPES[case["dtype"]], **seg)
     if not case["train"]:
         return out
-    return out, relative_position_bias_backward_b200(s["grad"], s["buckets"], s["q_pos"], s["k_pos"],
+    return out, relative_position_bias_backward_b200(s["grad"], buckets, s["q_pos"], s["k_pos"],
                                                      layout=case["layout"], **seg)
 
 
@@ -212,7 +216,6 @@ def _own_cross(s, case):
     return (out, dq, dk, dv) if dbias is None else (out, dq, dk, dv, dbias)
 
 
-@functools.lru_cache(maxsize=None)
 def _thresholds(n, first, top):
     """Smallest distances of buckets first + 1 ... n - 1 of ``n`` logarithmic ones, in whole numbers: the
     smallest t with t^(n-first) >= first^(n-first-k) * top^k."""
@@ -234,9 +237,7 @@ def _plain_buckets(s, case):
         half = count // 2 if kind == "log" else count
         dist = delta.abs() if kind == "log" else delta.clamp(min=0)
         first = half // 2
-        u = dist.clamp(max=first)
-        for t in _thresholds(half, first, top):
-            u = u + (dist >= t)
+        u = dist.clamp(max=first) + torch.bucketize(dist, s["thresholds"], right=True)
         if kind == "log":
             u = u + (delta < 0) * half
     if case["chains"] > 1:
