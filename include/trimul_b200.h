@@ -327,6 +327,115 @@ int trimul_b200_forward_static(const trimul_desc* desc, const void* z, const uin
                                const trimul_weights* w, void* out, const void* residual,
                                void* stream, int32_t* status);
 
+/*
+ * ------------------------------------------------------------------------------------------------
+ * Operators beside the block: the learned relative position bias by buckets and cross attention.
+ * Both have no counterpart among the reference's public kernels under these names; the conventions at the
+ * top of this file hold (nothing allocates, synchronises or throws; caller-owned buffers; captured in
+ * CUDA graphs without restriction).
+ * ------------------------------------------------------------------------------------------------
+ */
+
+/*
+ * Rule that maps a distance d = q_pos - k_pos to a bucket.
+ *   CLIPPED  clip(d, -r, r) + r with r = max_distance; count = 2 r + 1
+ *   LOG      count / 2 buckets for d >= 0 and as many for d < 0 (these after those); of |d|: exact below
+ *            near = count / 4, then `n_thresholds` thresholds, ascending: near + (thresholds reached)
+ *   CAUSAL   the same of max(d, 0) over all `count` buckets, near = count / 2
+ * `segments` != 0: positions of different segments take the bucket `count`, and the table has count + 1 rows.
+ */
+#define TRIMUL_BUCKETS_CLIPPED 0
+#define TRIMUL_BUCKETS_LOG     1
+#define TRIMUL_BUCKETS_CAUSAL  2
+#define TRIMUL_MAX_THRESHOLDS  250
+#define TRIMUL_MAX_BUCKETS     1024       /* rows of the table                                        */
+#define TRIMUL_MAX_LUT         8192       /* largest distance with a bucket of its own                */
+typedef struct trimul_buckets {
+    int32_t kind;
+    int32_t count;
+    int32_t max_distance;                 /* CLIPPED only                                             */
+    int32_t segments;
+    int32_t n_thresholds;
+    int32_t thresholds[TRIMUL_MAX_THRESHOLDS];
+} trimul_buckets;
+
+#define TRIMUL_RELPOS_HEADS 0             /* out[b,h,i,j] = table[u, h]; j contiguous                 */
+#define TRIMUL_RELPOS_PAIR  1             /* out[b,i,j,c] = add[b,i,j,c] + table[u, c]; dense         */
+typedef struct trimul_relpos_desc {
+    uint32_t struct_bytes;
+    int32_t  layout;
+    int32_t  dtype;                       /* of out, add and the upstream gradient                    */
+    int32_t  table_dtype;                 /* of the table and of its gradient                         */
+    int32_t  B, Lq, Lk;
+    int32_t  channels;                    /* heads or channels: columns of the table                  */
+    int32_t  wide_index;                  /* bit 0 q_pos, 1 k_pos, 2 q_seg, 3 k_seg: int64 instead of
+                                             int32.  Values of 2^30 and beyond are taken as 2^30 - 1   */
+    int32_t  reserved;
+    int64_t  q_pos_b, k_pos_b, q_seg_b, k_seg_b;   /* batch strides in elements, 0 where shared       */
+    int64_t  stride_b, stride_h, stride_i;         /* HEADS: of out or of the upstream gradient       */
+} trimul_relpos_desc;
+
+/*
+ * Forward.  table [rows, channels] dense; out (and add, PAIR only, may be NULL): see the layout; q_seg and
+ * k_seg NULL unless buckets->segments.  HEADS: out is 16-byte aligned, its strides are multiples of 16 bytes,
+ * and a row's storage reaches to the next multiple of 16 bytes behind Lk (those elements are written too).
+ */
+int trimul_b200_relpos_bias(const trimul_relpos_desc* desc, const trimul_buckets* buckets, const void* table,
+                            const void* q_pos, const void* k_pos, const void* q_seg, const void* k_seg,
+                            const void* add, void* out, void* stream);
+/*
+ * Gradient of the table: dtable[u, c] = sum of grad over all positions of bucket u, in fp32 and in a fixed
+ * order (the same bits every time), rounded once to table_dtype.  HEADS: grad may have any strides with j
+ * contiguous; PAIR: dense.
+ */
+int trimul_b200_relpos_bias_grad_workspace_bytes(const trimul_relpos_desc* desc, const trimul_buckets* buckets,
+                                                 size_t* bytes);
+int trimul_b200_relpos_bias_grad(const trimul_relpos_desc* desc, const trimul_buckets* buckets,
+                                 const void* q_pos, const void* k_pos, const void* q_seg, const void* k_seg,
+                                 const void* grad, void* dtable, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+
+/* A [B, L, heads, D] tensor; strides in elements, D contiguous. */
+typedef struct trimul_attn_tensor {
+    void*   p;
+    int64_t b, l, h;
+} trimul_attn_tensor;
+
+/*
+ * Cross attention of Lq queries to Lk keys: o_i = sum_j softmax_j(scale q_i.k_j + bias_ij) v_j over the
+ * kept keys.  Hk key heads serve H query heads, H / Hk consecutive ones each.  A row without a kept key
+ * gives zeros, and zero gradients.  Masked keys and values may hold anything, NaN included.
+ */
+#define TRIMUL_ATTN_FLAG_PLAIN 1u         /* the CUDA-core kernels also where tensor-core ones exist  */
+typedef struct trimul_attn_desc {
+    uint32_t struct_bytes;
+    int32_t  dtype;                       /* of every tensor: TRIMUL_DTYPE_*                          */
+    int32_t  B, Lq, Lk, H, Hk, D;         /* D at most 256                                            */
+    float    scale;
+    uint32_t flags;
+    trimul_attn_tensor q, k, v, o;        /* o: written by forward, read by backward                  */
+    trimul_attn_tensor dout, dq, dk, dv;  /* backward                                                 */
+    const void* bias;                     /* NULL or [bias_batch, bias_heads, Lq, Lk], j contiguous   */
+    int64_t  bias_b, bias_h, bias_i;
+    int32_t  bias_batch, bias_heads;      /* 1 (serves all), or B / H                                 */
+    const uint8_t* mask;                  /* NULL or [B, Lk] bytes, mask_b apart; 0 = masked          */
+    int64_t  mask_b;
+    float*   stats;                       /* [B, H, Lq, 2]: row maximum and log2 of the row's sum;
+                                             forward: may be NULL; backward: what forward wrote       */
+    void*    o_lo;                        /* bf16 only, [B, Lq, H, D] dense: the rounding of o; may be
+                                             NULL in forward; backward: what forward wrote, or NULL   */
+    void*    dbias;                       /* NULL, or the gradient of the bias, [bias_batch,
+                                             bias_heads, Lq, Lk]; rows start at multiples of 16 bytes
+                                             and their storage reaches to the next multiple behind Lk */
+    int64_t  dbias_b, dbias_h, dbias_i;
+} trimul_attn_desc;
+
+int trimul_b200_attn_workspace_bytes(const trimul_attn_desc* desc, int32_t backward, size_t* bytes);
+int trimul_b200_attn_forward(const trimul_attn_desc* desc, void* workspace, size_t workspace_bytes,
+                             void* stream, int32_t* status);
+int trimul_b200_attn_backward(const trimul_attn_desc* desc, void* workspace, size_t workspace_bytes,
+                              void* stream, int32_t* status);
+
 #ifdef __cplusplus
 }
 #endif

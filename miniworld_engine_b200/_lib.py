@@ -42,7 +42,18 @@ EXPORTED_SYMBOLS = (
     "trimul_b200_contract_scatter",
     "trimul_b200_peer_barrier",
     "trimul_b200_selftest_expiring_wait",
+    "trimul_b200_relpos_bias",
+    "trimul_b200_relpos_bias_grad_workspace_bytes",
+    "trimul_b200_relpos_bias_grad",
+    "trimul_b200_attn_workspace_bytes",
+    "trimul_b200_attn_forward",
+    "trimul_b200_attn_backward",
 )
+
+BUCKETS_CLIPPED, BUCKETS_LOG, BUCKETS_CAUSAL = 0, 1, 2
+MAX_THRESHOLDS, MAX_BUCKETS, MAX_LUT = 250, 1024, 8192
+RELPOS_HEADS, RELPOS_PAIR = 0, 1
+ATTN_FLAG_PLAIN = 1
 
 
 class Desc(C.Structure):
@@ -66,6 +77,31 @@ class Weights(C.Structure):
 class Planes(C.Structure):
     _fields_ = [("base", C.c_void_p)] + [(n, C.c_int64) for n in (
         "rows", "cols", "pitch", "plane_stride", "chunk_stride", "row_chunk", "col_chunk")]
+
+
+class Buckets(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("kind", "count", "max_distance", "segments", "n_thresholds")] + [
+        ("thresholds", C.c_int32 * MAX_THRESHOLDS)]
+
+
+class RelposDesc(C.Structure):
+    _fields_ = [("struct_bytes", C.c_uint32)] + [(n, C.c_int32) for n in (
+        "layout", "dtype", "table_dtype", "B", "Lq", "Lk", "channels", "wide_index", "reserved")] + [
+        (n, C.c_int64) for n in ("q_pos_b", "k_pos_b", "q_seg_b", "k_seg_b", "stride_b", "stride_h", "stride_i")]
+
+
+class AttnTensor(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("b", C.c_int64), ("l", C.c_int64), ("h", C.c_int64)]
+
+
+class AttnDesc(C.Structure):
+    _fields_ = [("struct_bytes", C.c_uint32)] + [(n, C.c_int32) for n in ("dtype", "B", "Lq", "Lk", "H", "Hk", "D")] + [
+        ("scale", C.c_float), ("flags", C.c_uint32)] + [
+        (n, AttnTensor) for n in ("q", "k", "v", "o", "dout", "dq", "dk", "dv")] + [
+        ("bias", C.c_void_p), ("bias_b", C.c_int64), ("bias_h", C.c_int64), ("bias_i", C.c_int64),
+        ("bias_batch", C.c_int32), ("bias_heads", C.c_int32), ("mask", C.c_void_p), ("mask_b", C.c_int64),
+        ("stats", C.c_void_p), ("o_lo", C.c_void_p), ("dbias", C.c_void_p),
+        ("dbias_b", C.c_int64), ("dbias_h", C.c_int64), ("dbias_i", C.c_int64)]
 
 
 class TrimulLibraryError(RuntimeError):
@@ -119,6 +155,16 @@ def load():
                                              C.c_void_p, C.c_void_p]
     lib.trimul_b200_selftest_expiring_wait.restype = C.c_int
     lib.trimul_b200_selftest_expiring_wait.argtypes = [C.c_uint32, C.c_void_p, C.c_void_p]
+    PR, PB, PA, V = C.POINTER(RelposDesc), C.POINTER(Buckets), C.POINTER(AttnDesc), C.c_void_p
+    for name, args in (
+            ("trimul_b200_relpos_bias", [PR, PB, V, V, V, V, V, V, V, V]),
+            ("trimul_b200_relpos_bias_grad_workspace_bytes", [PR, PB, C.POINTER(C.c_size_t)]),
+            ("trimul_b200_relpos_bias_grad", [PR, PB, V, V, V, V, V, V, V, C.c_size_t, V]),
+            ("trimul_b200_attn_workspace_bytes", [PA, C.c_int32, C.POINTER(C.c_size_t)]),
+            ("trimul_b200_attn_forward", [PA, V, C.c_size_t, V, V]),
+            ("trimul_b200_attn_backward", [PA, V, C.c_size_t, V, V])):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = C.c_int, args
     if lib.trimul_b200_abi_version() != ABI_VERSION:
         raise TrimulLibraryError(
             f"ABI mismatch: library {lib.trimul_b200_abi_version()}, binding {ABI_VERSION}; rebuild the library")
@@ -143,6 +189,16 @@ def check(code: int, what: str) -> None:
     if code == E_INVALID:
         raise ValueError(msg)
     raise TrimulLibraryError(msg)
+
+
+def dtype_code(dtype) -> int:
+    """``TRIMUL_DTYPE_*`` of a torch dtype."""
+    name = str(dtype)
+    if name == "torch.bfloat16":
+        return DTYPE_BF16
+    if name == "torch.float32":
+        return DTYPE_FP32
+    raise NotImplementedError(f"trimul_b200 supports torch.bfloat16 and torch.float32, got {dtype}")
 
 
 def make_desc(B, N, c, *, dtype, direction, mask_kind=MASK_NONE, eps_in=1e-5, eps_out=1e-5,

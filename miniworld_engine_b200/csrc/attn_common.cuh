@@ -1,0 +1,49 @@
+// Cross attention: what its kernels share.
+//
+//   x_ij = scale q_i . k_j + bias_ij   over the kept keys j,   p_ij = exp(x_ij - m_i) / l_i,   o_i = sum_j p_ij v_j
+//
+// with m_i the row's maximum and l_i the sum of exp(x_ij - m_i).  A row without a kept key gives o_i = 0 and zero
+// gradients.  Statistics of a row are kept as the pair (m_i, log2 l_i) rather than their sum: a mask of the type's lowest
+// value (-3.4e38) on a whole row would swallow log l_i, and every probability would come back as 1.  For the same reason
+// x - m is formed before it is scaled to base 2 wherever a bias takes part.
+#pragma once
+
+#include "../../include/trimul_b200.h"
+#include "ptx_sm100.cuh"
+
+namespace trimul {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Strides in elements; the head dimension is contiguous.
+struct AttnTensor {
+    void* p;
+    long long b, l, h;
+};
+struct AttnParams {
+    int B, Lq, Lk, H, Hk, D;
+    float scale;
+    AttnTensor q, k, v, o, dout, dq, dk, dv;
+    const void* bias;                      // null, or strides below (0 where one bias serves several)
+    long long bias_b, bias_h, bias_i;
+    const uint8_t* mask;                   // null, or [B] rows of Lk bytes, mask_b apart; 0 = masked key
+    long long mask_b;
+    float2* stats;                         // [B][H][Lq]: (m, log2 l); (0, +inf) for a row without keys
+    void* o_lo;                            // [B][Lq][H][D]: what rounding o to 16 bits left over, or null
+    float* delta;                          // [B][H][Lq]: sum_d dout o
+    void* ds;                              // gradient of x, or null: written with the strides below
+    long long ds_b, ds_h, ds_i;
+    int32_t* status;
+};
+
+__device__ __forceinline__ float at_float(float v) { return v; }
+__device__ __forceinline__ float at_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void at_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void at_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ float ex2f(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+}  // namespace trimul

@@ -1,0 +1,416 @@
+// Cross attention on the CUDA cores: fp32 inputs, head dimensions that the tensor-core kernels do not take, and the
+// cross-check of those kernels.  All arithmetic in fp32.
+//
+// A block owns kT rows of queries (forward, gradient of q and of the bias) or of keys (gradients of k and v) and walks
+// over tiles of kT rows of the other side.  256 threads as 16 x 16; thread (ty, tx) owns rows ty * kR + r and columns
+// tx + 16 c of a kT x kT tile of scores, r, c < kR = kT / 16, both operands read from shared memory in four-element
+// pieces along the head dimension (pitch D rounded up to 4, plus 4: the sixteen rows that a half warp reads at once then
+// lie in different banks).  What bounds it is the shared-memory pipe: 2 kR reads of 16 bytes for 4 kR^2 multiply-adds.
+#pragma once
+
+#include "attn_common.cuh"
+
+namespace trimul {
+
+constexpr int kApThreads = 256;
+
+__host__ __device__ inline int ap_pitch(int D) { return (D + 3) / 4 * 4 + 4; }
+template <int kT> __host__ __device__ inline int ap_ppitch() { return kT + 4; }
+// `tiles` operand tiles and `scores` score tiles of shared memory
+template <int kT> inline int ap_smem(int D, int tiles, int scores) {
+    return (tiles * kT * ap_pitch(D) + scores * kT * ap_ppitch<kT>() + 3 * kT) * 4;
+}
+
+// kT rows of a tensor into shared memory as fp32, zeros behind the last row, in masked rows and behind column D.
+template <typename T, int kT>
+__device__ __forceinline__ void ap_load(float* dst, const T* src, long long stride, int row0, int rows, int D,
+                                        const uint8_t* keep) {
+    const int pitch = ap_pitch(D), cols = pitch - 4;
+    for (int e = threadIdx.x; e < kT * cols; e += kApThreads) {
+        const int r = e / cols, d = e - r * cols;
+        const bool in = row0 + r < rows && d < D && (keep == nullptr || keep[row0 + r] != 0);
+        dst[r * pitch + d] = in ? at_float(src[(long long)(row0 + r) * stride + d]) : 0.f;
+    }
+}
+
+// acc[r][c] = A[ty kR + r] . B[tx + 16 c]
+template <int kR>
+__device__ __forceinline__ void ap_dot(float (&acc)[kR][kR], const float* A, const float* B, int D, int ty, int tx) {
+    const int pitch = ap_pitch(D);
+#pragma unroll
+    for (int r = 0; r < kR; ++r)
+#pragma unroll
+        for (int c = 0; c < kR; ++c) acc[r][c] = 0.f;
+    for (int d = 0; d < D; d += 4) {
+        float4 a[kR], b[kR];
+#pragma unroll
+        for (int r = 0; r < kR; ++r) a[r] = *reinterpret_cast<const float4*>(A + (ty * kR + r) * pitch + d);
+#pragma unroll
+        for (int c = 0; c < kR; ++c) b[c] = *reinterpret_cast<const float4*>(B + (tx + 16 * c) * pitch + d);
+#pragma unroll
+        for (int r = 0; r < kR; ++r)
+#pragma unroll
+            for (int c = 0; c < kR; ++c) {
+                acc[r][c] = fmaf(a[r].x, b[c].x, acc[r][c]);
+                acc[r][c] = fmaf(a[r].y, b[c].y, acc[r][c]);
+                acc[r][c] = fmaf(a[r].z, b[c].z, acc[r][c]);
+                acc[r][c] = fmaf(a[r].w, b[c].w, acc[r][c]);
+            }
+    }
+}
+// out[r][c] += sum_j P[ty kR + r][j] X[j][tx + 16 c], c < kC
+template <int kT, int kR, int kC>
+__device__ __forceinline__ void ap_mix(float (&out)[kR][kC], const float* P, const float* X, int D, int ty, int tx) {
+    const int pitch = ap_pitch(D), pp = ap_ppitch<kT>();
+    for (int j = 0; j < kT; j += 4) {
+        float4 a[kR];
+#pragma unroll
+        for (int r = 0; r < kR; ++r) a[r] = *reinterpret_cast<const float4*>(P + (ty * kR + r) * pp + j);
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            const int d = tx + 16 * c;
+            if (d >= D) break;
+            const float x0 = X[j * pitch + d], x1 = X[(j + 1) * pitch + d], x2 = X[(j + 2) * pitch + d],
+                        x3 = X[(j + 3) * pitch + d];
+#pragma unroll
+            for (int r = 0; r < kR; ++r) {
+                out[r][c] = fmaf(a[r].x, x0, out[r][c]);
+                out[r][c] = fmaf(a[r].y, x1, out[r][c]);
+                out[r][c] = fmaf(a[r].z, x2, out[r][c]);
+                out[r][c] = fmaf(a[r].w, x3, out[r][c]);
+            }
+        }
+    }
+}
+// Largest and sum over the sixteen threads of a row (a half warp).
+__device__ __forceinline__ float ap_row_max(float v) {
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float ap_row_sum(float v) {
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Scores of a tile: scale and bias, -inf at masked keys and behind the last one.
+template <typename T, int kR>
+__device__ __forceinline__ void ap_scores(float (&s)[kR][kR], const AttnParams& p, int b, int h, int i0, int j0, int ty, int tx) {
+    const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
+    const T* bias = p.bias != nullptr ? static_cast<const T*>(p.bias) + b * p.bias_b + h * p.bias_h : nullptr;
+#pragma unroll
+    for (int c = 0; c < kR; ++c) {
+        const int j = j0 + tx + 16 * c;
+        const bool kept = j < p.Lk && (keep == nullptr || keep[j] != 0);
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+            const int i = i0 + ty * kR + r;
+            s[r][c] = !kept ? -INFINITY
+                            : fmaf(s[r][c], p.scale, bias != nullptr && i < p.Lq ? at_float(bias[i * p.bias_i + j]) : 0.f);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// forward: grid (query tiles, H, B)
+// ---------------------------------------------------------------------------------------
+template <typename T, int kT, int kC>
+__global__ void __launch_bounds__(kApThreads) attn_plain_fwd_kernel(const __grid_constant__ AttnParams p) {
+    constexpr int kR = kT / 16;
+    extern __shared__ __align__(16) float sm[];
+    const int pitch = ap_pitch(p.D), pp = ap_ppitch<kT>();
+    float *Q = sm, *K = Q + kT * pitch, *V = K + kT * pitch, *P = V + kT * pitch;
+    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+    const int i0 = blockIdx.x * kT, h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hk);
+    griddep_wait();
+    griddep_launch_dependents();
+    const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
+    const T* k = static_cast<const T*>(p.k.p) + b * p.k.b + hk * p.k.h;
+    const T* v = static_cast<const T*>(p.v.p) + b * p.v.b + hk * p.v.h;
+    ap_load<T, kT>(Q, static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h, p.q.l, i0, p.Lq, p.D, nullptr);
+    float o[kR][kC], m[kR], l[kR];
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < kC; ++c) o[r][c] = 0.f;
+    }
+    for (int j0 = 0; j0 < p.Lk; j0 += kT) {
+        __syncthreads();
+        ap_load<T, kT>(K, k, p.k.l, j0, p.Lk, p.D, keep);
+        ap_load<T, kT>(V, v, p.v.l, j0, p.Lk, p.D, keep);
+        __syncthreads();
+        float s[kR][kR];
+        ap_dot<kR>(s, Q, K, p.D, ty, tx);
+        ap_scores<T, kR>(s, p, b, h, i0, j0, ty, tx);
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+            float mx = s[r][0];
+#pragma unroll
+            for (int c = 1; c < kR; ++c) mx = fmaxf(mx, s[r][c]);
+            const float mn = fmaxf(m[r], ap_row_max(mx));
+            const float base = mn == -INFINITY ? 0.f : mn;
+            const float corr = exp2f((m[r] - base) * kLog2e);
+            m[r] = mn;
+            float t = 0.f;
+#pragma unroll
+            for (int c = 0; c < kR; ++c) {
+                const float e = exp2f((s[r][c] - base) * kLog2e);
+                t += e;
+                P[(ty * kR + r) * pp + tx + 16 * c] = e;
+            }
+            l[r] = l[r] * corr + ap_row_sum(t);
+#pragma unroll
+            for (int c = 0; c < kC; ++c) o[r][c] *= corr;
+        }
+        __syncwarp();            // a row's probabilities are written and read by the same half warp
+        ap_mix<kT, kR, kC>(o, P, V, p.D, ty, tx);
+    }
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+        const int i = i0 + ty * kR + r;
+        if (i >= p.Lq) continue;
+        const bool empty = m[r] == -INFINITY;
+        const float inv = empty ? 0.f : 1.f / l[r];
+        T* dst = static_cast<T*>(p.o.p) + b * p.o.b + (long long)i * p.o.l + h * p.o.h;
+        const long long lo = (((long long)b * p.Lq + i) * p.H + h) * p.D;
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            const int d = tx + 16 * c;
+            if (d >= p.D) break;
+            const float y = empty ? 0.f : o[r][c] * inv;
+            at_store(dst + d, y);
+            if constexpr (sizeof(T) == 2) {
+                if (p.o_lo != nullptr) {
+                    const float rest = y - __bfloat162float(__float2bfloat16_rn(y));
+                    static_cast<__nv_bfloat16*>(p.o_lo)[lo + d] = __float2bfloat16_rn(rest);
+                }
+            }
+        }
+        if (tx == 0 && p.stats != nullptr)
+            p.stats[((long long)b * p.H + h) * p.Lq + i] = empty ? make_float2(0.f, INFINITY) : make_float2(m[r], log2f(l[r]));
+    }
+}
+
+// delta_i = sum_d dout_id o_id, a warp per row.  With 16-bit outputs the part that rounding took off o is added back:
+// where the probabilities' gradients nearly cancel against delta, half a step of o would be all that is left.
+template <typename T>
+__global__ void __launch_bounds__(kApThreads) attn_delta_kernel(const __grid_constant__ AttnParams p) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const long long row = (long long)blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5);
+    if (row >= (long long)p.B * p.Lq * p.H) return;
+    const int lane = threadIdx.x & 31;
+    const int h = (int)(row % p.H);
+    const long long bi = row / p.H;
+    const int i = (int)(bi % p.Lq), b = (int)(bi / p.Lq);
+    const T* o = static_cast<const T*>(p.o.p) + b * p.o.b + (long long)i * p.o.l + h * p.o.h;
+    const T* g = static_cast<const T*>(p.dout.p) + b * p.dout.b + (long long)i * p.dout.l + h * p.dout.h;
+    float t = 0.f;
+    for (int d = lane; d < p.D; d += 32) {
+        float y = at_float(o[d]);
+        if constexpr (sizeof(T) == 2) {
+            if (p.o_lo != nullptr) y += __bfloat162float(static_cast<const __nv_bfloat16*>(p.o_lo)[row * p.D + d]);
+        }
+        t = fmaf(y, at_float(g[d]), t);
+    }
+#pragma unroll
+    for (int s = 16; s >= 1; s >>= 1) t += __shfl_xor_sync(0xffffffffu, t, s);
+    if (lane == 0) p.delta[((long long)b * p.H + h) * p.Lq + i] = t;
+}
+
+// Probabilities and score gradients of a tile from its scores s and products g = dout . v.
+template <int kR>
+__device__ __forceinline__ void ap_probs(float (&s)[kR][kR], float (&g)[kR][kR], const AttnParams& p, int b, int h, int i0, int ty) {
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+        const int i = i0 + ty * kR + r;
+        float2 st = make_float2(0.f, INFINITY);
+        float delta = 0.f;
+        if (i < p.Lq) {
+            st = p.stats[((long long)b * p.H + h) * p.Lq + i];
+            delta = p.delta[((long long)b * p.H + h) * p.Lq + i];
+        }
+#pragma unroll
+        for (int c = 0; c < kR; ++c) {
+            const float e = exp2f(fmaf(s[r][c] - st.x, kLog2e, -st.y));
+            s[r][c] = e;
+            g[r][c] = e == 0.f ? 0.f : e * (g[r][c] - delta);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// gradient of q, and of the scores where the bias wants one: grid (query tiles, H, B)
+// ---------------------------------------------------------------------------------------
+template <typename T, int kT, int kC>
+__global__ void __launch_bounds__(kApThreads) attn_plain_dq_kernel(const __grid_constant__ AttnParams p) {
+    constexpr int kR = kT / 16;
+    extern __shared__ __align__(16) float sm[];
+    const int pitch = ap_pitch(p.D), pp = ap_ppitch<kT>();
+    float *Q = sm, *G = Q + kT * pitch, *K = G + kT * pitch, *V = K + kT * pitch, *P = V + kT * pitch;
+    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+    const int i0 = blockIdx.x * kT, h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hk);
+    griddep_wait();
+    griddep_launch_dependents();
+    const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
+    const T* k = static_cast<const T*>(p.k.p) + b * p.k.b + hk * p.k.h;
+    const T* v = static_cast<const T*>(p.v.p) + b * p.v.b + hk * p.v.h;
+    ap_load<T, kT>(Q, static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h, p.q.l, i0, p.Lq, p.D, nullptr);
+    ap_load<T, kT>(G, static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h, p.dout.l, i0, p.Lq, p.D, nullptr);
+    float o[kR][kC];
+#pragma unroll
+    for (int r = 0; r < kR; ++r)
+#pragma unroll
+        for (int c = 0; c < kC; ++c) o[r][c] = 0.f;
+    for (int j0 = 0; j0 < p.Lk; j0 += kT) {
+        __syncthreads();
+        ap_load<T, kT>(K, k, p.k.l, j0, p.Lk, p.D, keep);
+        ap_load<T, kT>(V, v, p.v.l, j0, p.Lk, p.D, keep);
+        __syncthreads();
+        float s[kR][kR], g[kR][kR];
+        ap_dot<kR>(s, Q, K, p.D, ty, tx);
+        ap_scores<T, kR>(s, p, b, h, i0, j0, ty, tx);
+        ap_dot<kR>(g, G, V, p.D, ty, tx);
+        ap_probs<kR>(s, g, p, b, h, i0, ty);
+#pragma unroll
+        for (int r = 0; r < kR; ++r) {
+            const int i = i0 + ty * kR + r;
+#pragma unroll
+            for (int c = 0; c < kR; ++c) {
+                const int j = j0 + tx + 16 * c;
+                P[(ty * kR + r) * pp + tx + 16 * c] = g[r][c];
+                if (p.ds != nullptr && i < p.Lq && j < p.Lk)
+                    at_store(static_cast<T*>(p.ds) + b * p.ds_b + h * p.ds_h + i * p.ds_i + j, g[r][c]);
+            }
+        }
+        __syncwarp();
+        ap_mix<kT, kR, kC>(o, P, K, p.D, ty, tx);
+    }
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+        const int i = i0 + ty * kR + r;
+        if (i >= p.Lq) continue;
+        T* dst = static_cast<T*>(p.dq.p) + b * p.dq.b + (long long)i * p.dq.l + h * p.dq.h;
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            const int d = tx + 16 * c;
+            if (d >= p.D) break;
+            at_store(dst + d, o[r][c] * p.scale);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// gradients of k and v: grid (key tiles, Hk, B); the query heads that share the key head are summed here
+// ---------------------------------------------------------------------------------------
+template <typename T, int kT, int kC>
+__global__ void __launch_bounds__(kApThreads) attn_plain_dkv_kernel(const __grid_constant__ AttnParams p) {
+    constexpr int kR = kT / 16;
+    extern __shared__ __align__(16) float sm[];
+    const int pitch = ap_pitch(p.D), pp = ap_ppitch<kT>();
+    float *Q = sm, *G = Q + kT * pitch, *K = G + kT * pitch, *V = K + kT * pitch, *P = V + kT * pitch, *S = P + kT * pp;
+    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+    const int j0 = blockIdx.x * kT, hk = blockIdx.y, b = blockIdx.z, group = p.H / p.Hk;
+    griddep_wait();
+    griddep_launch_dependents();
+    const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
+    ap_load<T, kT>(K, static_cast<const T*>(p.k.p) + b * p.k.b + hk * p.k.h, p.k.l, j0, p.Lk, p.D, keep);
+    ap_load<T, kT>(V, static_cast<const T*>(p.v.p) + b * p.v.b + hk * p.v.h, p.v.l, j0, p.Lk, p.D, keep);
+    float dk[kR][kC], dv[kR][kC];
+#pragma unroll
+    for (int r = 0; r < kR; ++r)
+#pragma unroll
+        for (int c = 0; c < kC; ++c) dk[r][c] = dv[r][c] = 0.f;
+    for (int h = hk * group; h < (hk + 1) * group; ++h) {
+        const T* q = static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h;
+        const T* go = static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h;
+        for (int i0 = 0; i0 < p.Lq; i0 += kT) {
+            __syncthreads();
+            ap_load<T, kT>(Q, q, p.q.l, i0, p.Lq, p.D, nullptr);
+            ap_load<T, kT>(G, go, p.dout.l, i0, p.Lq, p.D, nullptr);
+            __syncthreads();
+            float s[kR][kR], g[kR][kR];
+            ap_dot<kR>(s, Q, K, p.D, ty, tx);
+            ap_scores<T, kR>(s, p, b, h, i0, j0, ty, tx);
+            ap_dot<kR>(g, G, V, p.D, ty, tx);
+            ap_probs<kR>(s, g, p, b, h, i0, ty);
+#pragma unroll
+            for (int r = 0; r < kR; ++r)
+#pragma unroll
+                for (int c = 0; c < kR; ++c) {          // transposed: rows of keys
+                    P[(tx + 16 * c) * pp + ty * kR + r] = s[r][c];
+                    S[(tx + 16 * c) * pp + ty * kR + r] = g[r][c];
+                }
+            __syncthreads();
+            ap_mix<kT, kR, kC>(dv, P, G, p.D, ty, tx);
+            ap_mix<kT, kR, kC>(dk, S, Q, p.D, ty, tx);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kR; ++r) {
+        const int j = j0 + ty * kR + r;
+        if (j >= p.Lk) continue;
+        const bool kept = keep == nullptr || keep[j] != 0;     // zero whatever the upstream gradient holds
+        T* dkp = static_cast<T*>(p.dk.p) + b * p.dk.b + (long long)j * p.dk.l + hk * p.dk.h;
+        T* dvp = static_cast<T*>(p.dv.p) + b * p.dv.b + (long long)j * p.dv.l + hk * p.dv.h;
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+            const int d = tx + 16 * c;
+            if (d >= p.D) break;
+            at_store(dkp + d, kept ? dk[r][c] * p.scale : 0.f);
+            at_store(dvp + d, kept ? dv[r][c] : 0.f);
+        }
+    }
+}
+
+// Gradient of a bias that serves several batch elements or heads: the scores' gradients [B][H][Lq][pitch] summed over
+// the broadcast axes, in fp32 and in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(kApThreads)
+attn_bias_sum_kernel(const T* ds, long long ds_b, long long ds_h, long long ds_i, T* out, long long out_b, long long out_h,
+                     long long out_i, int B, int H, int Lq, int Lk, int sum_b, int sum_h) {
+    constexpr int kN = 16 / (int)sizeof(T);
+    griddep_wait();
+    griddep_launch_dependents();
+    const int nch = (Lk + kN - 1) / kN;
+    const int ob = sum_b ? 1 : B, oh = sum_h ? 1 : H;
+    const long long items = (long long)ob * oh * Lq * nch;
+    for (long long it = (long long)blockIdx.x * kApThreads + threadIdx.x; it < items; it += (long long)gridDim.x * kApThreads) {
+        const int c = (int)(it % nch);
+        const long long r = it / nch;
+        const int i = (int)(r % Lq);
+        const int x = (int)(r / Lq);
+        const int h0 = x % oh, b0 = x / oh;
+        float acc[kN];
+#pragma unroll
+        for (int e = 0; e < kN; ++e) acc[e] = 0.f;
+        const int nb = sum_b ? B : 1, nh = sum_h ? H : 1;
+#pragma unroll 4
+        for (int s = 0; s < nb * nh; ++s) {
+            const int b = b0 + s / nh, h = h0 + s % nh;
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(ds + b * ds_b + h * ds_h + i * ds_i) + c);
+            if constexpr (sizeof(T) == 2) {
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    acc[2 * e] += bf16_lo(w[e]);
+                    acc[2 * e + 1] += bf16_hi(w[e]);
+                }
+            } else {
+                acc[0] += __uint_as_float(v.x); acc[1] += __uint_as_float(v.y);
+                acc[2] += __uint_as_float(v.z); acc[3] += __uint_as_float(v.w);
+            }
+        }
+        uint4 v;
+        if constexpr (sizeof(T) == 2)
+            v = make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]), pack_bf16x2(acc[4], acc[5]), pack_bf16x2(acc[6], acc[7]));
+        else
+            v = make_uint4(__float_as_uint(acc[0]), __float_as_uint(acc[1]), __float_as_uint(acc[2]), __float_as_uint(acc[3]));
+        *(reinterpret_cast<uint4*>(out + b0 * out_b + h0 * out_h + i * out_i) + c) = v;
+    }
+}
+
+}  // namespace trimul

@@ -1,0 +1,375 @@
+// C-ABI of the operators beside the block: the relative position bias by buckets and cross attention.  Argument
+// checks, choice of kernel and launches; declarations in include/trimul_b200.h.  Nothing here allocates device
+// memory, synchronises or throws.
+
+#include "../../include/trimul_b200.h"
+
+#include <algorithm>
+#include <cstddef>
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "host_common.cuh"
+#include "attn_plain.cuh"
+#include "relpos_kernels.cuh"
+
+using namespace trimul;
+
+namespace {
+
+constexpr int kMaxSmem = 227 * 1024;
+inline bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t align_up(int64_t v, int64_t m) { return ceil_div(v, m) * m; }
+inline int elem_size(int dtype) { return dtype == TRIMUL_DTYPE_BF16 ? 2 : 4; }
+inline bool known_dtype(int d) { return d == TRIMUL_DTYPE_BF16 || d == TRIMUL_DTYPE_FP32; }
+
+// ---------------------------------------------------------------------------------------
+// relative position bias
+// ---------------------------------------------------------------------------------------
+int lut_reach(const trimul_buckets* b) {       // distances beyond it share the outermost buckets
+    if (b->kind == TRIMUL_BUCKETS_CLIPPED) return b->max_distance;
+    const int near = b->kind == TRIMUL_BUCKETS_LOG ? b->count / 4 : b->count / 2;
+    return b->n_thresholds > 0 ? b->thresholds[b->n_thresholds - 1] : near;
+}
+
+int check_buckets(const trimul_buckets* b) {
+    if (b == nullptr || b->count <= 0) return TRIMUL_E_INVALID;
+    if (b->kind == TRIMUL_BUCKETS_CLIPPED) {
+        if (b->max_distance < 0 || (int64_t)b->count != 2 * (int64_t)b->max_distance + 1) return TRIMUL_E_INVALID;
+    } else if (b->kind == TRIMUL_BUCKETS_LOG || b->kind == TRIMUL_BUCKETS_CAUSAL) {
+        if (b->kind == TRIMUL_BUCKETS_LOG && (b->count % 2) != 0) return TRIMUL_E_INVALID;
+        const int half = b->kind == TRIMUL_BUCKETS_LOG ? b->count / 2 : b->count, near = half / 2;
+        if (near < 1 || b->n_thresholds < 0 || b->n_thresholds > TRIMUL_MAX_THRESHOLDS) return TRIMUL_E_INVALID;
+        if (near + b->n_thresholds > half - 1) return TRIMUL_E_INVALID;
+        for (int i = 0; i < b->n_thresholds; ++i)
+            if (b->thresholds[i] < (i == 0 ? near : b->thresholds[i - 1])) return TRIMUL_E_INVALID;
+    } else {
+        return TRIMUL_E_INVALID;
+    }
+    if ((int64_t)b->count + (b->segments != 0) > TRIMUL_MAX_BUCKETS) return TRIMUL_E_UNSUPPORTED;
+    if (lut_reach(b) > TRIMUL_MAX_LUT) return TRIMUL_E_UNSUPPORTED;
+    return TRIMUL_OK;
+}
+
+int check_relpos(const trimul_relpos_desc* d, const trimul_buckets* b) {
+    if (d == nullptr || d->struct_bytes != sizeof(trimul_relpos_desc)) return TRIMUL_E_INVALID;
+    const int rc = check_buckets(b);
+    if (rc != TRIMUL_OK) return rc;
+    if (d->layout != TRIMUL_RELPOS_HEADS && d->layout != TRIMUL_RELPOS_PAIR) return TRIMUL_E_INVALID;
+    if (!known_dtype(d->dtype) || !known_dtype(d->table_dtype)) return TRIMUL_E_INVALID;
+    if (d->B <= 0 || d->Lq <= 0 || d->Lk <= 0 || d->channels <= 0) return TRIMUL_E_INVALID;
+    if (d->wide_index < 0 || d->wide_index > 15) return TRIMUL_E_INVALID;
+    if (d->channels > 8192 || d->Lk > (1 << 24)) return TRIMUL_E_UNSUPPORTED;
+    if ((int64_t)d->B * d->Lq > (1 << 30)) return TRIMUL_E_UNSUPPORTED;
+    if (d->layout == TRIMUL_RELPOS_HEADS &&
+        (d->stride_b < 0 || d->stride_h < 0 || d->stride_i < 0)) return TRIMUL_E_INVALID;
+    return TRIMUL_OK;
+}
+
+RelposParams relpos_params(const trimul_relpos_desc* d, const trimul_buckets* b, const void* table, const void* q_pos,
+                           const void* k_pos, const void* q_seg, const void* k_seg) {
+    RelposParams p = {};
+    p.B = d->B; p.Lq = d->Lq; p.Lk = d->Lk; p.C = d->channels;
+    p.rows = b->count + (b->segments != 0);
+    p.M = lut_reach(b);
+    p.q_pos = q_pos; p.k_pos = k_pos;
+    if (b->segments != 0) { p.q_seg = q_seg; p.k_seg = k_seg; }
+    p.q_pos_b = d->q_pos_b; p.k_pos_b = d->k_pos_b; p.q_seg_b = d->q_seg_b; p.k_seg_b = d->k_seg_b;
+    p.q_pos64 = d->wide_index & 1; p.k_pos64 = (d->wide_index >> 1) & 1;
+    p.q_seg64 = (d->wide_index >> 2) & 1; p.k_seg64 = (d->wide_index >> 3) & 1;
+    p.table = table;
+    p.table_bf16 = d->table_dtype == TRIMUL_DTYPE_BF16;
+    p.sB = d->stride_b; p.sH = d->stride_h; p.sI = d->stride_i;
+    return p;
+}
+
+inline int lut_bytes(int M) { return (2 * M + 1) * 2; }
+
+template <typename T>
+int run_relpos_forward(const trimul_relpos_desc* d, const trimul_buckets* b, const RelposParams& p, const void* add,
+                       void* out, cudaStream_t st) {
+    constexpr int kN = RpVec<T>::kN;
+    if (d->layout == TRIMUL_RELPOS_HEADS) {
+        const int64_t items = (int64_t)d->B * d->Lq * ceil_div(d->Lk, kN);
+        const int groups = (int)ceil_div(d->channels, kN);
+        const int64_t blocks = std::min<int64_t>(ceil_div(items, kRpThreads), ceil_div(16 * (int64_t)sm_count(), groups));
+        const int smem = ((p.rows + 63) & ~63) * 16 + lut_bytes(p.M);
+        if (!ensure_smem(relpos_heads_kernel<T>, TRIMUL_MAX_BUCKETS * 16 + lut_bytes(TRIMUL_MAX_LUT))) return TRIMUL_E_CUDA;
+        return launch_stage(relpos_heads_kernel<T>, dim3((unsigned)blocks, (unsigned)groups), kRpThreads, smem, st, true, p, *b,
+                            static_cast<T*>(out));
+    }
+    // 16-byte pieces of channels where the tensors allow them
+    const bool vec = (d->channels % kN) == 0 && aligned(add, 16) && aligned(out, 16) && aligned(p.table, 16);
+    const int lanes = std::min(vec ? d->channels / kN : d->channels, kRpPairThreads), side = kRpPairThreads / lanes;
+    const int64_t total = (int64_t)d->B * d->Lq * d->Lk;
+    const int64_t per_block = align_up(std::max<int64_t>(ceil_div(total, 8 * (int64_t)sm_count()), 4 * side), 4 * side);
+    if (per_block > (1 << 30)) return TRIMUL_E_UNSUPPORTED;
+    const dim3 grid((unsigned)ceil_div(total, per_block));
+    auto kernel = vec ? relpos_pair_kernel<T, true> : relpos_pair_kernel<T, false>;
+    if (!ensure_smem(kernel, lut_bytes(TRIMUL_MAX_LUT))) return TRIMUL_E_CUDA;
+    return launch_stage(kernel, grid, kRpPairThreads, lut_bytes(p.M), st, true, p, *b, static_cast<const T*>(add),
+                        static_cast<T*>(out), (int)per_block);
+}
+
+// Launch shape of the gradient: `parts` partial tables of rows * channels sums each.
+struct RelposGradPlan {
+    int threads, smem, parts, lane_channels, column_blocks;
+    int64_t per_part;          // rows (heads) or positions of a warp (pair)
+};
+RelposGradPlan plan_relpos_grad(const trimul_relpos_desc* d, const trimul_buckets* b, bool wide_lanes) {
+    RelposGradPlan g = {};
+    const int rows = b->count + (b->segments != 0), lut = lut_bytes(lut_reach(b));
+    const int kN = d->dtype == TRIMUL_DTYPE_BF16 ? 8 : 4;
+    if (d->layout == TRIMUL_RELPOS_HEADS) {
+        g.threads = 128;
+        while (g.threads > 32 && rows * g.threads * 4 > 96 * 1024) g.threads /= 2;
+        g.smem = rows * g.threads * 4 + lut;
+        const int64_t all = (int64_t)d->B * d->Lq;
+        const int nch = (int)ceil_div(d->Lk, kN), side = std::max(1, g.threads / std::min(nch, g.threads));
+        int64_t parts = std::max<int64_t>(1, 4 * (int64_t)sm_count() / d->channels);
+        g.per_part = align_up(std::max<int64_t>(ceil_div(all, parts), 4 * side), side);
+        g.parts = (int)ceil_div(all, g.per_part);
+        return g;
+    }
+    const int64_t total = (int64_t)d->B * d->Lq * d->Lk;
+    g.lane_channels = wide_lanes && rows * 128 * 4 + lut <= kMaxSmem ? 4 : 1;
+    const int copy = rows * 32 * g.lane_channels * 4;
+    int warps = std::min(8, (kMaxSmem - lut) / copy);
+    g.threads = 32 * warps;
+    g.smem = warps * copy + lut;
+    g.column_blocks = (int)ceil_div(d->channels, 32 * g.lane_channels);
+    const int64_t blocks = std::max<int64_t>(1, sm_count() / g.column_blocks);
+    g.per_part = align_up(std::max<int64_t>(ceil_div(total, blocks * warps), 32), 32);
+    g.parts = (int)ceil_div(total, g.per_part * warps);
+    return g;
+}
+
+template <typename T>
+int run_relpos_grad(const trimul_relpos_desc* d, const trimul_buckets* b, const RelposParams& p, const void* grad,
+                    void* dtable, float* partial, cudaStream_t st) {
+    constexpr int kN = RpVec<T>::kN;
+    int rc;
+    const bool wide = (d->channels % 4) == 0 && aligned(grad, 4 * sizeof(T));
+    const RelposGradPlan g = plan_relpos_grad(d, b, wide);
+    if (d->layout == TRIMUL_RELPOS_HEADS) {
+        const bool vec = aligned(grad, 16) && (p.sB % kN) == 0 && (p.sH % kN) == 0 && (p.sI % kN) == 0;
+        auto kernel = vec ? relpos_heads_grad_kernel<T, true> : relpos_heads_grad_kernel<T, false>;
+        if (!ensure_smem(kernel, kMaxSmem)) return TRIMUL_E_CUDA;
+        rc = launch_stage(kernel, dim3((unsigned)g.parts, (unsigned)d->channels), g.threads, g.smem, st, true, p, *b,
+                          static_cast<const T*>(grad), partial, (int)g.per_part);
+    } else {
+        auto kernel = g.lane_channels == 4 ? relpos_pair_grad_kernel<T, 4> : relpos_pair_grad_kernel<T, 1>;
+        if (!ensure_smem(kernel, kMaxSmem)) return TRIMUL_E_CUDA;
+        rc = launch_stage(kernel, dim3((unsigned)g.parts, (unsigned)g.column_blocks), g.threads, g.smem, st, true, p, *b,
+                          static_cast<const T*>(grad), partial, (long long)g.per_part);
+    }
+    if (rc != TRIMUL_OK) return rc;
+    const int n = p.rows * p.C;
+    return launch_stage(relpos_reduce_kernel, dim3((unsigned)ceil_div(n, 32)), kRpReduceThreads, 0, st, true,
+                        static_cast<const float*>(partial), dtable, p.table_bf16, g.parts, n);
+}
+
+// ---------------------------------------------------------------------------------------
+// cross attention
+// ---------------------------------------------------------------------------------------
+int check_attn(const trimul_attn_desc* d) {
+    if (d == nullptr || d->struct_bytes != sizeof(trimul_attn_desc)) return TRIMUL_E_INVALID;
+    if (!known_dtype(d->dtype)) return TRIMUL_E_INVALID;
+    if (d->B <= 0 || d->Lq <= 0 || d->Lk <= 0 || d->H <= 0 || d->Hk <= 0 || d->D <= 0) return TRIMUL_E_INVALID;
+    if ((d->H % d->Hk) != 0) return TRIMUL_E_INVALID;
+    if (d->D > 256 || d->B > 65535 || d->H > 65535) return TRIMUL_E_UNSUPPORTED;
+    if (d->Lq > (1 << 24) || d->Lk > (1 << 24)) return TRIMUL_E_UNSUPPORTED;
+    if ((d->bias != nullptr || d->dbias != nullptr) &&
+        ((d->bias_batch != 1 && d->bias_batch != d->B) || (d->bias_heads != 1 && d->bias_heads != d->H)))
+        return TRIMUL_E_INVALID;
+    if (d->dbias != nullptr) {
+        const int n = 16 / elem_size(d->dtype);
+        if (d->bias == nullptr || !aligned(d->dbias, 16)) return TRIMUL_E_INVALID;
+        if ((d->dbias_b % n) || (d->dbias_h % n) || (d->dbias_i % n) || d->dbias_i < align_up(d->Lk, n)) return TRIMUL_E_INVALID;
+    }
+    return TRIMUL_OK;
+}
+inline bool sums_bias(const trimul_attn_desc* d) {
+    return d->dbias != nullptr && ((d->bias_batch == 1 && d->B > 1) || (d->bias_heads == 1 && d->H > 1));
+}
+inline AttnTensor tensor_of(const trimul_attn_tensor& t) { return AttnTensor{t.p, t.b, t.l, t.h}; }
+
+AttnParams attn_params(const trimul_attn_desc* d, int32_t* status) {
+    AttnParams p = {};
+    p.B = d->B; p.Lq = d->Lq; p.Lk = d->Lk; p.H = d->H; p.Hk = d->Hk; p.D = d->D;
+    p.scale = d->scale;
+    p.q = tensor_of(d->q); p.k = tensor_of(d->k); p.v = tensor_of(d->v); p.o = tensor_of(d->o);
+    p.dout = tensor_of(d->dout); p.dq = tensor_of(d->dq); p.dk = tensor_of(d->dk); p.dv = tensor_of(d->dv);
+    p.bias = d->bias;
+    p.bias_b = d->bias_batch == 1 ? 0 : d->bias_b;
+    p.bias_h = d->bias_heads == 1 ? 0 : d->bias_h;
+    p.bias_i = d->bias_i;
+    p.mask = d->mask; p.mask_b = d->mask_b;
+    p.stats = reinterpret_cast<float2*>(d->stats);
+    p.o_lo = d->dtype == TRIMUL_DTYPE_BF16 ? d->o_lo : nullptr;
+    p.status = status;
+    return p;
+}
+
+// Workspace of the backward pass: delta, then the scores' gradients where the bias's gradient sums them.
+struct AttnWorkspace {
+    int64_t delta, ds, ds_pitch, total;
+};
+AttnWorkspace attn_workspace(const trimul_attn_desc* d, bool backward) {
+    AttnWorkspace w = {};
+    int64_t at = 0;
+    if (backward) {
+        w.delta = at;
+        at += align_up((int64_t)d->B * d->H * d->Lq * 4, 256);
+        w.ds = at;
+        w.ds_pitch = align_up(d->Lk, 16 / elem_size(d->dtype));
+        if (sums_bias(d)) at += align_up((int64_t)d->B * d->H * d->Lq * w.ds_pitch * elem_size(d->dtype), 256);
+    }
+    w.total = at;
+    return w;
+}
+
+template <typename T, int kT, int kC> int launch_plain_fwd(const AttnParams& p, cudaStream_t st) {
+    auto kernel = attn_plain_fwd_kernel<T, kT, kC>;
+    if (!ensure_smem(kernel, ap_smem<kT>(16 * kC, 3, 1))) return TRIMUL_E_CUDA;
+    return launch_stage(kernel, dim3((unsigned)ceil_div(p.Lq, kT), p.H, p.B), kApThreads, ap_smem<kT>(p.D, 3, 1), st, true, p);
+}
+template <typename T, int kT, int kC> int launch_plain_bwd(const AttnParams& p, cudaStream_t st) {
+    auto dq = attn_plain_dq_kernel<T, kT, kC>;
+    auto dkv = attn_plain_dkv_kernel<T, kT, kC>;
+    if (!ensure_smem(dq, ap_smem<kT>(16 * kC, 4, 1)) || !ensure_smem(dkv, ap_smem<kT>(16 * kC, 4, 2))) return TRIMUL_E_CUDA;
+    const int rc = launch_stage(dkv, dim3((unsigned)ceil_div(p.Lk, kT), p.Hk, p.B), kApThreads, ap_smem<kT>(p.D, 4, 2), st, true, p);
+    if (rc != TRIMUL_OK) return rc;
+    return launch_stage(dq, dim3((unsigned)ceil_div(p.Lq, kT), p.H, p.B), kApThreads, ap_smem<kT>(p.D, 4, 1), st, true, p);
+}
+template <typename T> int run_plain_fwd(const AttnParams& p, cudaStream_t st) {
+    if (p.D <= 32) return launch_plain_fwd<T, 64, 2>(p, st);
+    if (p.D <= 64) return launch_plain_fwd<T, 64, 4>(p, st);
+    if (p.D <= 128) return launch_plain_fwd<T, 64, 8>(p, st);
+    return launch_plain_fwd<T, 32, 16>(p, st);
+}
+template <typename T> int run_plain_bwd(const AttnParams& p, cudaStream_t st) {
+    if (p.D <= 32) return launch_plain_bwd<T, 64, 2>(p, st);
+    if (p.D <= 64) return launch_plain_bwd<T, 64, 4>(p, st);
+    return launch_plain_bwd<T, 32, 16>(p, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int trimul_b200_relpos_bias(const trimul_relpos_desc* d, const trimul_buckets* b, const void* table, const void* q_pos,
+                            const void* k_pos, const void* q_seg, const void* k_seg, const void* add, void* out,
+                            void* stream) {
+    const int rc = check_relpos(d, b);
+    if (rc != TRIMUL_OK) return rc;
+    if (table == nullptr || q_pos == nullptr || k_pos == nullptr || out == nullptr) return TRIMUL_E_INVALID;
+    if (b->segments != 0 && (q_seg == nullptr || k_seg == nullptr)) return TRIMUL_E_INVALID;
+    if (d->layout == TRIMUL_RELPOS_HEADS) {
+        const int n = 16 / elem_size(d->dtype);
+        if (add != nullptr || !aligned(out, 16)) return TRIMUL_E_INVALID;
+        if ((d->stride_b % n) || (d->stride_h % n) || (d->stride_i % n) || d->stride_i < align_up(d->Lk, n))
+            return TRIMUL_E_INVALID;
+    }
+    const RelposParams p = relpos_params(d, b, table, q_pos, k_pos, q_seg, k_seg);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return d->dtype == TRIMUL_DTYPE_BF16 ? run_relpos_forward<__nv_bfloat16>(d, b, p, add, out, st)
+                                         : run_relpos_forward<float>(d, b, p, add, out, st);
+}
+
+int trimul_b200_relpos_bias_grad_workspace_bytes(const trimul_relpos_desc* d, const trimul_buckets* b, size_t* bytes) {
+    const int rc = check_relpos(d, b);
+    if (rc != TRIMUL_OK) return rc;
+    if (bytes == nullptr) return TRIMUL_E_INVALID;
+    int64_t parts = 0;
+    for (bool wide : {false, true}) parts = std::max<int64_t>(parts, plan_relpos_grad(d, b, wide).parts);
+    *bytes = (size_t)(parts * (b->count + (b->segments != 0)) * d->channels * 4);
+    return TRIMUL_OK;
+}
+
+int trimul_b200_relpos_bias_grad(const trimul_relpos_desc* d, const trimul_buckets* b, const void* q_pos, const void* k_pos,
+                                 const void* q_seg, const void* k_seg, const void* grad, void* dtable, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+    size_t need = 0;
+    const int rc = trimul_b200_relpos_bias_grad_workspace_bytes(d, b, &need);
+    if (rc != TRIMUL_OK) return rc;
+    if (q_pos == nullptr || k_pos == nullptr || grad == nullptr || dtable == nullptr || workspace == nullptr)
+        return TRIMUL_E_INVALID;
+    if (b->segments != 0 && (q_seg == nullptr || k_seg == nullptr)) return TRIMUL_E_INVALID;
+    if (workspace_bytes < need) return TRIMUL_E_WORKSPACE;
+    if (!aligned(workspace, 16)) return TRIMUL_E_INVALID;
+    const RelposParams p = relpos_params(d, b, nullptr, q_pos, k_pos, q_seg, k_seg);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    float* partial = static_cast<float*>(workspace);
+    return d->dtype == TRIMUL_DTYPE_BF16 ? run_relpos_grad<__nv_bfloat16>(d, b, p, grad, dtable, partial, st)
+                                         : run_relpos_grad<float>(d, b, p, grad, dtable, partial, st);
+}
+
+int trimul_b200_attn_workspace_bytes(const trimul_attn_desc* d, int32_t backward, size_t* bytes) {
+    const int rc = check_attn(d);
+    if (rc != TRIMUL_OK) return rc;
+    if (bytes == nullptr) return TRIMUL_E_INVALID;
+    *bytes = (size_t)attn_workspace(d, backward != 0).total;
+    return TRIMUL_OK;
+}
+
+int trimul_b200_attn_forward(const trimul_attn_desc* d, void* workspace, size_t workspace_bytes, void* stream,
+                             int32_t* status) {
+    const int rc = check_attn(d);
+    if (rc != TRIMUL_OK) return rc;
+    if (!d->q.p || !d->k.p || !d->v.p || !d->o.p) return TRIMUL_E_INVALID;
+    const AttnWorkspace w = attn_workspace(d, false);
+    if (w.total > 0 && (workspace == nullptr || !aligned(workspace, 256))) return TRIMUL_E_INVALID;
+    if (workspace_bytes < (size_t)w.total) return TRIMUL_E_WORKSPACE;
+    const AttnParams p = attn_params(d, status);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return d->dtype == TRIMUL_DTYPE_BF16 ? run_plain_fwd<__nv_bfloat16>(p, st) : run_plain_fwd<float>(p, st);
+}
+
+int trimul_b200_attn_backward(const trimul_attn_desc* d, void* workspace, size_t workspace_bytes, void* stream,
+                              int32_t* status) {
+    int rc = check_attn(d);
+    if (rc != TRIMUL_OK) return rc;
+    if (!d->q.p || !d->k.p || !d->v.p || !d->o.p || !d->dout.p || !d->dq.p || !d->dk.p || !d->dv.p || !d->stats)
+        return TRIMUL_E_INVALID;
+    const AttnWorkspace w = attn_workspace(d, true);
+    if (workspace == nullptr || !aligned(workspace, 256)) return TRIMUL_E_INVALID;
+    if (workspace_bytes < (size_t)w.total) return TRIMUL_E_WORKSPACE;
+    AttnParams p = attn_params(d, status);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    p.delta = reinterpret_cast<float*>(ws + w.delta);
+    if (d->dbias != nullptr) {
+        if (sums_bias(d)) {
+            p.ds = ws + w.ds;
+            p.ds_i = w.ds_pitch; p.ds_h = w.ds_pitch * d->Lq; p.ds_b = p.ds_h * d->H;
+        } else {
+            p.ds = d->dbias;
+            p.ds_i = d->dbias_i; p.ds_h = d->bias_heads == 1 ? 0 : d->dbias_h; p.ds_b = d->bias_batch == 1 ? 0 : d->dbias_b;
+        }
+    }
+    const bool bf16 = d->dtype == TRIMUL_DTYPE_BF16;
+    const int64_t rows = (int64_t)d->B * d->Lq * d->H;
+    const dim3 grid((unsigned)ceil_div(rows, kApThreads / 32));
+    if (bf16) rc = launch_stage(attn_delta_kernel<__nv_bfloat16>, grid, kApThreads, 0, st, true, p);
+    else rc = launch_stage(attn_delta_kernel<float>, grid, kApThreads, 0, st, true, p);
+    if (rc != TRIMUL_OK) return rc;
+    rc = bf16 ? run_plain_bwd<__nv_bfloat16>(p, st) : run_plain_bwd<float>(p, st);
+    if (rc != TRIMUL_OK || !sums_bias(d)) return rc;
+    const int n = 16 / elem_size(d->dtype);
+    const int64_t items = (int64_t)d->bias_batch * d->bias_heads * d->Lq * ceil_div(d->Lk, n);
+    const dim3 sgrid((unsigned)std::min<int64_t>(ceil_div(items, kApThreads), 16 * (int64_t)sm_count()));
+    const int sum_b = d->bias_batch == 1, sum_h = d->bias_heads == 1;
+    if (bf16)
+        return launch_stage(attn_bias_sum_kernel<__nv_bfloat16>, sgrid, kApThreads, 0, st, true,
+                            static_cast<const __nv_bfloat16*>(p.ds), p.ds_b, p.ds_h, p.ds_i,
+                            static_cast<__nv_bfloat16*>(d->dbias), (long long)d->dbias_b, (long long)d->dbias_h,
+                            (long long)d->dbias_i, d->B, d->H, d->Lq, d->Lk, sum_b, sum_h);
+    return launch_stage(attn_bias_sum_kernel<float>, sgrid, kApThreads, 0, st, true, static_cast<const float*>(p.ds), p.ds_b,
+                        p.ds_h, p.ds_i, static_cast<float*>(d->dbias), (long long)d->dbias_b, (long long)d->dbias_h,
+                        (long long)d->dbias_i, d->B, d->H, d->Lq, d->Lk, sum_b, sum_h);
+}
+
+}  // extern "C"

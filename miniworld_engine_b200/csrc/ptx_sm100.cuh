@@ -169,7 +169,7 @@ __device__ __forceinline__ bool mbar_wait_loop(uint64_t* bar, uint32_t parity, v
     report_timeout(status, stage, detail);
     return false;
 }
-__device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+static __device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                             int32_t* status, int stage, int detail, uint64_t limit_ns) {
     return mbar_wait_loop(bar, parity, abort_flag, status, stage, detail, limit_ns);
 }
@@ -988,7 +988,7 @@ __device__ __forceinline__ void fold_row_any(uint8_t* wbase, int sub_bytes, int 
     s = ssum;
     bias = 0.5f * bsum;
 }
-__device__ __noinline__ void fold_row_unaligned(uint8_t* wbase, int sub_bytes, int n, const float* gamma, const float* beta,
+static __device__ __noinline__ void fold_row_unaligned(uint8_t* wbase, int sub_bytes, int n, const float* gamma, const float* beta,
                                                 int nsub, float& s, float& bias) {
     fold_row_any<false>(wbase, sub_bytes, n, gamma, beta, nsub, s, bias);
 }

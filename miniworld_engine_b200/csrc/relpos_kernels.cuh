@@ -1,0 +1,498 @@
+// Learned relative position bias by buckets, and the gradient of its table.
+//
+//   u(b,i,j) = bucket(q_pos[b,i] - k_pos[b,j])      (a bucket of its own for positions of different segments)
+//   heads:  out[b,h,i,j]  = table[u, h]             an attention's additive bias, j contiguous
+//   pair:   out[b,i,j,c]  = add[b,i,j,c] + table[u, c]     the pair tensor's input embedding, c contiguous
+//   d table[u, c] = sum of the upstream gradient over all positions of bucket u
+//
+// Every kernel is bound by device memory: the large tensor is read or written once.  The bucket of a distance is looked
+// up in a table over [-M, M] in shared memory that each block builds from the rule (distances beyond M share the
+// outermost buckets), so no rule costs more per element than another and nothing has to be kept between calls.
+#pragma once
+
+#include "../../include/trimul_b200.h"
+#include "ptx_sm100.cuh"
+
+namespace trimul {
+
+constexpr int kRpPosLimit = (1 << 30) - 1;   // positions are clamped here: no difference overflows 32 bits
+
+struct RelposParams {
+    int B, Lq, Lk, C;
+    int rows;                              // buckets, the segments' one included
+    int M;                                 // largest distance of the look-up table
+    const void *q_pos, *k_pos, *q_seg, *k_seg;      // seg: null when segments are not told apart
+    long long q_pos_b, k_pos_b, q_seg_b, k_seg_b;   // batch strides in elements (0: shared)
+    int q_pos64, k_pos64, q_seg64, k_seg64;         // 64-bit integers instead of 32-bit ones
+    const void* table;
+    int table_bf16;
+    long long sB, sH, sI;                  // strides of out / grad in elements (heads); sB only (pair)
+};
+
+__device__ __forceinline__ int rp_load(const void* p, long long i, int is64) {
+    if (is64) {
+        const long long v = __ldg(static_cast<const long long*>(p) + i);
+        return (int)(v > kRpPosLimit ? kRpPosLimit : v < -kRpPosLimit ? -kRpPosLimit : v);
+    }
+    return min(max(__ldg(static_cast<const int*>(p) + i), -kRpPosLimit), kRpPosLimit);
+}
+__device__ __forceinline__ float rp_table(const RelposParams& p, int u, int c) {
+    const long long i = (long long)u * p.C + c;
+    return p.table_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.table)[i])
+                        : static_cast<const float*>(p.table)[i];
+}
+
+// Bucket of distance d, |d| <= M, straight from the rule.  Logarithmic rules: exact up to `near`, then one bucket per
+// threshold reached.
+__device__ __forceinline__ int rp_rule(const trimul_buckets& b, int d) {
+    if (b.kind == TRIMUL_BUCKETS_CLIPPED) return d + b.max_distance;
+    const int half = b.kind == TRIMUL_BUCKETS_LOG ? b.count / 2 : b.count;
+    const int n = b.kind == TRIMUL_BUCKETS_LOG ? abs(d) : max(d, 0);
+    int lo = 0, hi = b.n_thresholds;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (b.thresholds[mid] <= n) lo = mid + 1; else hi = mid;
+    }
+    return min(n, half / 2) + lo + (b.kind == TRIMUL_BUCKETS_LOG && d < 0 ? half : 0);
+}
+__device__ __forceinline__ void rp_build_lut(uint16_t* lut, const trimul_buckets& b, int M) {
+    for (int i = threadIdx.x; i <= 2 * M; i += blockDim.x) lut[i] = (uint16_t)rp_rule(b, i - M);
+}
+__device__ __forceinline__ int rp_bucket(const uint16_t* lut, int M, int d) { return lut[min(max(d, -M), M) + M]; }
+
+template <typename T> struct RpVec;       // 16 bytes of T
+template <> struct RpVec<__nv_bfloat16> {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
+        f[0] = bf16_lo(v.x); f[1] = bf16_hi(v.x); f[2] = bf16_lo(v.y); f[3] = bf16_hi(v.y);
+        f[4] = bf16_lo(v.z); f[5] = bf16_hi(v.z); f[6] = bf16_lo(v.w); f[7] = bf16_hi(v.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+        return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+    }
+};
+template <> struct RpVec<float> {
+    static constexpr int kN = 4;
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
+        f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+};
+__device__ __forceinline__ float rp_float(float v) { return v; }
+__device__ __forceinline__ float rp_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void rp_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void rp_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// ---------------------------------------------------------------------------------------
+// heads, forward.  One block column (blockIdx.y) per group of kN heads; an item is kN consecutive j of one row: kN
+// table rows of the group (16 bytes each) are turned into kN 16-byte stores, one per head.  Rows of `out` are padded to
+// whole 16-byte pieces by the caller, so the last piece of a row is stored whole.
+// Table rows are kept with their low three bits xor-ed by the next three: neighbouring lanes of a warp are kN rows apart
+// where buckets follow the distance, and would otherwise meet in one bank.
+// ---------------------------------------------------------------------------------------
+constexpr int kRpThreads = 128;
+
+__device__ __forceinline__ void rp_transpose(uint4 (&r)[8]) {        // 8 x 8 bf16, rows of 16 bytes
+    uint4 o[8];
+    const uint32_t* in = &r[0].x;
+    uint32_t* out = &o[0].x;
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t a = in[(2 * j) * 4 + m], b = in[(2 * j + 1) * 4 + m];
+            out[(2 * m) * 4 + j] = __byte_perm(a, b, 0x5410);
+            out[(2 * m + 1) * 4 + j] = __byte_perm(a, b, 0x7632);
+        }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = o[i];
+}
+__device__ __forceinline__ void rp_transpose(uint4 (&r)[4]) {        // 4 x 4 fp32
+    const uint4 a = r[0], b = r[1], c = r[2], d = r[3];
+    r[0] = make_uint4(a.x, b.x, c.x, d.x);
+    r[1] = make_uint4(a.y, b.y, c.y, d.y);
+    r[2] = make_uint4(a.z, b.z, c.z, d.z);
+    r[3] = make_uint4(a.w, b.w, c.w, d.w);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRpThreads)
+relpos_heads_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule, T* out) {
+    constexpr int kN = RpVec<T>::kN;
+    extern __shared__ __align__(16) uint8_t smem[];
+    T* tab = reinterpret_cast<T*>(smem);                                       // [rows rounded up to 64][kN]
+    uint16_t* lut = reinterpret_cast<uint16_t*>(smem + ((p.rows + 63) & ~63) * 16);
+    rp_build_lut(lut, rule, p.M);
+    griddep_wait();
+    griddep_launch_dependents();
+    const int h0 = blockIdx.y * kN;
+    for (int e = threadIdx.x; e < p.rows * kN; e += kRpThreads) {
+        const int u = e / kN, h = e % kN;
+        rp_store(tab + (u ^ ((u >> 3) & 7)) * kN + h, h0 + h < p.C ? rp_table(p, u, h0 + h) : 0.f);
+    }
+    __syncthreads();
+    const int nch = (p.Lk + kN - 1) / kN;
+    const long long items = (long long)p.B * p.Lq * nch;
+    const int nh = min(kN, p.C - h0);
+    for (long long it = (long long)blockIdx.x * kRpThreads + threadIdx.x; it < items; it += (long long)gridDim.x * kRpThreads) {
+        const long long row = it / nch;
+        const int j0 = (int)(it - row * nch) * kN;
+        const int b = (int)(row / p.Lq), i = (int)(row - (long long)b * p.Lq);
+        const int q = rp_load(p.q_pos, b * p.q_pos_b + i, p.q_pos64);
+        const int qs = p.q_seg != nullptr ? rp_load(p.q_seg, b * p.q_seg_b + i, p.q_seg64) : 0;
+        uint4 r[kN];
+#pragma unroll
+        for (int e = 0; e < kN; ++e) {
+            const int j = min(j0 + e, p.Lk - 1);
+            int u = rp_bucket(lut, p.M, q - rp_load(p.k_pos, b * p.k_pos_b + j, p.k_pos64));
+            if (p.q_seg != nullptr && rp_load(p.k_seg, b * p.k_seg_b + j, p.k_seg64) != qs) u = p.rows - 1;
+            r[e] = *reinterpret_cast<const uint4*>(tab + (u ^ ((u >> 3) & 7)) * kN);
+        }
+        rp_transpose(r);
+        T* o = out + b * p.sB + h0 * p.sH + i * p.sI + j0;
+#pragma unroll
+        for (int h = 0; h < kN; ++h)
+            if (h < nh) *reinterpret_cast<uint4*>(o + h * p.sH) = r[h];
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// pair, forward.  A thread owns 16 bytes of a position's channels (kVec; else single channels), a block a run of
+// consecutive positions; the table's rows come through L1 (a few buckets are live at a time).
+// ---------------------------------------------------------------------------------------
+constexpr int kRpPairThreads = 256;
+
+struct RpCursor {          // position -> (batch element, row, column), stepped without divisions
+    int b, i, j;
+    __device__ __forceinline__ void init(const RelposParams& p, long long pos) {
+        const long long row = pos / p.Lk;
+        j = (int)(pos - row * p.Lk);
+        b = (int)(row / p.Lq);
+        i = (int)(row - (long long)b * p.Lq);
+    }
+    __device__ __forceinline__ void step(const RelposParams& p, int n) {
+        j += n;
+        while (j >= p.Lk) {
+            j -= p.Lk;
+            if (++i == p.Lq) { i = 0; ++b; }
+        }
+    }
+    __device__ __forceinline__ int bucket(const RelposParams& p, const uint16_t* lut) const {
+        const int d = rp_load(p.q_pos, b * p.q_pos_b + i, p.q_pos64) - rp_load(p.k_pos, b * p.k_pos_b + j, p.k_pos64);
+        int u = rp_bucket(lut, p.M, d);
+        if (p.q_seg != nullptr && rp_load(p.q_seg, b * p.q_seg_b + i, p.q_seg64) != rp_load(p.k_seg, b * p.k_seg_b + j, p.k_seg64))
+            u = p.rows - 1;
+        return u;
+    }
+};
+
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kRpPairThreads)
+relpos_pair_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule, const T* add, T* out,
+                   int per_block) {
+    constexpr int kN = kVec ? RpVec<T>::kN : 1;
+    constexpr int kU = 4;
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint16_t* lut = reinterpret_cast<uint16_t*>(smem);
+    rp_build_lut(lut, rule, p.M);
+    griddep_wait();
+    griddep_launch_dependents();
+    __syncthreads();
+    // lanes of one position side by side; wide tensors take several passes over the channels
+    const int per_pos = p.C / kN;
+    const int lanes = min(per_pos, kRpPairThreads);
+    const int side = kRpPairThreads / lanes;                  // positions at once
+    const int ty = threadIdx.x / lanes, tx = threadIdx.x % lanes;
+    if (ty >= side) return;
+    const long long total = (long long)p.B * p.Lq * p.Lk;
+    const long long first = (long long)blockIdx.x * per_block, last = min(first + per_block, total);
+    long long pos = first + ty;
+    if (pos >= last) return;
+    RpCursor cur;
+    cur.init(p, pos);
+    while (pos < last) {
+        int u[kU];
+        const int n = (int)min((long long)kU, (last - pos + side - 1) / side);
+#pragma unroll
+        for (int s = 0; s < kU; ++s) {
+            if (s < n) {
+                u[s] = cur.bucket(p, lut);
+                cur.step(p, side);
+            }
+        }
+        for (int v = tx; v < per_pos; v += lanes) {
+            if constexpr (kVec) {
+                uint4 a[kU];
+#pragma unroll
+                for (int s = 0; s < kU; ++s)
+                    if (s < n)
+                        a[s] = add != nullptr ? __ldcs(reinterpret_cast<const uint4*>(add + (pos + (long long)s * side) * p.C) + v)
+                                              : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                for (int s = 0; s < kU; ++s)
+                    if (s < n) {
+                        float f[kN];
+                        RpVec<T>::unpack(a[s], f);
+                        if (p.table_bf16) {
+#pragma unroll
+                            for (int e = 0; e < kN; ++e) f[e] += rp_table(p, u[s], v * kN + e);
+                        } else {
+                            const float4* t = reinterpret_cast<const float4*>(static_cast<const float*>(p.table) + (long long)u[s] * p.C + v * kN);
+#pragma unroll
+                            for (int e = 0; e < kN / 4; ++e) {
+                                const float4 w = __ldg(t + e);
+                                f[4 * e] += w.x; f[4 * e + 1] += w.y; f[4 * e + 2] += w.z; f[4 * e + 3] += w.w;
+                            }
+                        }
+                        __stcs(reinterpret_cast<uint4*>(out + (pos + (long long)s * side) * p.C) + v, RpVec<T>::pack(f));
+                    }
+            } else {
+#pragma unroll
+                for (int s = 0; s < kU; ++s)
+                    if (s < n) {
+                        const long long at = (pos + (long long)s * side) * p.C + v;
+                        rp_store(out + at, (add != nullptr ? rp_float(add[at]) : 0.f) + rp_table(p, u[s], v));
+                    }
+            }
+        }
+        pos += (long long)n * side;
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// heads, gradient of the table.  Block (part, h) sums the rows of its part for head h.  Sums live in shared memory, one
+// column per thread: no atomics, so the result does not depend on the order of anything.  A thread keeps kN consecutive
+// j and walks down the rows; where the outermost distances of its piece share a bucket (buckets are monotone on either
+// side of zero, so everything between shares it too), the piece is summed in registers.
+// ---------------------------------------------------------------------------------------
+template <typename T, bool kVec>
+__global__ void relpos_heads_grad_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule,
+                                         const T* grad, float* partial, int rows_per_part) {
+    constexpr int kN = RpVec<T>::kN;
+    constexpr int kU = 4;
+    extern __shared__ __align__(16) uint8_t smem[];
+    float* acc = reinterpret_cast<float*>(smem);                               // [rows][threads]
+    const int nt = blockDim.x, tid = threadIdx.x;
+    uint16_t* lut = reinterpret_cast<uint16_t*>(smem + (size_t)p.rows * nt * 4);
+    rp_build_lut(lut, rule, p.M);
+    for (int u = 0; u < p.rows; ++u) acc[u * nt + tid] = 0.f;
+    griddep_wait();
+    griddep_launch_dependents();
+    __syncthreads();
+    const int h = blockIdx.y;
+    const int nch = (p.Lk + kN - 1) / kN;
+    const int tpr = min(nch, nt);                             // threads of one row
+    const int side = nt / tpr;                                // rows at once
+    const int ty = tid / tpr, tx = tid % tpr;
+    const long long rows = (long long)p.B * p.Lq;
+    const long long r0 = (long long)blockIdx.x * rows_per_part, r1 = min(r0 + rows_per_part, rows);
+    int run = 0;
+    float sum = 0.f;
+    auto put = [&](int u, float v) {
+        if (u != run) {
+            acc[run * nt + tid] += sum;
+            run = u;
+            sum = 0.f;
+        }
+        sum += v;
+    };
+    if (ty < side) {
+        for (int c = tx; c < nch; c += tpr) {
+            const int j0 = c * kN;
+            const int nj = min(kN, p.Lk - j0);
+            int kp[kN], ks[kN], kmin = 0, kmax = 0;
+            bool one_seg = true;
+            int b_now = -1;
+            for (long long r = r0 + ty; r < r1; r += (long long)kU * side) {
+                float g[kU][kN];
+                if constexpr (kVec) {
+                    uint4 raw[kU];
+#pragma unroll
+                    for (int s = 0; s < kU; ++s) {
+                        const long long rr = r + (long long)s * side;
+                        raw[s] = make_uint4(0u, 0u, 0u, 0u);
+                        if (rr < r1 && nj == kN) {
+                            const int b = (int)(rr / p.Lq), i = (int)(rr - (long long)b * p.Lq);
+                            raw[s] = __ldcs(reinterpret_cast<const uint4*>(grad + b * p.sB + h * p.sH + i * p.sI + j0));
+                        }
+                    }
+#pragma unroll
+                    for (int s = 0; s < kU; ++s) RpVec<T>::unpack(raw[s], g[s]);
+                }
+                if (!kVec || nj < kN) {
+#pragma unroll
+                    for (int s = 0; s < kU; ++s) {
+                        const long long rr = r + (long long)s * side;
+                        const int b = (int)(rr / p.Lq), i = (int)(rr - (long long)b * p.Lq);
+                        const T* src = grad + b * p.sB + h * p.sH + i * p.sI + j0;
+#pragma unroll
+                        for (int e = 0; e < kN; ++e) g[s][e] = rr < r1 && e < nj ? rp_float(src[e]) : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < kU; ++s) {
+                    const long long rr = r + (long long)s * side;
+                    if (rr >= r1) break;
+                    const int b = (int)(rr / p.Lq), i = (int)(rr - (long long)b * p.Lq);
+                    if (b != b_now) {
+                        b_now = b;
+#pragma unroll
+                        for (int e = 0; e < kN; ++e) {
+                            const int j = min(j0 + e, p.Lk - 1);
+                            kp[e] = rp_load(p.k_pos, b * p.k_pos_b + j, p.k_pos64);
+                            ks[e] = p.k_seg != nullptr ? rp_load(p.k_seg, b * p.k_seg_b + j, p.k_seg64) : 0;
+                        }
+                        kmin = kmax = kp[0];
+                        one_seg = true;
+#pragma unroll
+                        for (int e = 1; e < kN; ++e) {
+                            kmin = min(kmin, kp[e]);
+                            kmax = max(kmax, kp[e]);
+                            one_seg = one_seg && ks[e] == ks[0];
+                        }
+                    }
+                    const int q = rp_load(p.q_pos, b * p.q_pos_b + i, p.q_pos64);
+                    const int qs = p.q_seg != nullptr ? rp_load(p.q_seg, b * p.q_seg_b + i, p.q_seg64) : 0;
+                    const bool apart = one_seg && ks[0] != qs;
+                    const int ulo = rp_bucket(lut, p.M, q - kmax), uhi = rp_bucket(lut, p.M, q - kmin);
+                    // d >= 0 and d < 0 may share a bucket only where everything between does (one-sided rules)
+                    if (apart || (one_seg && ulo == uhi)) {
+                        float t = 0.f;
+#pragma unroll
+                        for (int e = 0; e < kN; ++e) t += g[s][e];
+                        put(apart ? p.rows - 1 : ulo, t);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < kN; ++e) {
+                            if (e < nj) put(ks[e] != qs ? p.rows - 1 : rp_bucket(lut, p.M, q - kp[e]), g[s][e]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    acc[run * nt + tid] += sum;
+    __syncthreads();
+    // a warp per bucket: lanes over the threads' columns
+    const int warp = tid >> 5, lane = tid & 31, warps = nt >> 5;
+    for (int u = warp; u < p.rows; u += warps) {
+        float t = 0.f;
+        for (int e = lane; e < nt; e += 32) t += acc[u * nt + e];
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        if (lane == 0) partial[((long long)blockIdx.x * p.rows + u) * p.C + h] = t;
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// pair, gradient of the table.  A warp owns a run of consecutive positions and 32 kL channels (blockIdx.y), kL per lane,
+// and a private set of sums [rows][32 kL] in shared memory; the running bucket's sum stays in registers until the bucket
+// changes (the test is uniform over the warp).
+// ---------------------------------------------------------------------------------------
+template <typename T, int kL>
+__device__ __forceinline__ void rp_load_lane(const T* p, float (&f)[kL]) {
+    if constexpr (kL == 1) f[0] = rp_float(p[0]);
+    else if constexpr (sizeof(T) == 2) {
+        const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
+        f[0] = bf16_lo(v.x); f[1] = bf16_hi(v.x); f[2] = bf16_lo(v.y); f[3] = bf16_hi(v.y);
+    } else {
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(p));
+        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    }
+}
+
+template <typename T, int kL>
+__global__ void relpos_pair_grad_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule,
+                                        const T* grad, float* partial, long long pos_per_warp) {
+    constexpr int kU = 8;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int nt = blockDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = nt >> 5;
+    float* sums = reinterpret_cast<float*>(smem);                              // [warps][rows][32 kL]
+    uint16_t* lut = reinterpret_cast<uint16_t*>(smem + (size_t)warps * p.rows * 32 * kL * 4);
+    rp_build_lut(lut, rule, p.M);
+    for (int e = tid; e < warps * p.rows * 32 * kL; e += nt) sums[e] = 0.f;
+    griddep_wait();
+    griddep_launch_dependents();
+    __syncthreads();
+    const int c0 = blockIdx.y * 32 * kL + lane * kL;
+    const bool live = c0 < p.C;
+    float* acc = sums + (size_t)warp * p.rows * 32 * kL + lane * kL;
+    const long long total = (long long)p.B * p.Lq * p.Lk;
+    const long long first = ((long long)blockIdx.x * warps + warp) * pos_per_warp, last = min(first + pos_per_warp, total);
+    int run = 0;
+    float sum[kL];
+#pragma unroll
+    for (int e = 0; e < kL; ++e) sum[e] = 0.f;
+    RpCursor cur;
+    if (first < last) cur.init(p, min(first + lane, total - 1));
+    for (long long pos = first; pos < last; pos += 32) {
+        const int n = (int)min(32ll, last - pos);
+        int u = 0;
+        if (lane < n) {
+            u = cur.bucket(p, lut);
+            cur.step(p, 32);
+        }
+        for (int s0 = 0; s0 < n; s0 += kU) {
+            float g[kU][kL];
+#pragma unroll
+            for (int s = 0; s < kU; ++s) {
+#pragma unroll
+                for (int e = 0; e < kL; ++e) g[s][e] = 0.f;
+                if (s0 + s < n && live) rp_load_lane<T, kL>(grad + (pos + s0 + s) * p.C + c0, g[s]);
+            }
+#pragma unroll
+            for (int s = 0; s < kU; ++s) {
+                const int us = __shfl_sync(0xffffffffu, u, (s0 + s) & 31);
+                if (s0 + s >= n) break;
+                if (us != run) {
+#pragma unroll
+                    for (int e = 0; e < kL; ++e) {
+                        acc[run * 32 * kL + e] += sum[e];
+                        sum[e] = 0.f;
+                    }
+                    run = us;
+                }
+#pragma unroll
+                for (int e = 0; e < kL; ++e) sum[e] += g[s][e];
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < kL; ++e) acc[run * 32 * kL + e] += sum[e];
+    __syncthreads();
+    const int width = min(32 * kL, p.C - (int)blockIdx.y * 32 * kL);
+    for (int e = tid; e < p.rows * 32 * kL; e += nt) {
+        const int c = e % (32 * kL), u = e / (32 * kL);
+        if (c >= width) continue;
+        float t = 0.f;
+        for (int w = 0; w < warps; ++w) t += sums[(size_t)w * p.rows * 32 * kL + e];
+        partial[((long long)blockIdx.x * p.rows + u) * p.C + blockIdx.y * 32 * kL + c] = t;
+    }
+}
+
+// partial [parts][n] -> out [n], in a fixed order: eight threads share an output's parts.
+constexpr int kRpReduceThreads = 256;
+__global__ void __launch_bounds__(kRpReduceThreads)
+relpos_reduce_kernel(const float* partial, void* out, int out_bf16, int parts, int n) {
+    __shared__ float s[8][33];
+    griddep_wait();
+    griddep_launch_dependents();
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int o = blockIdx.x * 32 + x;
+    float t = 0.f;
+    if (o < n) {
+#pragma unroll 8
+        for (int k = y; k < parts; k += 8) t += partial[(long long)k * n + o];
+    }
+    s[y][x] = t;
+    __syncthreads();
+    if (y == 0 && o < n) {
+        for (int k = 1; k < 8; ++k) t += s[k][x];
+        if (out_bf16) static_cast<__nv_bfloat16*>(out)[o] = __float2bfloat16_rn(t);
+        else static_cast<float*>(out)[o] = t;
+    }
+}
+
+}  // namespace trimul
