@@ -11,6 +11,7 @@
 #include <cuda_runtime.h>
 
 #include "host_common.cuh"
+#include "attn_fwd_sm100.cuh"
 #include "attn_plain.cuh"
 #include "relpos_kernels.cuh"
 
@@ -213,13 +214,70 @@ AttnParams attn_params(const trimul_attn_desc* d, int32_t* status) {
     return p;
 }
 
-// Workspace of the backward pass: delta, then the scores' gradients where the bias's gradient sums them.
+// ---------------------------------------------------------------------------------------
+// choice of kernels.  Tensor cores: bf16 whose rows TMA can fetch (16-byte aligned, no axis repeated in place)
+// ---------------------------------------------------------------------------------------
+bool tma_rows(const trimul_attn_tensor& t, int L, int H, int B) {
+    auto ok = [](int n, int64_t s) { return n == 1 || (s > 0 && (s % 8) == 0); };
+    return aligned(t.p, 16) && ok(L, t.l) && ok(H, t.h) && ok(B, t.b);
+}
+bool tensor_cores(const trimul_attn_desc* d) {
+    if (d->dtype != TRIMUL_DTYPE_BF16 || (d->flags & TRIMUL_ATTN_FLAG_PLAIN) != 0) return false;
+    return (d->D % 8) == 0 && d->D <= 128;
+}
+bool tensor_core_forward(const trimul_attn_desc* d) {
+    if (!tensor_cores(d) || !tma_rows(d->q, d->Lq, d->H, d->B) || !tma_rows(d->k, d->Lk, d->Hk, d->B) ||
+        !tma_rows(d->v, d->Lk, d->Hk, d->B) || !tma_rows(d->o, d->Lq, d->H, d->B) || !aligned(d->o_lo, 16))
+        return false;
+    if (d->bias == nullptr) return true;
+    return tma_rows(trimul_attn_tensor{const_cast<void*>(d->bias), d->bias_b, d->bias_i, d->bias_h}, d->Lq, d->bias_heads, d->bias_batch);
+}
+
+bool encode_rows(CUtensorMap* map, const AttnTensor& t, int D, int L, int H, int B) {
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)L, (uint64_t)H, (uint64_t)B};
+    const uint64_t any = (uint64_t)align_up(D, 8);       // of an axis with one entry
+    const uint64_t strides[3] = {L > 1 ? (uint64_t)t.l : any, H > 1 ? (uint64_t)t.h : any, B > 1 ? (uint64_t)t.b : any};
+    const uint32_t box[4] = {64, kAfRows, 1, 1};
+    return encode_bf16(map, t.p, 4, dims, strides, box, 128);
+}
+bool encode_bias(CUtensorMap* map, const trimul_attn_desc* d) {
+    return encode_rows(map, AttnTensor{const_cast<void*>(d->bias), d->bias_b, d->bias_i, d->bias_h}, d->Lk, d->Lq, d->bias_heads,
+                       d->bias_batch);
+}
+
+// Key splits of the forward pass: where the blocks leave SMs idle, each block takes a share of the key tiles (two at
+// least: a lone tile's products and exponentials do not overlap) and a second kernel joins the parts.
+int forward_splits(const trimul_attn_desc* d) {
+    const int64_t blocks = ceil_div(d->Lq, 2 * kAfRows) * d->H * d->B, tiles = ceil_div(d->Lk, kAfRows);
+    const int64_t room = sm_count() / blocks;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(room, tiles / 2));
+}
+
+// Workspace.  Both directions: the key mask as bits and its list of tiles.  Forward: the parts of split rows.  Backward:
+// delta, then the scores' gradients where the bias's gradient sums them.
 struct AttnWorkspace {
-    int64_t delta, ds, ds_pitch, total;
+    int64_t words, list, part_o, part_ml, delta, ds, ds_pitch, total;
+    int splits;
 };
 AttnWorkspace attn_workspace(const trimul_attn_desc* d, bool backward) {
     AttnWorkspace w = {};
     int64_t at = 0;
+    const bool tc = tensor_cores(d);
+    const int64_t tiles = ceil_div(d->Lk, kAfRows);
+    if (tc && d->mask != nullptr) {
+        w.words = at;
+        at += align_up(d->B * tiles * 16, 256);
+        w.list = at;
+        at += align_up(d->B * (tiles + 1) * 4, 256);
+    }
+    w.splits = tc && !backward ? forward_splits(d) : 1;
+    if (w.splits > 1) {
+        const int64_t rows = (int64_t)w.splits * d->B * d->H * d->Lq;
+        w.part_o = at;
+        at += align_up(rows * d->D * 4, 256);
+        w.part_ml = at;
+        at += align_up(rows * 8, 256);
+    }
     if (backward) {
         w.delta = at;
         at += align_up((int64_t)d->B * d->H * d->Lq * 4, 256);
@@ -254,6 +312,54 @@ template <typename T> int run_plain_bwd(const AttnParams& p, cudaStream_t st) {
     if (p.D <= 32) return launch_plain_bwd<T, 64, 2>(p, st);
     if (p.D <= 64) return launch_plain_bwd<T, 64, 4>(p, st);
     return launch_plain_bwd<T, 32, 16>(p, st);
+}
+
+int run_mask(const trimul_attn_desc* d, uint32_t* words, int* list, cudaStream_t st) {
+    return launch_stage(attn_mask_kernel, dim3((unsigned)d->B), kMaskPrepThreads, 0, st, true, d->mask, (long long)d->mask_b, d->Lk,
+                        (int)ceil_div(d->Lk, kAfRows), words, list);
+}
+
+template <int kD, bool kBias>
+int launch_fwd(const AttnFwdParams& fp, const CUtensorMap (&m)[4], cudaStream_t st) {
+    using L = AfLayout<kD, kBias>;
+    auto kernel = attn_fwd_sm100_kernel<kD, kBias>;
+    if (!ensure_smem(kernel, L::kSmem)) return TRIMUL_E_CUDA;
+    const dim3 grid((unsigned)ceil_div(fp.a.Lq, 2 * kAfRows), (unsigned)fp.a.H, (unsigned)(fp.a.B * fp.splits));
+    return launch_stage(kernel, grid, kAfThreads, L::kSmem, st, true, m[0], m[1], m[2], m[3], fp);
+}
+int run_fwd(const trimul_attn_desc* d, const AttnParams& p, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
+    AttnFwdParams fp = {};
+    fp.a = p;
+    fp.n_tiles = (int)ceil_div(d->Lk, kAfRows);
+    fp.splits = w.splits;
+    fp.tiles_per_split = (int)ceil_div(fp.n_tiles, w.splits);
+    fp.bias_b1 = d->bias_batch == 1;
+    fp.bias_h1 = d->bias_heads == 1;
+    if (w.splits > 1) {
+        fp.part_o = reinterpret_cast<float*>(ws + w.part_o);
+        fp.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
+    }
+    CUtensorMap m[4];
+    if (!encode_rows(&m[0], p.q, d->D, d->Lq, d->H, d->B) || !encode_rows(&m[1], p.k, d->D, d->Lk, d->Hk, d->B) ||
+        !encode_rows(&m[2], p.v, d->D, d->Lk, d->Hk, d->B))
+        return TRIMUL_E_CUDA;
+    m[3] = m[0];
+    if (d->bias != nullptr && !encode_bias(&m[3], d)) return TRIMUL_E_CUDA;
+    if (d->mask != nullptr) {
+        uint32_t* words = reinterpret_cast<uint32_t*>(ws + w.words);
+        int* list = reinterpret_cast<int*>(ws + w.list);
+        const int rc = run_mask(d, words, list, st);
+        if (rc != TRIMUL_OK) return rc;
+        fp.words = words;
+        fp.list = list;
+    }
+    int rc;
+    if (d->D <= 64) rc = d->bias != nullptr ? launch_fwd<64, true>(fp, m, st) : launch_fwd<64, false>(fp, m, st);
+    else rc = d->bias != nullptr ? launch_fwd<128, true>(fp, m, st) : launch_fwd<128, false>(fp, m, st);
+    if (rc != TRIMUL_OK || w.splits == 1) return rc;
+    const int64_t rows = (int64_t)d->B * d->H * d->Lq;
+    return launch_stage(attn_combine_kernel<__nv_bfloat16>, dim3((unsigned)ceil_div(rows, 8)), 256, 0, st, true, p,
+                        static_cast<const float*>(fp.part_o), static_cast<const float2*>(fp.part_ml), w.splits);
 }
 
 }  // namespace
@@ -325,6 +431,7 @@ int trimul_b200_attn_forward(const trimul_attn_desc* d, void* workspace, size_t 
     if (workspace_bytes < (size_t)w.total) return TRIMUL_E_WORKSPACE;
     const AttnParams p = attn_params(d, status);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (tensor_core_forward(d)) return run_fwd(d, p, w, static_cast<uint8_t*>(workspace), st);
     return d->dtype == TRIMUL_DTYPE_BF16 ? run_plain_fwd<__nv_bfloat16>(p, st) : run_plain_fwd<float>(p, st);
 }
 

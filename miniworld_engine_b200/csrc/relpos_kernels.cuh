@@ -121,9 +121,9 @@ template <typename T>
 __global__ void __launch_bounds__(kRpThreads)
 relpos_heads_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule, T* out) {
     constexpr int kN = RpVec<T>::kN;
-    extern __shared__ __align__(16) uint8_t smem[];
-    T* tab = reinterpret_cast<T*>(smem);                                       // [rows rounded up to 64][kN]
-    uint16_t* lut = reinterpret_cast<uint16_t*>(smem + ((p.rows + 63) & ~63) * 16);
+    extern __shared__ __align__(16) uint8_t rp_smem[];
+    T* tab = reinterpret_cast<T*>(rp_smem);                                      // [rows rounded up to 64][kN]
+    uint16_t* lut = reinterpret_cast<uint16_t*>(rp_smem + ((p.rows + 63) & ~63) * 16);
     rp_build_lut(lut, rule, p.M);
     griddep_wait();
     griddep_launch_dependents();
@@ -194,8 +194,8 @@ relpos_pair_kernel(const __grid_constant__ RelposParams p, const __grid_constant
                    int per_block) {
     constexpr int kN = kVec ? RpVec<T>::kN : 1;
     constexpr int kU = 4;
-    extern __shared__ __align__(16) uint8_t smem[];
-    uint16_t* lut = reinterpret_cast<uint16_t*>(smem);
+    extern __shared__ __align__(16) uint8_t rp_smem[];
+    uint16_t* lut = reinterpret_cast<uint16_t*>(rp_smem);
     rp_build_lut(lut, rule, p.M);
     griddep_wait();
     griddep_launch_dependents();
@@ -272,10 +272,10 @@ __global__ void relpos_heads_grad_kernel(const __grid_constant__ RelposParams p,
                                          const T* grad, float* partial, int rows_per_part) {
     constexpr int kN = RpVec<T>::kN;
     constexpr int kU = 4;
-    extern __shared__ __align__(16) uint8_t smem[];
-    float* acc = reinterpret_cast<float*>(smem);                               // [rows][threads]
+    extern __shared__ __align__(16) uint8_t rp_smem[];
+    float* acc = reinterpret_cast<float*>(rp_smem);                               // [rows][threads]
     const int nt = blockDim.x, tid = threadIdx.x;
-    uint16_t* lut = reinterpret_cast<uint16_t*>(smem + (size_t)p.rows * nt * 4);
+    uint16_t* lut = reinterpret_cast<uint16_t*>(rp_smem + (size_t)p.rows * nt * 4);
     rp_build_lut(lut, rule, p.M);
     for (int u = 0; u < p.rows; ++u) acc[u * nt + tid] = 0.f;
     griddep_wait();
@@ -407,10 +407,10 @@ template <typename T, int kL>
 __global__ void relpos_pair_grad_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule,
                                         const T* grad, float* partial, long long pos_per_warp) {
     constexpr int kU = 8;
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(16) uint8_t rp_smem[];
     const int nt = blockDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = nt >> 5;
-    float* sums = reinterpret_cast<float*>(smem);                              // [warps][rows][32 kL]
-    uint16_t* lut = reinterpret_cast<uint16_t*>(smem + (size_t)warps * p.rows * 32 * kL * 4);
+    float* sums = reinterpret_cast<float*>(rp_smem);                              // [warps][rows][32 kL]
+    uint16_t* lut = reinterpret_cast<uint16_t*>(rp_smem + (size_t)warps * p.rows * 32 * kL * 4);
     rp_build_lut(lut, rule, p.M);
     for (int e = tid; e < warps * p.rows * 32 * kL; e += nt) sums[e] = 0.f;
     griddep_wait();
