@@ -11,6 +11,7 @@
 #include <cuda_runtime.h>
 
 #include "host_common.cuh"
+#include "attn_bwd_sm100.cuh"
 #include "attn_fwd_sm100.cuh"
 #include "attn_plain.cuh"
 #include "relpos_kernels.cuh"
@@ -233,6 +234,11 @@ bool tensor_core_forward(const trimul_attn_desc* d) {
     return tma_rows(trimul_attn_tensor{const_cast<void*>(d->bias), d->bias_b, d->bias_i, d->bias_h}, d->Lq, d->bias_heads, d->bias_batch);
 }
 
+bool tensor_core_backward(const trimul_attn_desc* d) {
+    return tensor_core_forward(d) && tma_rows(d->dout, d->Lq, d->H, d->B) && tma_rows(d->dq, d->Lq, d->H, d->B) &&
+           tma_rows(d->dk, d->Lk, d->Hk, d->B) && tma_rows(d->dv, d->Lk, d->Hk, d->B);
+}
+
 bool encode_rows(CUtensorMap* map, const AttnTensor& t, int D, int L, int H, int B) {
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)L, (uint64_t)H, (uint64_t)B};
     const uint64_t any = (uint64_t)align_up(D, 8);       // of an axis with one entry
@@ -362,6 +368,44 @@ int run_fwd(const trimul_attn_desc* d, const AttnParams& p, const AttnWorkspace&
                         static_cast<const float*>(fp.part_o), static_cast<const float2*>(fp.part_ml), w.splits);
 }
 
+template <int kD, bool kBias>
+int launch_bwd(const AttnBwdParams& bp, const CUtensorMap (&m)[5], cudaStream_t st) {
+    using KV = AbKvLayout<kD, kBias>;
+    using Q = AbQLayout<kD, kBias>;
+    auto dkv = attn_dkv_sm100_kernel<kD, kBias>;
+    auto dq = attn_dq_sm100_kernel<kD, kBias>;
+    if (!ensure_smem(dkv, KV::kSmem) || !ensure_smem(dq, Q::kSmem)) return TRIMUL_E_CUDA;
+    const AttnParams& p = bp.a;
+    const int rc = launch_stage(dkv, dim3((unsigned)bp.n_tiles, (unsigned)p.Hk, (unsigned)p.B), kAbThreads, KV::kSmem, st, true,
+                                m[0], m[1], m[2], m[3], m[4], bp);
+    if (rc != TRIMUL_OK) return rc;
+    return launch_stage(dq, dim3((unsigned)ceil_div(p.Lq, kAfRows), (unsigned)p.H, (unsigned)p.B), kAbThreads, Q::kSmem, st, true,
+                        m[0], m[1], m[2], m[3], m[4], bp);
+}
+int run_bwd(const trimul_attn_desc* d, const AttnParams& p, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
+    AttnBwdParams bp = {};
+    bp.a = p;
+    bp.n_tiles = (int)ceil_div(d->Lk, kAfRows);
+    bp.bias_b1 = d->bias_batch == 1;
+    bp.bias_h1 = d->bias_heads == 1;
+    CUtensorMap m[5];
+    if (!encode_rows(&m[0], p.q, d->D, d->Lq, d->H, d->B) || !encode_rows(&m[1], p.k, d->D, d->Lk, d->Hk, d->B) ||
+        !encode_rows(&m[2], p.v, d->D, d->Lk, d->Hk, d->B) || !encode_rows(&m[3], p.dout, d->D, d->Lq, d->H, d->B))
+        return TRIMUL_E_CUDA;
+    m[4] = m[0];
+    if (d->bias != nullptr && !encode_bias(&m[4], d)) return TRIMUL_E_CUDA;
+    if (d->mask != nullptr) {
+        uint32_t* words = reinterpret_cast<uint32_t*>(ws + w.words);
+        int* list = reinterpret_cast<int*>(ws + w.list);
+        const int rc = run_mask(d, words, list, st);
+        if (rc != TRIMUL_OK) return rc;
+        bp.words = words;
+        bp.list = list;
+    }
+    if (d->D <= 64) return d->bias != nullptr ? launch_bwd<64, true>(bp, m, st) : launch_bwd<64, false>(bp, m, st);
+    return d->bias != nullptr ? launch_bwd<128, true>(bp, m, st) : launch_bwd<128, false>(bp, m, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -463,7 +507,8 @@ int trimul_b200_attn_backward(const trimul_attn_desc* d, void* workspace, size_t
     if (bf16) rc = launch_stage(attn_delta_kernel<__nv_bfloat16>, grid, kApThreads, 0, st, true, p);
     else rc = launch_stage(attn_delta_kernel<float>, grid, kApThreads, 0, st, true, p);
     if (rc != TRIMUL_OK) return rc;
-    rc = bf16 ? run_plain_bwd<__nv_bfloat16>(p, st) : run_plain_bwd<float>(p, st);
+    if (tensor_core_backward(d)) rc = run_bwd(d, p, w, ws, st);
+    else rc = bf16 ? run_plain_bwd<__nv_bfloat16>(p, st) : run_plain_bwd<float>(p, st);
     if (rc != TRIMUL_OK || !sums_bias(d)) return rc;
     const int n = 16 / elem_size(d->dtype);
     const int64_t items = (int64_t)d->bias_batch * d->bias_heads * d->Lq * ceil_div(d->Lk, n);

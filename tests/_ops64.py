@@ -10,6 +10,7 @@ import math
 import torch
 
 E32 = 2.0 ** -24
+FLUSH = 2.0 ** -126      # smallest normal fp32 number: exponentials below it may come out as zero
 
 
 def half_step(dtype) -> float:
@@ -55,7 +56,8 @@ def attention64(q, k, v, bias=None, mask=None, scale=None, grad=None):
     half a step of the inputs' type and e = 2^-24 of the arithmetic: r for the probabilities and score gradients that
     enter a product, r for each result, and for every fp32 sum its length times e of the sum of absolute values.  The
     score of a pair is off by dx = e ((D + 3) scale sum|q||k| + 3|x| + 3|max|), a probability relatively by dx, the row's
-    largest dx (through its sum), and (Lk + 8) e."""
+    largest dx (through its sum), and (Lk + 8) e; one below 2^-126 may be zero, so 2^-126 is added to each
+    probability's error and goes wherever the probability goes (into ds times |dp - delta|, which is far from 1)."""
     dtype = q.dtype
     r = half_step(dtype) if dtype != torch.float32 else 0.0
     last = half_step(dtype)
@@ -84,7 +86,7 @@ def attention64(q, k, v, bias=None, mask=None, scale=None, grad=None):
     dx = E32 * ((D + 3) * size + 3 * xa + 3 * m0.abs())
     R = dx + torch.where(p > 0, dx, 0.0).amax(-1, keepdim=True) + (Lk + 8) * E32
     o = p @ V
-    o_err = (p * (R + r + Lk * E32)) @ V.abs()
+    o_err = (p * (R + r + Lk * E32) + FLUSH) @ V.abs()
     res = {"out": (o, o_err + last * o.abs())}
     if grad is not None:
         g = grad.double().transpose(1, 2)
@@ -93,13 +95,13 @@ def attention64(q, k, v, bias=None, mask=None, scale=None, grad=None):
         delta = (g * o).sum(-1, keepdim=True)
         Ed = (g.abs() * (o_err + r * r * o.abs() + E32 * D * o.abs())).sum(-1, keepdim=True)
         ds = p * (dp - delta)
-        dse = p * (R * (dp - delta).abs() + Eg + Ed) + r * ds.abs()
+        dse = (p * R + FLUSH) * (dp - delta).abs() + p * (Eg + Ed) + r * ds.abs()
         dq = ds @ K * scale
         dq_e = (dse + Lk * E32 * ds.abs()) @ K.abs() * abs(scale) + last * dq.abs()
         dk = ds.transpose(-1, -2) @ Q * scale
         dk_e = (dse + Lq * G * E32 * ds.abs()).transpose(-1, -2) @ Q.abs() * abs(scale)
         dv = p.transpose(-1, -2) @ g
-        dv_e = (p * (R + r + Lq * G * E32)).transpose(-1, -2) @ g.abs()
+        dv_e = (p * (R + r + Lq * G * E32) + FLUSH).transpose(-1, -2) @ g.abs()
         dk, dk_e, dv, dv_e = (t.unflatten(1, (Hk, G)).sum(2) for t in (dk, dk_e, dv, dv_e))
         res |= {"dq": (dq, dq_e), "dk": (dk, dk_e + last * dk.abs()), "dv": (dv, dv_e + last * dv.abs())}
         if bias is not None:
