@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG_DIR, "libtrimul_b200.so")
@@ -104,6 +105,11 @@ class AttnDesc(C.Structure):
         ("dbias_b", C.c_int64), ("dbias_h", C.c_int64), ("dbias_i", C.c_int64)]
 
 
+# the same two descriptors as packers (native layout: what the compiler gives the C structures)
+RELPOS_DESC = struct.Struct("@I9i7q")
+ATTN_DESC = struct.Struct("@I7ifI" + 8 * "Pqqq" + "PqqqiiPqPPPqqq")
+
+
 class TrimulLibraryError(RuntimeError):
     """The C-ABI library is missing, stale or returned an error code."""
 
@@ -155,7 +161,7 @@ def load():
                                              C.c_void_p, C.c_void_p]
     lib.trimul_b200_selftest_expiring_wait.restype = C.c_int
     lib.trimul_b200_selftest_expiring_wait.argtypes = [C.c_uint32, C.c_void_p, C.c_void_p]
-    PR, PB, PA, V = C.POINTER(RelposDesc), C.POINTER(Buckets), C.POINTER(AttnDesc), C.c_void_p
+    PR = PB = PA = V = C.c_void_p      # descriptors come as structures or as the packers' bytes
     for name, args in (
             ("trimul_b200_relpos_bias", [PR, PB, V, V, V, V, V, V, V, V]),
             ("trimul_b200_relpos_bias_grad_workspace_bytes", [PR, PB, C.POINTER(C.c_size_t)]),

@@ -32,6 +32,8 @@ def _laid_out(t: torch.Tensor, tensor_cores: bool) -> torch.Tensor:
     16-byte boundary and no axis repeated in place (a copy where it is not)."""
     if t.requires_grad:
         t = t.detach()
+    if t.is_contiguous():
+        return t if not tensor_cores or t.data_ptr() % 16 == 0 else t.clone()
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         return t.contiguous()
     if any(s < 0 for s in t.stride()):
@@ -41,86 +43,77 @@ def _laid_out(t: torch.Tensor, tensor_cores: bool) -> torch.Tensor:
     return t
 
 
-def _tensor(t: torch.Tensor) -> _lib.AttnTensor:
-    return _lib.AttnTensor(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+_NONE = (0, 0, 0, 0)
+_workspace_sizes: dict = {}      # of the library's answers, by what they depend on
+
+
+def _tensor(t: torch.Tensor) -> tuple:
+    b, l, h, _ = t.stride()
+    return t.data_ptr(), b, l, h
 
 
 class _Call:
-    """Checked arguments of one call and their descriptor."""
+    """Checked arguments of one call.  ``pack`` makes the library's descriptor of them (as bytes: setting the fields of a
+    ctypes structure one by one costs more than the launch of a small problem)."""
+
+    __slots__ = ("device", "code", "tensor_cores", "q", "k", "v", "sizes", "empty", "head", "bias", "bias_args", "bias_shape",
+                 "mask", "mask_args")
 
     def __init__(self, q, k, v, bias, key_mask, scale, plain_kernels):
         if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
             raise ValueError("q, k and v must be [B, L, heads, D]")
         B, Lq, H, D = q.shape
-        if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        kshape = k.shape
+        _, Lk, Hk, _ = kshape
+        if kshape != v.shape or kshape[0] != B or kshape[3] != D:
             raise ValueError(f"k and v must both be [{B}, Lk, key heads, {D}], got {tuple(k.shape)} and {tuple(v.shape)}")
-        Lk, Hk = k.shape[1], k.shape[2]
         if H and (Hk == 0 or H % Hk):
             raise ValueError(f"the {H} query heads must be a multiple of the {Hk} key heads")
         if D == 0:
             raise ValueError("the head dimension must not be empty")
         _require_cuda(q, "q")
-        self.device = q.device
-        self.code = _dtype_code(q)
+        device, dtype = q.device, q.dtype
+        code = _dtype_code(q)
         for name, t in (("k", k), ("v", v), ("bias", bias)):
-            if t is not None and (t.dtype != q.dtype or t.device != q.device):
-                raise ValueError(f"{name} must be {q.dtype} on {q.device} like q, got {t.dtype} on {t.device}")
-        tc = self.code == _lib.DTYPE_BF16 and D % 8 == 0 and D <= 128 and not plain_kernels
-        self.tensor_cores = tc
+            if t is not None and (t.dtype is not dtype or t.device != device):
+                raise ValueError(f"{name} must be {dtype} on {device} like q, got {t.dtype} on {t.device}")
+        tc = code == _lib.DTYPE_BF16 and D % 8 == 0 and D <= 128 and not plain_kernels
+        self.device, self.code, self.tensor_cores = device, code, tc
         self.q, self.k, self.v = _laid_out(q, tc), _laid_out(k, tc), _laid_out(v, tc)
         self.sizes = (B, Lq, Lk, H, Hk, D)
         self.empty = B == 0 or Lq == 0 or H == 0
         scale = D ** -0.5 if scale is None else float(scale)
         if not math.isfinite(scale):
             raise ValueError(f"scale must be finite, got {scale}")
-        d = _lib.AttnDesc()
-        d.struct_bytes = C.sizeof(_lib.AttnDesc)
-        d.dtype = self.code
-        d.B, d.Lq, d.Lk, d.H, d.Hk, d.D = self.sizes
-        d.scale = scale
-        d.flags = _lib.ATTN_FLAG_PLAIN if plain_kernels else 0
-        d.q, d.k, d.v = _tensor(self.q), _tensor(self.k), _tensor(self.v)
-        self.bias_shape = None
-        self.keep = []
+        self.head = (_lib.ATTN_DESC.size, code, B, Lq, Lk, H, Hk, D, scale, _lib.ATTN_FLAG_PLAIN if plain_kernels else 0)
+        self.bias = self.bias_shape = self.mask = None
+        self.bias_args, self.mask_args = (0, 0, 0, 0, 0, 0), (0, 0)
         if bias is not None:
             shape = tuple(bias.shape)
-            if bias.dim() not in (2, 3, 4):
+            if len(shape) not in (2, 3, 4):
                 raise ValueError(f"bias must be [(B,) (H,) Lq, Lk], got {shape}")
             full = (1,) * (4 - len(shape)) + shape
             if full[0] not in (1, B) or full[1] not in (1, H) or full[2:] != (Lq, Lk):
                 raise ValueError(f"bias must be [1 or {B}, 1 or {H}, {Lq}, {Lk}], got {shape}")
             self.bias_shape = shape
             bias = bias.detach() if bias.requires_grad else bias
-            bias = bias.reshape(full) if len(shape) < 4 else bias
+            bias = bias[(None,) * (4 - len(shape))] if len(shape) < 4 else bias
             if not self.empty and Lk:
-                bias = self._bias_rows(bias)
-            d.bias = bias.data_ptr()
-            d.bias_batch, d.bias_heads = full[:2]
-            d.bias_b, d.bias_h, d.bias_i = bias.stride(0), bias.stride(1), bias.stride(2)
-            self.keep.append(bias)
+                bias = _bias_rows(bias, tc)
+            b, h, i, _ = bias.stride()
+            self.bias, self.bias_args = bias, (bias.data_ptr(), b, h, i, full[0], full[1])
         if key_mask is not None:
             if tuple(key_mask.shape) != (B, Lk):
                 raise ValueError(f"key_mask must be [B, Lk] = {(B, Lk)}, got {tuple(key_mask.shape)}")
-            if key_mask.device != q.device:
-                raise ValueError(f"key_mask is on {key_mask.device}, q on {q.device}")
+            if key_mask.device != device:
+                raise ValueError(f"key_mask is on {key_mask.device}, q on {device}")
             m = _mask_bytes(key_mask)
-            d.mask, d.mask_b = m.data_ptr(), m.stride(0)
-            self.keep.append(m)
-        self.desc = d
+            self.mask, self.mask_args = m, (m.data_ptr(), m.stride(0))
 
-    def _bias_rows(self, bias):
-        """The bias with contiguous rows; for the tensor-core kernels, which fetch it in tiles, with rows on 16-byte
-        boundaries (a copy where they are not, as ``relative_position_bias_b200`` never needs)."""
-        rows_ok = bias.shape[3] == 1 or bias.stride(3) == 1
-        if self.tensor_cores:
-            fine = rows_ok and bias.data_ptr() % 16 == 0 and all(
-                n == 1 or (s % 8 == 0 and s > 0) for n, s in zip(bias.shape[:3], bias.stride()[:3]))
-            if not fine:
-                wide = _rows_of(bias.shape, bias.dtype, bias.device)
-                wide.copy_(bias)
-                return wide
-            return bias
-        return bias if rows_ok and all(s >= 0 for s in bias.stride()) else bias.contiguous()
+    def pack(self, o, stats, o_lo, dout=_NONE, dq=_NONE, dk=_NONE, dv=_NONE, dbias=_NONE) -> bytes:
+        """``trimul_attn_desc``; ``o`` ... ``dv`` as ``_tensor`` gives them."""
+        return _lib.ATTN_DESC.pack(*self.head, *_tensor(self.q), *_tensor(self.k), *_tensor(self.v), *o, *dout, *dq, *dk, *dv,
+                                   *self.bias_args, *self.mask_args, stats, o_lo, *dbias)
 
     def status(self):
         """The device's status words; none where a capture would have to create them."""
@@ -128,11 +121,33 @@ class _Call:
             return None
         return _status_words(self.device).data_ptr()
 
-    def workspace(self, backward):
-        n = C.c_size_t()
-        _lib.check(_lib.load().trimul_b200_attn_workspace_bytes(C.byref(self.desc), int(backward), C.byref(n)),
-                   "trimul_b200_attn_workspace_bytes")
-        return torch.empty(n.value, dtype=torch.uint8, device=self.device) if n.value else None
+    def workspace(self, desc: bytes, backward: bool, bias_grad: bool = False):
+        """Scratch memory of its own for every call: calls on several streams, and graphs replayed side by side, share none."""
+        key = (self.head, bias_grad, self.mask is not None, self.bias_args[4:], backward)
+        n = _workspace_sizes.get(key)
+        if n is None:
+            size = C.c_size_t()
+            _lib.check(_lib.load().trimul_b200_attn_workspace_bytes(desc, int(backward), C.byref(size)),
+                       "trimul_b200_attn_workspace_bytes")
+            n = size.value
+            if len(_workspace_sizes) >= 1024:
+                _workspace_sizes.clear()
+            _workspace_sizes[key] = n
+        return torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+
+
+def _bias_rows(bias, tensor_cores):
+    """The bias with contiguous rows; for the tensor-core kernels, which fetch it in tiles, with rows on 16-byte
+    boundaries (a copy where they are not, as ``relative_position_bias_b200`` never needs)."""
+    rows_ok = bias.shape[3] == 1 or bias.stride(3) == 1
+    if tensor_cores:
+        if rows_ok and bias.data_ptr() % 16 == 0 and all(
+                n == 1 or (s % 8 == 0 and s > 0) for n, s in zip(bias.shape[:3], bias.stride()[:3])):
+            return bias
+        wide = _rows_of(bias.shape, bias.dtype, bias.device)
+        wide.copy_(bias)
+        return wide
+    return bias if rows_ok and all(s >= 0 for s in bias.stride()) else bias.contiguous()
 
 
 def _rows_of(shape, dtype, device):
@@ -146,7 +161,7 @@ def _rows_of(shape, dtype, device):
 def _forward(call: _Call, q, state: bool):
     B, Lq, Lk, H, Hk, D = call.sizes
     with _on_device(call.device):
-        out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=call.device)
+        out = q.new_empty((B, Lq, H, D))
         rows = torch.empty((B, H, Lq, 2), dtype=torch.float32, device=call.device) if state else None
         rounding = torch.empty_like(out) if state and call.code == _lib.DTYPE_BF16 else None
         kept = AttentionState(rows, rounding) if state else None
@@ -156,12 +171,9 @@ def _forward(call: _Call, q, state: bool):
                 if rounding is not None:
                     rounding.zero_()
             return out.zero_(), kept
-        d = call.desc
-        d.o = _tensor(out)
-        d.stats = rows.data_ptr() if state else None
-        d.o_lo = rounding.data_ptr() if rounding is not None else None
-        ws = call.workspace(False)
-        rc = _lib.load().trimul_b200_attn_forward(C.byref(d), ws.data_ptr() if ws is not None else None,
+        desc = call.pack(_tensor(out), rows.data_ptr() if state else 0, rounding.data_ptr() if rounding is not None else 0)
+        ws = call.workspace(desc, False)
+        rc = _lib.load().trimul_b200_attn_forward(desc, ws.data_ptr() if ws is not None else None,
                                                   ws.numel() if ws is not None else 0, _stream_handle(call.device),
                                                   call.status())
     _lib.check(rc, "trimul_b200_attn_forward")
@@ -207,17 +219,14 @@ def cross_attention_backward_b200(grad: torch.Tensor, q: torch.Tensor, k: torch.
                 if t is not None:
                     t.zero_()
             return dq, dk, dv, dbias
-        d = call.desc
-        d.o, d.dout, d.dq, d.dk, d.dv = _tensor(out), _tensor(grad), _tensor(dq), _tensor(dk), _tensor(dv)
-        d.stats = rows.data_ptr()
-        d.o_lo = rounding.data_ptr() if rounding is not None else None
+        dbias_args = _NONE
         if want:
             full = dbias[(None,) * (4 - dbias.dim())]
-            d.dbias = full.data_ptr()
-            d.dbias_b, d.dbias_h, d.dbias_i = full.stride(0), full.stride(1), full.stride(2)
-        ws = call.workspace(True)
-        rc = _lib.load().trimul_b200_attn_backward(C.byref(d), ws.data_ptr(), ws.numel(), _stream_handle(call.device),
-                                                   call.status())
+            dbias_args = (full.data_ptr(), *full.stride()[:3])
+        desc = call.pack(_tensor(out), rows.data_ptr(), rounding.data_ptr() if rounding is not None else 0, _tensor(grad),
+                         _tensor(dq), _tensor(dk), _tensor(dv), dbias_args)
+        ws = call.workspace(desc, True, want)
+        rc = _lib.load().trimul_b200_attn_backward(desc, ws.data_ptr(), ws.numel(), _stream_handle(call.device), call.status())
     _lib.check(rc, "trimul_b200_attn_backward")
     return dq, dk, dv, dbias
 

@@ -14,6 +14,7 @@
 #include "attn_bwd_sm100.cuh"
 #include "attn_fwd_sm100.cuh"
 #include "attn_plain.cuh"
+#include "attn_short.cuh"
 #include "relpos_kernels.cuh"
 
 using namespace trimul;
@@ -104,20 +105,21 @@ int run_relpos_forward(const trimul_relpos_desc* d, const trimul_buckets* b, con
     }
     // 16-byte pieces of channels where the tensors allow them
     const bool vec = (d->channels % kN) == 0 && aligned(add, 16) && aligned(out, 16) && aligned(p.table, 16);
-    const int lanes = std::min(vec ? d->channels / kN : d->channels, kRpPairThreads), side = kRpPairThreads / lanes;
+    const int per_pos = vec ? d->channels / kN : d->channels;
     const int64_t total = (int64_t)d->B * d->Lq * d->Lk;
-    const int64_t per_block = align_up(std::max<int64_t>(ceil_div(total, 8 * (int64_t)sm_count()), 4 * side), 4 * side);
+    // eight pieces a thread at least, then as many positions as make all blocks resident at once
+    const int64_t per_block = std::max<int64_t>(ceil_div(total, 8 * (int64_t)sm_count()), ceil_div(8 * kRpPairThreads, per_pos));
     if (per_block > (1 << 30)) return TRIMUL_E_UNSUPPORTED;
     const dim3 grid((unsigned)ceil_div(total, per_block));
     auto kernel = vec ? relpos_pair_kernel<T, true> : relpos_pair_kernel<T, false>;
-    if (!ensure_smem(kernel, lut_bytes(TRIMUL_MAX_LUT))) return TRIMUL_E_CUDA;
-    return launch_stage(kernel, grid, kRpPairThreads, lut_bytes(p.M), st, true, p, *b, static_cast<const T*>(add),
+    if (!ensure_smem(kernel, lut_bytes(TRIMUL_MAX_LUT) + 4 * kRpPairThreads)) return TRIMUL_E_CUDA;
+    return launch_stage(kernel, grid, kRpPairThreads, lut_bytes(p.M) + 4 * kRpPairThreads, st, true, p, *b, static_cast<const T*>(add),
                         static_cast<T*>(out), (int)per_block);
 }
 
 // Launch shape of the gradient: `parts` partial tables of rows * channels sums each.
 struct RelposGradPlan {
-    int threads, smem, parts, lane_channels, column_blocks;
+    int threads, smem, parts, lane_channels, column_blocks, parts_per_b;
     int64_t per_part;          // rows (heads) or positions of a warp (pair)
 };
 RelposGradPlan plan_relpos_grad(const trimul_relpos_desc* d, const trimul_buckets* b, bool wide_lanes) {
@@ -127,18 +129,19 @@ RelposGradPlan plan_relpos_grad(const trimul_relpos_desc* d, const trimul_bucket
     if (d->layout == TRIMUL_RELPOS_HEADS) {
         g.threads = 128;
         while (g.threads > 32 && rows * g.threads * 4 > 96 * 1024) g.threads /= 2;
-        g.smem = rows * g.threads * 4 + lut;
-        const int64_t all = (int64_t)d->B * d->Lq;
+        // eight blocks on every SM, parts of at least four steps and at most 1024 rows (whose positions a block keeps)
         const int nch = (int)ceil_div(d->Lk, kN), side = std::max(1, g.threads / std::min(nch, g.threads));
-        int64_t parts = std::max<int64_t>(1, 4 * (int64_t)sm_count() / d->channels);
-        g.per_part = align_up(std::max<int64_t>(ceil_div(all, parts), 4 * side), side);
-        g.parts = (int)ceil_div(all, g.per_part);
+        const int64_t parts = std::max<int64_t>(1, 8 * (int64_t)sm_count() / d->channels / d->B);
+        g.per_part = std::min<int64_t>(1024, std::max<int64_t>(ceil_div(d->Lq, parts), std::min<int64_t>(16 * side, d->Lq)));
+        g.parts_per_b = (int)ceil_div(d->Lq, g.per_part);
+        g.parts = d->B * g.parts_per_b;
+        g.smem = rows * g.threads * 4 + (int)g.per_part * 8 + lut;
         return g;
     }
     const int64_t total = (int64_t)d->B * d->Lq * d->Lk;
     g.lane_channels = wide_lanes && rows * 128 * 4 + lut <= kMaxSmem ? 4 : 1;
     const int copy = rows * 32 * g.lane_channels * 4;
-    int warps = std::min(8, (kMaxSmem - lut) / copy);
+    const int warps = std::min(8, (kMaxSmem - lut) / copy);
     g.threads = 32 * warps;
     g.smem = warps * copy + lut;
     g.column_blocks = (int)ceil_div(d->channels, 32 * g.lane_channels);
@@ -160,7 +163,7 @@ int run_relpos_grad(const trimul_relpos_desc* d, const trimul_buckets* b, const 
         auto kernel = vec ? relpos_heads_grad_kernel<T, true> : relpos_heads_grad_kernel<T, false>;
         if (!ensure_smem(kernel, kMaxSmem)) return TRIMUL_E_CUDA;
         rc = launch_stage(kernel, dim3((unsigned)g.parts, (unsigned)d->channels), g.threads, g.smem, st, true, p, *b,
-                          static_cast<const T*>(grad), partial, (int)g.per_part);
+                          static_cast<const T*>(grad), partial, g.parts_per_b, (int)g.per_part);
     } else {
         auto kernel = g.lane_channels == 4 ? relpos_pair_grad_kernel<T, 4> : relpos_pair_grad_kernel<T, 1>;
         if (!ensure_smem(kernel, kMaxSmem)) return TRIMUL_E_CUDA;
@@ -251,6 +254,25 @@ bool encode_bias(CUtensorMap* map, const trimul_attn_desc* d) {
                        d->bias_batch);
 }
 
+// Few query rows per key head: the kernel that reads keys and values once for all of them.  Its rows are 16-byte pieces.
+constexpr int kShortRows = 8;
+bool short_sizes(const trimul_attn_desc* d) {
+    const int n = 16 / elem_size(d->dtype);
+    return (d->flags & TRIMUL_ATTN_FLAG_PLAIN) == 0 && (int64_t)d->Lq * (d->H / d->Hk) <= kShortRows && (d->D % n) == 0 && d->D <= 32 * n;
+}
+bool short_rows(const trimul_attn_desc* d) {
+    const int n = 16 / elem_size(d->dtype);
+    auto ok = [&](const trimul_attn_tensor& t) {
+        return aligned(t.p, 16) && (t.l % n) == 0 && (t.h % n) == 0 && (t.b % n) == 0;
+    };
+    return short_sizes(d) && ok(d->k) && ok(d->v);
+}
+// Enough blocks for four on every SM, and keys for two steps of every warp.
+int short_splits(const trimul_attn_desc* d) {
+    const int64_t blocks = (int64_t)d->B * d->Hk;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(4 * sm_count() / blocks, d->Lk / 256));
+}
+
 // Key splits of the forward pass: where the blocks leave SMs idle, each block takes a share of the key tiles (two at
 // least: a lone tile's products and exponentials do not overlap) and a second kernel joins the parts.
 int forward_splits(const trimul_attn_desc* d) {
@@ -260,10 +282,10 @@ int forward_splits(const trimul_attn_desc* d) {
 }
 
 // Workspace.  Both directions: the key mask as bits and its list of tiles.  Forward: the parts of split rows.  Backward:
-// delta, then the scores' gradients where the bias's gradient sums them.
+// delta, then the scores' gradients where the bias's gradient sums them.  Depends on sizes, type, flags, the shape of the bias and
+// on whether there are a mask and a gradient of the bias, not on addresses or strides.
 struct AttnWorkspace {
     int64_t words, list, part_o, part_ml, delta, ds, ds_pitch, total;
-    int splits;
 };
 AttnWorkspace attn_workspace(const trimul_attn_desc* d, bool backward) {
     AttnWorkspace w = {};
@@ -276,9 +298,10 @@ AttnWorkspace attn_workspace(const trimul_attn_desc* d, bool backward) {
         w.list = at;
         at += align_up(d->B * (tiles + 1) * 4, 256);
     }
-    w.splits = tc && !backward ? forward_splits(d) : 1;
-    if (w.splits > 1) {
-        const int64_t rows = (int64_t)w.splits * d->B * d->H * d->Lq;
+    // by sizes alone, so that a caller may keep the answer: room for either kernel's parts
+    const int splits = backward ? 1 : std::max(short_sizes(d) ? short_splits(d) : 1, tc ? forward_splits(d) : 1);
+    if (splits > 1) {
+        const int64_t rows = (int64_t)splits * d->B * d->H * d->Lq;
         w.part_o = at;
         at += align_up(rows * d->D * 4, 256);
         w.part_ml = at;
@@ -325,6 +348,39 @@ int run_mask(const trimul_attn_desc* d, uint32_t* words, int* list, cudaStream_t
                         (int)ceil_div(d->Lk, kAfRows), words, list);
 }
 
+template <typename T>
+int run_combine(const AttnParams& p, const float* part_o, const float2* part_ml, int splits, cudaStream_t st) {
+    const int64_t rows = (int64_t)p.B * p.H * p.Lq;
+    return launch_stage(attn_combine_kernel<T>, dim3((unsigned)ceil_div(rows, 8)), 256, 0, st, true, p, part_o, part_ml, splits);
+}
+
+template <typename T, int kLanes>
+int launch_short(const AttnShortParams& sp, int rows, cudaStream_t st) {
+    auto kernel = rows <= 1 ? attn_short_kernel<T, kLanes, 1> : rows <= 2 ? attn_short_kernel<T, kLanes, 2>
+                : rows <= 4 ? attn_short_kernel<T, kLanes, 4> : attn_short_kernel<T, kLanes, 8>;
+    return launch_stage(kernel, dim3((unsigned)sp.splits, (unsigned)sp.a.Hk, (unsigned)sp.a.B), kAsThreads, 0, st,
+                        true, sp);
+}
+template <typename T>
+int run_short(const trimul_attn_desc* d, const AttnParams& p, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
+    AttnShortParams sp = {};
+    sp.a = p;
+    sp.splits = short_splits(d);
+    sp.keys_per_split = (int)ceil_div(d->Lk, sp.splits);
+    if (sp.splits > 1) {
+        sp.part_o = reinterpret_cast<float*>(ws + w.part_o);
+        sp.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
+    }
+    const int rows = d->Lq * (d->H / d->Hk), pieces = d->D / (16 / (int)sizeof(T));
+    int rc;
+    if (pieces <= 4) rc = launch_short<T, 4>(sp, rows, st);
+    else if (pieces <= 8) rc = launch_short<T, 8>(sp, rows, st);
+    else if (pieces <= 16) rc = launch_short<T, 16>(sp, rows, st);
+    else rc = launch_short<T, 32>(sp, rows, st);
+    if (rc != TRIMUL_OK || sp.splits == 1) return rc;
+    return run_combine<T>(p, sp.part_o, sp.part_ml, sp.splits, st);
+}
+
 template <int kD, bool kBias>
 int launch_fwd(const AttnFwdParams& fp, const CUtensorMap (&m)[4], cudaStream_t st) {
     using L = AfLayout<kD, kBias>;
@@ -337,11 +393,11 @@ int run_fwd(const trimul_attn_desc* d, const AttnParams& p, const AttnWorkspace&
     AttnFwdParams fp = {};
     fp.a = p;
     fp.n_tiles = (int)ceil_div(d->Lk, kAfRows);
-    fp.splits = w.splits;
-    fp.tiles_per_split = (int)ceil_div(fp.n_tiles, w.splits);
+    fp.splits = forward_splits(d);
+    fp.tiles_per_split = (int)ceil_div(fp.n_tiles, fp.splits);
     fp.bias_b1 = d->bias_batch == 1;
     fp.bias_h1 = d->bias_heads == 1;
-    if (w.splits > 1) {
+    if (fp.splits > 1) {
         fp.part_o = reinterpret_cast<float*>(ws + w.part_o);
         fp.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
     }
@@ -362,10 +418,8 @@ int run_fwd(const trimul_attn_desc* d, const AttnParams& p, const AttnWorkspace&
     int rc;
     if (d->D <= 64) rc = d->bias != nullptr ? launch_fwd<64, true>(fp, m, st) : launch_fwd<64, false>(fp, m, st);
     else rc = d->bias != nullptr ? launch_fwd<128, true>(fp, m, st) : launch_fwd<128, false>(fp, m, st);
-    if (rc != TRIMUL_OK || w.splits == 1) return rc;
-    const int64_t rows = (int64_t)d->B * d->H * d->Lq;
-    return launch_stage(attn_combine_kernel<__nv_bfloat16>, dim3((unsigned)ceil_div(rows, 8)), 256, 0, st, true, p,
-                        static_cast<const float*>(fp.part_o), static_cast<const float2*>(fp.part_ml), w.splits);
+    if (rc != TRIMUL_OK || fp.splits == 1) return rc;
+    return run_combine<__nv_bfloat16>(p, fp.part_o, fp.part_ml, fp.splits, st);
 }
 
 template <int kD, bool kBias>
@@ -475,6 +529,9 @@ int trimul_b200_attn_forward(const trimul_attn_desc* d, void* workspace, size_t 
     if (workspace_bytes < (size_t)w.total) return TRIMUL_E_WORKSPACE;
     const AttnParams p = attn_params(d, status);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (short_rows(d))
+        return d->dtype == TRIMUL_DTYPE_BF16 ? run_short<__nv_bfloat16>(d, p, w, static_cast<uint8_t*>(workspace), st)
+                                             : run_short<float>(d, p, w, static_cast<uint8_t*>(workspace), st);
     if (tensor_core_forward(d)) return run_fwd(d, p, w, static_cast<uint8_t*>(workspace), st);
     return d->dtype == TRIMUL_DTYPE_BF16 ? run_plain_fwd<__nv_bfloat16>(p, st) : run_plain_fwd<float>(p, st);
 }

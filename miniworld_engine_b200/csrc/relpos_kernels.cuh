@@ -159,8 +159,9 @@ relpos_heads_kernel(const __grid_constant__ RelposParams p, const __grid_constan
 }
 
 // ---------------------------------------------------------------------------------------
-// pair, forward.  A thread owns 16 bytes of a position's channels (kVec; else single channels), a block a run of
-// consecutive positions; the table's rows come through L1 (a few buckets are live at a time).
+// pair, forward.  A block takes runs of kRpPairThreads consecutive positions: first each thread finds the bucket of one
+// position, then all stream the run's channels, 16 bytes a piece (kVec; else single channels), eight pieces in flight each;
+// the table's rows come through L1 (a few buckets are live at a time).
 // ---------------------------------------------------------------------------------------
 constexpr int kRpPairThreads = 256;
 
@@ -193,71 +194,76 @@ __global__ void __launch_bounds__(kRpPairThreads)
 relpos_pair_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule, const T* add, T* out,
                    int per_block) {
     constexpr int kN = kVec ? RpVec<T>::kN : 1;
-    constexpr int kU = 4;
+    constexpr int kU = 8;
     extern __shared__ __align__(16) uint8_t rp_smem[];
-    uint16_t* lut = reinterpret_cast<uint16_t*>(rp_smem);
+    int* su = reinterpret_cast<int*>(rp_smem);                                 // buckets of kRpPairThreads positions
+    uint16_t* lut = reinterpret_cast<uint16_t*>(su + kRpPairThreads);
     rp_build_lut(lut, rule, p.M);
     griddep_wait();
     griddep_launch_dependents();
-    __syncthreads();
-    // lanes of one position side by side; wide tensors take several passes over the channels
-    const int per_pos = p.C / kN;
-    const int lanes = min(per_pos, kRpPairThreads);
-    const int side = kRpPairThreads / lanes;                  // positions at once
-    const int ty = threadIdx.x / lanes, tx = threadIdx.x % lanes;
-    if (ty >= side) return;
     const long long total = (long long)p.B * p.Lq * p.Lk;
     const long long first = (long long)blockIdx.x * per_block, last = min(first + per_block, total);
-    long long pos = first + ty;
-    if (pos >= last) return;
+    const int per_pos = p.C / kN;
     RpCursor cur;
-    cur.init(p, pos);
-    while (pos < last) {
-        int u[kU];
-        const int n = (int)min((long long)kU, (last - pos + side - 1) / side);
-#pragma unroll
-        for (int s = 0; s < kU; ++s) {
-            if (s < n) {
-                u[s] = cur.bucket(p, lut);
-                cur.step(p, side);
-            }
+    if (first + threadIdx.x < last) cur.init(p, first + threadIdx.x);
+    // vector v of a run is channel piece v % per_pos of position v / per_pos: stepped, not divided
+    const int step_pos = kRpPairThreads / per_pos, step_c = kRpPairThreads % per_pos;
+    for (long long pos = first; pos < last; pos += kRpPairThreads) {
+        const int n = (int)min((long long)kRpPairThreads, last - pos);
+        __syncthreads();
+        if ((int)threadIdx.x < n) {
+            su[threadIdx.x] = cur.bucket(p, lut);
+            cur.step(p, kRpPairThreads);
         }
-        for (int v = tx; v < per_pos; v += lanes) {
+        __syncthreads();
+        const long long base = pos * per_pos;
+        const int vectors = n * per_pos;
+        int x = threadIdx.x / per_pos, c = threadIdx.x % per_pos;
+        for (int v0 = threadIdx.x; v0 < vectors; v0 += kU * kRpPairThreads) {
             if constexpr (kVec) {
                 uint4 a[kU];
 #pragma unroll
-                for (int s = 0; s < kU; ++s)
-                    if (s < n)
-                        a[s] = add != nullptr ? __ldcs(reinterpret_cast<const uint4*>(add + (pos + (long long)s * side) * p.C) + v)
-                                              : make_uint4(0u, 0u, 0u, 0u);
+                for (int s = 0; s < kU; ++s) {
+                    const int v = v0 + s * kRpPairThreads;
+                    a[s] = add != nullptr && v < vectors ? __ldcs(reinterpret_cast<const uint4*>(add) + base + v)
+                                                         : make_uint4(0u, 0u, 0u, 0u);
+                }
 #pragma unroll
-                for (int s = 0; s < kU; ++s)
-                    if (s < n) {
+                for (int s = 0; s < kU; ++s) {
+                    const int v = v0 + s * kRpPairThreads;
+                    if (v < vectors) {
+                        const long long t0 = (long long)su[x] * p.C + c * kN;
                         float f[kN];
                         RpVec<T>::unpack(a[s], f);
                         if (p.table_bf16) {
 #pragma unroll
-                            for (int e = 0; e < kN; ++e) f[e] += rp_table(p, u[s], v * kN + e);
+                            for (int e = 0; e < kN; ++e) f[e] += __bfloat162float(static_cast<const __nv_bfloat16*>(p.table)[t0 + e]);
                         } else {
-                            const float4* t = reinterpret_cast<const float4*>(static_cast<const float*>(p.table) + (long long)u[s] * p.C + v * kN);
+                            const float4* t = reinterpret_cast<const float4*>(static_cast<const float*>(p.table) + t0);
 #pragma unroll
                             for (int e = 0; e < kN / 4; ++e) {
                                 const float4 w = __ldg(t + e);
                                 f[4 * e] += w.x; f[4 * e + 1] += w.y; f[4 * e + 2] += w.z; f[4 * e + 3] += w.w;
                             }
                         }
-                        __stcs(reinterpret_cast<uint4*>(out + (pos + (long long)s * side) * p.C) + v, RpVec<T>::pack(f));
+                        __stcs(reinterpret_cast<uint4*>(out) + base + v, RpVec<T>::pack(f));
                     }
+                    x += step_pos;
+                    c += step_c;
+                    if (c >= per_pos) { c -= per_pos; ++x; }
+                }
             } else {
 #pragma unroll
-                for (int s = 0; s < kU; ++s)
-                    if (s < n) {
-                        const long long at = (pos + (long long)s * side) * p.C + v;
-                        rp_store(out + at, (add != nullptr ? rp_float(add[at]) : 0.f) + rp_table(p, u[s], v));
-                    }
+                for (int s = 0; s < kU; ++s) {
+                    const int v = v0 + s * kRpPairThreads;
+                    if (v < vectors)
+                        rp_store(out + base + v, (add != nullptr ? rp_float(add[base + v]) : 0.f) + rp_table(p, su[x], c));
+                    x += step_pos;
+                    c += step_c;
+                    if (c >= per_pos) { c -= per_pos; ++x; }
+                }
             }
         }
-        pos += (long long)n * side;
     }
 }
 
@@ -268,14 +274,14 @@ relpos_pair_kernel(const __grid_constant__ RelposParams p, const __grid_constant
 // side of zero, so everything between shares it too), the piece is summed in registers.
 // ---------------------------------------------------------------------------------------
 template <typename T, bool kVec>
-__global__ void relpos_heads_grad_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule,
-                                         const T* grad, float* partial, int rows_per_part) {
+__global__ void __launch_bounds__(kRpThreads) relpos_heads_grad_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule,
+                                         const T* grad, float* partial, int parts_per_b, int rows_per_part) {
     constexpr int kN = RpVec<T>::kN;
     constexpr int kU = 4;
     extern __shared__ __align__(16) uint8_t rp_smem[];
     float* acc = reinterpret_cast<float*>(rp_smem);                               // [rows][threads]
     const int nt = blockDim.x, tid = threadIdx.x;
-    uint16_t* lut = reinterpret_cast<uint16_t*>(rp_smem + (size_t)p.rows * nt * 4);
+    uint16_t* lut = reinterpret_cast<uint16_t*>(rp_smem + (size_t)p.rows * nt * 4 + rows_per_part * 8);
     rp_build_lut(lut, rule, p.M);
     for (int u = 0; u < p.rows; ++u) acc[u * nt + tid] = 0.f;
     griddep_wait();
@@ -286,8 +292,16 @@ __global__ void relpos_heads_grad_kernel(const __grid_constant__ RelposParams p,
     const int tpr = min(nch, nt);                             // threads of one row
     const int side = nt / tpr;                                // rows at once
     const int ty = tid / tpr, tx = tid % tpr;
-    const long long rows = (long long)p.B * p.Lq;
-    const long long r0 = (long long)blockIdx.x * rows_per_part, r1 = min(r0 + rows_per_part, rows);
+    const int b = blockIdx.x / parts_per_b;
+    const int r0 = (blockIdx.x - b * parts_per_b) * rows_per_part, r1 = min(r0 + rows_per_part, p.Lq);
+    const T* gb = grad + b * p.sB + h * p.sH;
+    // the part's query positions and segments
+    int* sq = reinterpret_cast<int*>(rp_smem + (size_t)p.rows * nt * 4);
+    for (int i = tid; i < r1 - r0; i += nt) {
+        sq[i] = rp_load(p.q_pos, b * p.q_pos_b + r0 + i, p.q_pos64);
+        sq[rows_per_part + i] = p.q_seg != nullptr ? rp_load(p.q_seg, b * p.q_seg_b + r0 + i, p.q_seg64) : 0;
+    }
+    __syncthreads();
     int run = 0;
     float sum = 0.f;
     auto put = [&](int u, float v) {
@@ -300,73 +314,58 @@ __global__ void relpos_heads_grad_kernel(const __grid_constant__ RelposParams p,
     };
     if (ty < side) {
         for (int c = tx; c < nch; c += tpr) {
-            const int j0 = c * kN;
-            const int nj = min(kN, p.Lk - j0);
-            int kp[kN], ks[kN], kmin = 0, kmax = 0;
+            const int j0 = c * kN, nj = min(kN, p.Lk - j0);
+            int kp[kN], ks[kN];
+#pragma unroll
+            for (int e = 0; e < kN; ++e) {
+                const int j = min(j0 + e, p.Lk - 1);
+                kp[e] = rp_load(p.k_pos, b * p.k_pos_b + j, p.k_pos64);
+                ks[e] = p.k_seg != nullptr ? rp_load(p.k_seg, b * p.k_seg_b + j, p.k_seg64) : 0;
+            }
+            int kmin = kp[0], kmax = kp[0];
             bool one_seg = true;
-            int b_now = -1;
-            for (long long r = r0 + ty; r < r1; r += (long long)kU * side) {
-                float g[kU][kN];
-                if constexpr (kVec) {
-                    uint4 raw[kU];
+#pragma unroll
+            for (int e = 1; e < kN; ++e) {
+                kmin = min(kmin, kp[e]);
+                kmax = max(kmax, kp[e]);
+                one_seg = one_seg && ks[e] == ks[0];
+            }
+            const T* src = gb + j0;
+            for (int r = r0 + ty; r < r1; r += kU * side) {
+                uint4 raw[kU];
+                if (kVec && nj == kN) {
+#pragma unroll
+                    for (int s = 0; s < kU; ++s)
+                        raw[s] = r + s * side < r1 ? __ldcs(reinterpret_cast<const uint4*>(src + (r + s * side) * p.sI))
+                                                   : make_uint4(0u, 0u, 0u, 0u);
+                } else {
 #pragma unroll
                     for (int s = 0; s < kU; ++s) {
-                        const long long rr = r + (long long)s * side;
-                        raw[s] = make_uint4(0u, 0u, 0u, 0u);
-                        if (rr < r1 && nj == kN) {
-                            const int b = (int)(rr / p.Lq), i = (int)(rr - (long long)b * p.Lq);
-                            raw[s] = __ldcs(reinterpret_cast<const uint4*>(grad + b * p.sB + h * p.sH + i * p.sI + j0));
-                        }
-                    }
+                        const T* row = src + (r + s * side) * p.sI;
+                        float g[kN];
 #pragma unroll
-                    for (int s = 0; s < kU; ++s) RpVec<T>::unpack(raw[s], g[s]);
-                }
-                if (!kVec || nj < kN) {
-#pragma unroll
-                    for (int s = 0; s < kU; ++s) {
-                        const long long rr = r + (long long)s * side;
-                        const int b = (int)(rr / p.Lq), i = (int)(rr - (long long)b * p.Lq);
-                        const T* src = grad + b * p.sB + h * p.sH + i * p.sI + j0;
-#pragma unroll
-                        for (int e = 0; e < kN; ++e) g[s][e] = rr < r1 && e < nj ? rp_float(src[e]) : 0.f;
+                        for (int e = 0; e < kN; ++e) g[e] = r + s * side < r1 && e < nj ? rp_float(row[e]) : 0.f;
+                        raw[s] = RpVec<T>::pack(g);
                     }
                 }
 #pragma unroll
                 for (int s = 0; s < kU; ++s) {
-                    const long long rr = r + (long long)s * side;
+                    const int rr = r + s * side;
                     if (rr >= r1) break;
-                    const int b = (int)(rr / p.Lq), i = (int)(rr - (long long)b * p.Lq);
-                    if (b != b_now) {
-                        b_now = b;
-#pragma unroll
-                        for (int e = 0; e < kN; ++e) {
-                            const int j = min(j0 + e, p.Lk - 1);
-                            kp[e] = rp_load(p.k_pos, b * p.k_pos_b + j, p.k_pos64);
-                            ks[e] = p.k_seg != nullptr ? rp_load(p.k_seg, b * p.k_seg_b + j, p.k_seg64) : 0;
-                        }
-                        kmin = kmax = kp[0];
-                        one_seg = true;
-#pragma unroll
-                        for (int e = 1; e < kN; ++e) {
-                            kmin = min(kmin, kp[e]);
-                            kmax = max(kmax, kp[e]);
-                            one_seg = one_seg && ks[e] == ks[0];
-                        }
-                    }
-                    const int q = rp_load(p.q_pos, b * p.q_pos_b + i, p.q_pos64);
-                    const int qs = p.q_seg != nullptr ? rp_load(p.q_seg, b * p.q_seg_b + i, p.q_seg64) : 0;
+                    float g[kN];
+                    RpVec<T>::unpack(raw[s], g);
+                    const int q = sq[rr - r0], qs = sq[rows_per_part + rr - r0];
                     const bool apart = one_seg && ks[0] != qs;
                     const int ulo = rp_bucket(lut, p.M, q - kmax), uhi = rp_bucket(lut, p.M, q - kmin);
-                    // d >= 0 and d < 0 may share a bucket only where everything between does (one-sided rules)
                     if (apart || (one_seg && ulo == uhi)) {
-                        float t = 0.f;
+                        float t = g[0];
 #pragma unroll
-                        for (int e = 0; e < kN; ++e) t += g[s][e];
+                        for (int e = 1; e < kN; ++e) t += g[e];
                         put(apart ? p.rows - 1 : ulo, t);
                     } else {
 #pragma unroll
                         for (int e = 0; e < kN; ++e) {
-                            if (e < nj) put(ks[e] != qs ? p.rows - 1 : rp_bucket(lut, p.M, q - kp[e]), g[s][e]);
+                            if (e < nj) put(ks[e] != qs ? p.rows - 1 : rp_bucket(lut, p.M, q - kp[e]), g[e]);
                         }
                     }
                 }
@@ -391,22 +390,63 @@ __global__ void relpos_heads_grad_kernel(const __grid_constant__ RelposParams p,
 // and a private set of sums [rows][32 kL] in shared memory; the running bucket's sum stays in registers until the bucket
 // changes (the test is uniform over the warp).
 // ---------------------------------------------------------------------------------------
-template <typename T, int kL>
-__device__ __forceinline__ void rp_load_lane(const T* p, float (&f)[kL]) {
-    if constexpr (kL == 1) f[0] = rp_float(p[0]);
-    else if constexpr (sizeof(T) == 2) {
-        const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
-        f[0] = bf16_lo(v.x); f[1] = bf16_hi(v.x); f[2] = bf16_lo(v.y); f[3] = bf16_hi(v.y);
-    } else {
-        const float4 v = __ldcs(reinterpret_cast<const float4*>(p));
-        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-    }
+template <typename T, int kL> struct RpLane { using V = T; };             // kL channels of a lane
+template <> struct RpLane<__nv_bfloat16, 4> { using V = uint2; };
+template <> struct RpLane<float, 4> { using V = float4; };
+__device__ __forceinline__ void rp_lane(const __nv_bfloat16& v, float (&f)[1]) { f[0] = __bfloat162float(v); }
+__device__ __forceinline__ void rp_lane(const float& v, float (&f)[1]) { f[0] = v; }
+__device__ __forceinline__ void rp_lane(const uint2& v, float (&f)[4]) {
+    f[0] = bf16_lo(v.x); f[1] = bf16_hi(v.x); f[2] = bf16_lo(v.y); f[3] = bf16_hi(v.y);
 }
+__device__ __forceinline__ void rp_lane(const float4& v, float (&f)[4]) { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+
+// `kRun` positions of one warp (their channels of this lane, and a bucket per lane).  Two of them live in registers: one is
+// added up while the other is in flight.
+template <typename T, int kL, int kRun>
+struct RpRun {
+    typename RpLane<T, kL>::V g[kRun];
+    int u, n;
+    __device__ __forceinline__ void load(const RelposParams& p, const uint16_t* lut, const T* grad, long long pos, long long last, int c0,
+                                         int lane, RpCursor& cur) {
+        n = (int)max(0ll, min((long long)kRun, last - pos));
+        const T* src = grad + pos * p.C + c0;
+#pragma unroll
+        for (int s = 0; s < kRun; ++s) {
+            g[s] = typename RpLane<T, kL>::V();
+            if (s < n && c0 < p.C) g[s] = __ldcs(reinterpret_cast<const typename RpLane<T, kL>::V*>(src + (long long)s * p.C));
+        }
+        u = 0;
+        if (lane < n) {
+            u = cur.bucket(p, lut);
+            cur.step(p, kRun);
+        }
+    }
+    __device__ __forceinline__ void add(float* acc, int& run, float (&sum)[kL]) const {
+#pragma unroll
+        for (int s = 0; s < kRun; ++s) {
+            if (s >= n) break;
+            const int us = __shfl_sync(0xffffffffu, u, s);
+            if (us != run) {
+#pragma unroll
+                for (int e = 0; e < kL; ++e) {
+                    acc[run * 32 * kL + e] += sum[e];
+                    sum[e] = 0.f;
+                }
+                run = us;
+            }
+            float f[kL];
+            rp_lane(g[s], f);
+#pragma unroll
+            for (int e = 0; e < kL; ++e) sum[e] += f[e];
+        }
+    }
+};
 
 template <typename T, int kL>
-__global__ void relpos_pair_grad_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule,
+__global__ void __launch_bounds__(256, 1)
+relpos_pair_grad_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule,
                                         const T* grad, float* partial, long long pos_per_warp) {
-    constexpr int kU = 8;
+    constexpr int kRun = sizeof(T) * kL == 16 ? 16 : 32;      // 64 registers a run
     extern __shared__ __align__(16) uint8_t rp_smem[];
     const int nt = blockDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = nt >> 5;
     float* sums = reinterpret_cast<float*>(rp_smem);                              // [warps][rows][32 kL]
@@ -417,7 +457,6 @@ __global__ void relpos_pair_grad_kernel(const __grid_constant__ RelposParams p, 
     griddep_launch_dependents();
     __syncthreads();
     const int c0 = blockIdx.y * 32 * kL + lane * kL;
-    const bool live = c0 < p.C;
     float* acc = sums + (size_t)warp * p.rows * 32 * kL + lane * kL;
     const long long total = (long long)p.B * p.Lq * p.Lk;
     const long long first = ((long long)blockIdx.x * warps + warp) * pos_per_warp, last = min(first + pos_per_warp, total);
@@ -427,37 +466,13 @@ __global__ void relpos_pair_grad_kernel(const __grid_constant__ RelposParams p, 
     for (int e = 0; e < kL; ++e) sum[e] = 0.f;
     RpCursor cur;
     if (first < last) cur.init(p, min(first + lane, total - 1));
-    for (long long pos = first; pos < last; pos += 32) {
-        const int n = (int)min(32ll, last - pos);
-        int u = 0;
-        if (lane < n) {
-            u = cur.bucket(p, lut);
-            cur.step(p, 32);
-        }
-        for (int s0 = 0; s0 < n; s0 += kU) {
-            float g[kU][kL];
-#pragma unroll
-            for (int s = 0; s < kU; ++s) {
-#pragma unroll
-                for (int e = 0; e < kL; ++e) g[s][e] = 0.f;
-                if (s0 + s < n && live) rp_load_lane<T, kL>(grad + (pos + s0 + s) * p.C + c0, g[s]);
-            }
-#pragma unroll
-            for (int s = 0; s < kU; ++s) {
-                const int us = __shfl_sync(0xffffffffu, u, (s0 + s) & 31);
-                if (s0 + s >= n) break;
-                if (us != run) {
-#pragma unroll
-                    for (int e = 0; e < kL; ++e) {
-                        acc[run * 32 * kL + e] += sum[e];
-                        sum[e] = 0.f;
-                    }
-                    run = us;
-                }
-#pragma unroll
-                for (int e = 0; e < kL; ++e) sum[e] += g[s][e];
-            }
-        }
+    RpRun<T, kL, kRun> a, b;
+    a.load(p, lut, grad, first, last, c0, lane, cur);
+    for (long long pos = first; pos < last; pos += 2 * kRun) {
+        b.load(p, lut, grad, pos + kRun, last, c0, lane, cur);
+        a.add(acc, run, sum);
+        a.load(p, lut, grad, pos + 2 * kRun, last, c0, lane, cur);
+        b.add(acc, run, sum);
     }
 #pragma unroll
     for (int e = 0; e < kL; ++e) acc[run * 32 * kL + e] += sum[e];

@@ -48,6 +48,7 @@ class PositionBuckets:
             raise NotImplementedError(f"at most {_lib.MAX_THRESHOLDS} shared buckets a side are supported, got {len(thresholds)}")
         self._struct = _lib.Buckets(kind, count, max_distance, int(self.segments), len(thresholds),
                                     (C.c_int32 * _lib.MAX_THRESHOLDS)(*thresholds))
+        self._address = C.addressof(self._struct)
 
     @staticmethod
     @functools.lru_cache(maxsize=256)
@@ -144,17 +145,22 @@ class _Call:
         self.lq, self.lk, self.channels = qp.shape[-1], kp.shape[-1], channels
         B = 1 if self.batch is None else self.batch
         self.empty = B == 0 or self.lq == 0 or self.lk == 0 or channels == 0
-        self.desc = _lib.RelposDesc(C.sizeof(_lib.RelposDesc), _LAYOUTS[layout], dtype_code, table_code, B, self.lq, self.lk,
-                                    channels, wide, 0, s0, s1, s2, s3, 0, 0, 0)
+        self.head = (_lib.RELPOS_DESC.size, _LAYOUTS[layout], dtype_code, table_code, B, self.lq, self.lk, channels, wide, 0,
+                     s0, s1, s2, s3)
 
     def shape(self, layout):
         lead = () if self.batch is None else (self.batch,)
         return (*lead, self.channels, self.lq, self.lk) if layout == "heads" else (*lead, self.lq, self.lk, self.channels)
 
-    def strides(self, t):
-        """Strides of a heads tensor into the descriptor."""
-        self.desc.stride_b = t.stride(0) if self.batch is not None else 0
-        self.desc.stride_h, self.desc.stride_i = t.stride(-3), t.stride(-2)
+    def pack(self, t=None) -> bytes:
+        """``trimul_relpos_desc``, with the strides of the heads tensor ``t``."""
+        if t is None:
+            return _lib.RELPOS_DESC.pack(*self.head, 0, 0, 0)
+        strides = t.stride()
+        return _lib.RELPOS_DESC.pack(*self.head, strides[0] if self.batch is not None else 0, strides[-3], strides[-2])
+
+
+_workspace_sizes: dict = {}      # of the library's answers, by what they depend on
 
 
 def _forward(table, buckets, q_pos, k_pos, q_segment, k_segment, layout, add, dtype):
@@ -189,13 +195,14 @@ def _forward(table, buckets, q_pos, k_pos, q_segment, k_segment, layout, add, dt
             out = torch.empty(*shape[:-1], pitch, dtype=dtype, device=device)
             if pitch != call.lk:
                 out = out[..., :call.lk]
-            call.strides(out)
+            desc = call.pack(out)
         else:
+            desc = call.pack()
             out = torch.empty(shape, dtype=dtype, device=device)
         if call.empty:
             return out
         rc = _lib.load().trimul_b200_relpos_bias(
-            C.byref(call.desc), C.byref(buckets._struct), table.data_ptr(), *call.args,
+            desc, buckets._address, table.data_ptr(), *call.args,
             add.data_ptr() if add is not None else None, out.data_ptr(), _stream_handle(device))
     _lib.check(rc, "trimul_b200_relpos_bias")
     return out
@@ -225,17 +232,24 @@ def relative_position_bias_backward_b200(grad: torch.Tensor, buckets: PositionBu
     else:
         if grad.shape[-1] > 1 and grad.stride(-1) != 1:
             grad = grad.contiguous()
-        call.strides(grad)
+    desc = call.pack(grad if layout == "heads" else None)
     with _on_device(device):
         out = torch.empty(buckets.rows, channels, dtype=dtype, device=device)
         if call.empty:
             return out.zero_()
-        lib, n = _lib.load(), C.c_size_t()
-        _lib.check(lib.trimul_b200_relpos_bias_grad_workspace_bytes(C.byref(call.desc), C.byref(buckets._struct), C.byref(n)),
-                   "trimul_b200_relpos_bias_grad_workspace_bytes")
-        ws = torch.empty(n.value, dtype=torch.uint8, device=device)
-        rc = lib.trimul_b200_relpos_bias_grad(C.byref(call.desc), C.byref(buckets._struct), *call.args, grad.data_ptr(),
-                                              out.data_ptr(), ws.data_ptr(), n.value, _stream_handle(device))
+        lib, key = _lib.load(), (call.head[:8], buckets)
+        n = _workspace_sizes.get(key)
+        if n is None:
+            size = C.c_size_t()
+            _lib.check(lib.trimul_b200_relpos_bias_grad_workspace_bytes(desc, buckets._address, C.byref(size)),
+                       "trimul_b200_relpos_bias_grad_workspace_bytes")
+            n = size.value
+            if len(_workspace_sizes) >= 1024:
+                _workspace_sizes.clear()
+            _workspace_sizes[key] = n
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
+        rc = lib.trimul_b200_relpos_bias_grad(desc, buckets._address, *call.args, grad.data_ptr(), out.data_ptr(), ws.data_ptr(),
+                                              n, _stream_handle(device))
     _lib.check(rc, "trimul_b200_relpos_bias_grad")
     return out
 
