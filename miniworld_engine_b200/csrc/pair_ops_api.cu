@@ -119,7 +119,7 @@ int run_relpos_forward(const trimul_relpos_desc* d, const trimul_buckets* b, con
 
 // Launch shape of the gradient: `parts` partial tables of rows * channels sums each.
 struct RelposGradPlan {
-    int threads, smem, parts, lane_channels, column_blocks, parts_per_b;
+    int threads, smem, parts, lane_channels, column_blocks, parts_per_b, heads;
     int64_t per_part;          // rows (heads) or positions of a warp (pair)
 };
 RelposGradPlan plan_relpos_grad(const trimul_relpos_desc* d, const trimul_buckets* b, bool wide_lanes) {
@@ -127,15 +127,21 @@ RelposGradPlan plan_relpos_grad(const trimul_relpos_desc* d, const trimul_bucket
     const int rows = b->count + (b->segments != 0), lut = lut_bytes(lut_reach(b));
     const int kN = d->dtype == TRIMUL_DTYPE_BF16 ? 8 : 4;
     if (d->layout == TRIMUL_RELPOS_HEADS) {
+        // four heads a block where three blocks' sums fit into an SM's shared memory, two where that holds for them
         g.threads = 128;
+        g.heads = d->channels >= 4 && rows * 4 * 128 * 4 <= 72 * 1024 ? 4 : d->channels >= 2 && rows * 2 * 128 * 4 <= 72 * 1024 ? 2 : 1;
         while (g.threads > 32 && rows * g.threads * 4 > 96 * 1024) g.threads /= 2;
-        // eight blocks on every SM, parts of at least four steps and at most 1024 rows (whose positions a block keeps)
-        const int nch = (int)ceil_div(d->Lk, kN), side = std::max(1, g.threads / std::min(nch, g.threads));
-        const int64_t parts = std::max<int64_t>(1, 8 * (int64_t)sm_count() / d->channels / d->B);
-        g.per_part = std::min<int64_t>(1024, std::max<int64_t>(ceil_div(d->Lq, parts), std::min<int64_t>(16 * side, d->Lq)));
+        // as many blocks as are resident at once, parts of at least four steps and at most 1024 rows (whose positions a
+        // block keeps)
+        const int sums = rows * g.heads * g.threads * 4, nch = (int)ceil_div(d->Lk, kN);
+        const int side = std::max(1, g.threads / std::min(nch, g.threads));
+        const int64_t resident = std::max(1, std::min(5, kMaxSmem / (sums + 4096)));
+        const int64_t parts = std::max<int64_t>(1, resident * sm_count() / ceil_div(d->channels, g.heads) / d->B);
+        g.per_part = std::min<int64_t>(1024, std::max<int64_t>(ceil_div(d->Lq, parts), std::min<int64_t>(16 / g.heads * side, d->Lq)));
         g.parts_per_b = (int)ceil_div(d->Lq, g.per_part);
         g.parts = d->B * g.parts_per_b;
-        g.smem = rows * g.threads * 4 + (int)g.per_part * 8 + lut;
+        g.column_blocks = (int)ceil_div(d->channels, g.heads);
+        g.smem = sums + (int)g.per_part * 8 + lut;
         return g;
     }
     const int64_t total = (int64_t)d->B * d->Lq * d->Lk;
@@ -160,9 +166,11 @@ int run_relpos_grad(const trimul_relpos_desc* d, const trimul_buckets* b, const 
     const RelposGradPlan g = plan_relpos_grad(d, b, wide);
     if (d->layout == TRIMUL_RELPOS_HEADS) {
         const bool vec = aligned(grad, 16) && (p.sB % kN) == 0 && (p.sH % kN) == 0 && (p.sI % kN) == 0;
-        auto kernel = vec ? relpos_heads_grad_kernel<T, true> : relpos_heads_grad_kernel<T, false>;
+        auto kernel = g.heads == 4 ? (vec ? relpos_heads_grad_kernel<T, true, 4> : relpos_heads_grad_kernel<T, false, 4>)
+                    : g.heads == 2 ? (vec ? relpos_heads_grad_kernel<T, true, 2> : relpos_heads_grad_kernel<T, false, 2>)
+                                   : (vec ? relpos_heads_grad_kernel<T, true, 1> : relpos_heads_grad_kernel<T, false, 1>);
         if (!ensure_smem(kernel, kMaxSmem)) return TRIMUL_E_CUDA;
-        rc = launch_stage(kernel, dim3((unsigned)g.parts, (unsigned)d->channels), g.threads, g.smem, st, true, p, *b,
+        rc = launch_stage(kernel, dim3((unsigned)g.parts, (unsigned)g.column_blocks), g.threads, g.smem, st, true, p, *b,
                           static_cast<const T*>(grad), partial, g.parts_per_b, (int)g.per_part);
     } else {
         auto kernel = g.lane_channels == 4 ? relpos_pair_grad_kernel<T, 4> : relpos_pair_grad_kernel<T, 1>;

@@ -268,49 +268,56 @@ relpos_pair_kernel(const __grid_constant__ RelposParams p, const __grid_constant
 }
 
 // ---------------------------------------------------------------------------------------
-// heads, gradient of the table.  Block (part, h) sums the rows of its part for head h.  Sums live in shared memory, one
-// column per thread: no atomics, so the result does not depend on the order of anything.  A thread keeps kN consecutive
-// j and walks down the rows; where the outermost distances of its piece share a bucket (buckets are monotone on either
-// side of zero, so everything between shares it too), the piece is summed in registers.
+// heads, gradient of the table.  Block (part, group of kH heads) sums the rows of its part.  Sums live in shared memory,
+// [rows][kH][threads]: a column per thread, no atomics, so the result does not depend on the order of anything.  A thread
+// keeps kN consecutive j and walks down the rows, all kH heads at once: the bucket of a position is found once for them.
+// Where the outermost distances of a piece share a bucket (buckets are monotone on either side of zero, so everything
+// between shares it too), the piece is summed in registers; the running bucket's sums go to shared memory when it changes.
 // ---------------------------------------------------------------------------------------
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kRpThreads) relpos_heads_grad_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule,
-                                         const T* grad, float* partial, int parts_per_b, int rows_per_part) {
+template <typename T, bool kVec, int kH>
+__global__ void __launch_bounds__(kRpThreads)
+relpos_heads_grad_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule, const T* grad,
+                         float* partial, int parts_per_b, int rows_per_part) {
     constexpr int kN = RpVec<T>::kN;
-    constexpr int kU = 4;
+    constexpr int kU = 4 / kH;
     extern __shared__ __align__(16) uint8_t rp_smem[];
-    float* acc = reinterpret_cast<float*>(rp_smem);                               // [rows][threads]
+    float* acc = reinterpret_cast<float*>(rp_smem);                               // [rows][kH][threads]
     const int nt = blockDim.x, tid = threadIdx.x;
-    uint16_t* lut = reinterpret_cast<uint16_t*>(rp_smem + (size_t)p.rows * nt * 4 + rows_per_part * 8);
+    int* sq = reinterpret_cast<int*>(acc + (size_t)p.rows * kH * nt);             // the part's query positions, then segments
+    uint16_t* lut = reinterpret_cast<uint16_t*>(sq + 2 * rows_per_part);
     rp_build_lut(lut, rule, p.M);
-    for (int u = 0; u < p.rows; ++u) acc[u * nt + tid] = 0.f;
+    for (int u = 0; u < p.rows * kH; ++u) acc[u * nt + tid] = 0.f;
     griddep_wait();
     griddep_launch_dependents();
-    __syncthreads();
-    const int h = blockIdx.y;
+    const int h0 = blockIdx.y * kH;
     const int nch = (p.Lk + kN - 1) / kN;
     const int tpr = min(nch, nt);                             // threads of one row
     const int side = nt / tpr;                                // rows at once
     const int ty = tid / tpr, tx = tid % tpr;
     const int b = blockIdx.x / parts_per_b;
-    const int r0 = (blockIdx.x - b * parts_per_b) * rows_per_part, r1 = min(r0 + rows_per_part, p.Lq);
-    const T* gb = grad + b * p.sB + h * p.sH;
-    // the part's query positions and segments
-    int* sq = reinterpret_cast<int*>(rp_smem + (size_t)p.rows * nt * 4);
-    for (int i = tid; i < r1 - r0; i += nt) {
-        sq[i] = rp_load(p.q_pos, b * p.q_pos_b + r0 + i, p.q_pos64);
-        sq[rows_per_part + i] = p.q_seg != nullptr ? rp_load(p.q_seg, b * p.q_seg_b + r0 + i, p.q_seg64) : 0;
+    // row r of the part is query first + r parts_per_b: near pairs, whose pieces have several buckets and cost most, then come
+    // to all threads alike as r goes on (with consecutive rows a few warps had them all: 64 us instead of 38 for 134 MB)
+    const int first = blockIdx.x - b * parts_per_b, r1 = (p.Lq - first + parts_per_b - 1) / parts_per_b;
+    const long long row_stride = p.sI * parts_per_b;
+    const T* gb = grad + b * p.sB + h0 * p.sH + first * p.sI;
+    for (int r = tid; r < r1; r += nt) {
+        const int i = first + r * parts_per_b;
+        sq[r] = rp_load(p.q_pos, b * p.q_pos_b + i, p.q_pos64);
+        sq[rows_per_part + r] = p.q_seg != nullptr ? rp_load(p.q_seg, b * p.q_seg_b + i, p.q_seg64) : 0;
     }
     __syncthreads();
     int run = 0;
-    float sum = 0.f;
-    auto put = [&](int u, float v) {
-        if (u != run) {
-            acc[run * nt + tid] += sum;
-            run = u;
-            sum = 0.f;
+    float sum[kH];
+#pragma unroll
+    for (int h = 0; h < kH; ++h) sum[h] = 0.f;
+    auto move_to = [&](int u) {
+        if (u == run) return;
+#pragma unroll
+        for (int h = 0; h < kH; ++h) {
+            acc[(run * kH + h) * nt + tid] += sum[h];
+            sum[h] = 0.f;
         }
-        sum += v;
+        run = u;
     };
     if (ty < side) {
         for (int c = tx; c < nch; c += tpr) {
@@ -331,57 +338,87 @@ __global__ void __launch_bounds__(kRpThreads) relpos_heads_grad_kernel(const __g
                 one_seg = one_seg && ks[e] == ks[0];
             }
             const T* src = gb + j0;
-            for (int r = r0 + ty; r < r1; r += kU * side) {
-                uint4 raw[kU];
-                if (kVec && nj == kN) {
+            // kU rows of this thread's piece; the next kU are in flight while these are added up
+            auto load = [&](uint4 (&raw)[kU][kH], int r) {
 #pragma unroll
-                    for (int s = 0; s < kU; ++s)
-                        raw[s] = r + s * side < r1 ? __ldcs(reinterpret_cast<const uint4*>(src + (r + s * side) * p.sI))
-                                                   : make_uint4(0u, 0u, 0u, 0u);
-                } else {
+                for (int s = 0; s < kU; ++s)
 #pragma unroll
-                    for (int s = 0; s < kU; ++s) {
-                        const T* row = src + (r + s * side) * p.sI;
-                        float g[kN];
+                    for (int h = 0; h < kH; ++h) {
+                        const bool in = r + s * side < r1 && h0 + h < p.C;
+                        const T* row = src + (r + s * side) * row_stride + h * p.sH;
+                        raw[s][h] = make_uint4(0u, 0u, 0u, 0u);
+                        if (kVec && nj == kN) {
+                            if (in) raw[s][h] = __ldcs(reinterpret_cast<const uint4*>(row));
+                        } else if (in) {
+                            float g[kN];
 #pragma unroll
-                        for (int e = 0; e < kN; ++e) g[e] = r + s * side < r1 && e < nj ? rp_float(row[e]) : 0.f;
-                        raw[s] = RpVec<T>::pack(g);
+                            for (int e = 0; e < kN; ++e) g[e] = e < nj ? rp_float(row[e]) : 0.f;
+                            raw[s][h] = RpVec<T>::pack(g);
+                        }
                     }
-                }
+            };
+            auto add = [&](const uint4 (&raw)[kU][kH], int r) {
 #pragma unroll
                 for (int s = 0; s < kU; ++s) {
                     const int rr = r + s * side;
                     if (rr >= r1) break;
-                    float g[kN];
-                    RpVec<T>::unpack(raw[s], g);
-                    const int q = sq[rr - r0], qs = sq[rows_per_part + rr - r0];
+                    const int q = sq[rr], qs = sq[rows_per_part + rr];
                     const bool apart = one_seg && ks[0] != qs;
                     const int ulo = rp_bucket(lut, p.M, q - kmax), uhi = rp_bucket(lut, p.M, q - kmin);
-                    if (apart || (one_seg && ulo == uhi)) {
-                        float t = g[0];
+                    float g[kH][kN];
 #pragma unroll
-                        for (int e = 1; e < kN; ++e) t += g[e];
-                        put(apart ? p.rows - 1 : ulo, t);
+                    for (int h = 0; h < kH; ++h) RpVec<T>::unpack(raw[s][h], g[h]);
+                    if (apart || (one_seg && ulo == uhi)) {
+                        move_to(apart ? p.rows - 1 : ulo);
+#pragma unroll
+                        for (int h = 0; h < kH; ++h) {
+#pragma unroll
+                            for (int w = kN / 2; w >= 1; w >>= 1)
+#pragma unroll
+                                for (int e = 0; e < w; ++e) g[h][e] += g[h][e + w];
+                            sum[h] += g[h][0];
+                        }
                     } else {
+                        int u[kN];
 #pragma unroll
                         for (int e = 0; e < kN; ++e) {
-                            if (e < nj) put(ks[e] != qs ? p.rows - 1 : rp_bucket(lut, p.M, q - kp[e]), g[e]);
+                            u[e] = rp_bucket(lut, p.M, q - kp[e]);
+                            if (ks[e] != qs) u[e] = p.rows - 1;
+                        }
+#pragma unroll
+                        for (int e = 0; e < kN; ++e) {
+                            if (e < nj) {
+                                move_to(u[e]);
+#pragma unroll
+                                for (int h = 0; h < kH; ++h) sum[h] += g[h][e];
+                            }
                         }
                     }
                 }
+            };
+            uint4 x[kU][kH], y[kU][kH];
+            const int step = kU * side;
+            load(x, ty);
+            for (int r = ty; r < r1; r += 2 * step) {
+                load(y, r + step);
+                add(x, r);
+                load(x, r + 2 * step);
+                add(y, r + step);
             }
         }
     }
-    acc[run * nt + tid] += sum;
+#pragma unroll
+    for (int h = 0; h < kH; ++h) acc[(run * kH + h) * nt + tid] += sum[h];
     __syncthreads();
-    // a warp per bucket: lanes over the threads' columns
+    // a warp per sum: lanes over the threads' columns
     const int warp = tid >> 5, lane = tid & 31, warps = nt >> 5;
-    for (int u = warp; u < p.rows; u += warps) {
+    for (int x = warp; x < p.rows * kH; x += warps) {
         float t = 0.f;
-        for (int e = lane; e < nt; e += 32) t += acc[u * nt + e];
+        for (int e = lane; e < nt; e += 32) t += acc[x * nt + e];
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-        if (lane == 0) partial[((long long)blockIdx.x * p.rows + u) * p.C + h] = t;
+        const int u = x / kH, h = h0 + x % kH;
+        if (lane == 0 && h < p.C) partial[((long long)blockIdx.x * p.rows + u) * p.C + h] = t;
     }
 }
 
