@@ -12,9 +12,10 @@
 //   warps 4-7, 8-11   softmax of one query tile each: a thread owns a row
 // The running maximum a row is scaled by lags behind the true one by up to 2^8: O is rescaled only when a row's maximum
 // has grown by more (accumulators and sums are fp32, where a common factor of 2^8 costs nothing).
-// Tensor memory: S of both tiles [0, 256), O of both from 256.  P overlays the first half of its own S where the 512
-// columns are full (kD = 128), and has columns of its own else.  tcgen05.mma of one thread run in the order of issue, so
-// the S of the next key tile, issued after the product that reads P, cannot overtake it.
+// Tensor memory: S of both tiles [0, 256), O of both from 256.  kD = 64: P has columns of its own, and the next scores are
+// issued as soon as the present ones are in registers.  kD = 128: the 512 columns are full, P overlays the first half of its
+// own S, and the next scores follow the product that reads P (tcgen05.mma of one thread run in the order of issue, so they
+// cannot overtake it).  P is handed over in halves of 64 keys, so that its product starts while the rest is exponentiated.
 // Head dimensions below kD are filled with zeros by the TMA loads.
 #pragma once
 
@@ -39,6 +40,7 @@ struct AfLayout {
     static constexpr int kOffRing = kOffBias + 2 * kBiasBufs * 2 * kAfSub;
     static constexpr int kOffBars = kOffRing + kStages * kTile;
     static constexpr int kSmem = kOffBars + 512;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
 struct AttnFwdParams {
@@ -120,8 +122,9 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBars);
     uint64_t* q_full = bars;                   // [2]
     uint64_t* s_full = q_full + 2;             // [2] scores of a key tile complete
-    uint64_t* p_full = s_full + 2;             // [2] probabilities in tensor memory, O rescaled where it had to be
-    uint64_t* o_full = p_full + 2;             // [2] last product complete
+    uint64_t* s_read = s_full + 2;             // [2] scores are in registers (kD = 64)
+    uint64_t* p_full = s_read + 2;             // [2][2] half of the probabilities in tensor memory, O rescaled where it had to be
+    uint64_t* o_full = p_full + 4;             // [2] product complete (kD = 128: the last one)
     uint64_t* b_full = o_full + 2;             // [2][kBb]
     uint64_t* b_empty = b_full + 2 * kBb;      // [2][kBb]
     uint64_t* full = b_empty + 2 * kBb;        // [kSt]
@@ -139,7 +142,9 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         for (int w = 0; w < 2; ++w) {
             mbar_init(&q_full[w], 1);
             mbar_init(&s_full[w], 1);
-            mbar_init(&p_full[w], 4);
+            mbar_init(&s_read[w], 4);
+            mbar_init(&p_full[2 * w], 4);
+            mbar_init(&p_full[2 * w + 1], 4);
             mbar_init(&o_full[w], 1);
         }
         for (int s = 0; s < 2 * kBb; ++s) {
@@ -222,23 +227,33 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
                     if (wait(&q_full[w], 0, 310 + w)) scores(w, 0);
                 umma_commit(&empty[0]);
             }
+            auto mix = [&](int w, int j, int half) {     // O_w += P_w V_j over 64 keys
+                const uint32_t v = smem_u32(ring + ((2 * j + 1) % kSt) * L::kTile);
+                const uint32_t pt = tmem + (kD == 128 ? w * 128 : 384 + w * 64);
+#pragma unroll
+                for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                    umma_bf16_ts(tmem + 256 + w * kD, pt + kk * 8, umma_smem_desc_mn_sw128(v + kk * 2048, kAfSub, 1024), idesc_o,
+                                 (j | kk) != 0);
+            };
             for (int j = 0; ok && j < n; ++j) {
                 const int sv = (2 * j + 1) % kSt, sk = (2 * j + 2) % kSt;
-                const uint32_t phv = ((2 * j + 1) / kSt) & 1, phk = ((2 * j + 2) / kSt) & 1;
+                const bool more = j + 1 < n;
+                if (kD == 64 && more && wait(&full[sk], ((2 * j + 2) / kSt) & 1, 340)) {
+                    // scores have columns of their own: the next ones follow as soon as these are in registers
+                    for (int w = 0; ok && w < tiles; ++w)
+                        if (wait(&s_read[w], j & 1, 350 + w)) scores(w, j + 1);
+                    umma_commit(&empty[sk]);
+                }
                 if (fp.words != nullptr) wait(&v_ok[j % kAfClean], (j / kAfClean) & 1, 320);
-                else wait(&full[sv], phv, 321);
+                else wait(&full[sv], ((2 * j + 1) / kSt) & 1, 321);
                 for (int w = 0; ok && w < tiles; ++w) {
-                    if (!wait(&p_full[w], j & 1, 330 + w)) break;
-                    const uint32_t v = smem_u32(ring + sv * L::kTile);
-                    const uint32_t pt = tmem + (kD == 128 ? w * 128 : 384 + w * 64);
-#pragma unroll
-                    for (int kk = 0; kk < 8; ++kk)
-                        umma_bf16_ts(tmem + 256 + w * kD, pt + kk * 8, umma_smem_desc_mn_sw128(v + kk * 2048, kAfSub, 1024), idesc_o,
-                                     (j | kk) != 0);
-                    if (j == n - 1) umma_commit(&o_full[w]);
+                    for (int half = 0; half < 2; ++half)
+                        if (wait(&p_full[2 * w + half], j & 1, 330 + w)) mix(w, j, half);
+                    if (!ok) break;
+                    if (kD == 64 || !more) umma_commit(&o_full[w]);
                     if (w == tiles - 1) umma_commit(&empty[sv]);
-                    if (j + 1 < n) {
-                        if (w == 0 && !wait(&full[sk], phk, 340)) break;
+                    if (kD == 128 && more) {
+                        if (w == 0 && !wait(&full[sk], ((2 * j + 2) / kSt) & 1, 340)) break;
                         scores(w, j + 1);
                         if (w == tiles - 1) umma_commit(&empty[sk]);
                     }
@@ -314,6 +329,11 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 #pragma unroll
                 for (int k = 0; k < 4; ++k) tmem_ld_32x32(tS + 32 * k, s[k]);
                 tmem_ld_wait();
+                if (kD == 64) {
+                    tcgen05_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_read[w]);
+                }
                 if constexpr (kBias) {
                     const int bs = w * kBb + j % kBb;
                     if (!(ok = warp_wait(&b_full[bs], (j / kBb) & 1, lane, abort_flag, p.status, kStageIdAttnFwd, 410 + w))) break;
@@ -352,15 +372,20 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
                 }
                 float mx[4] = {m, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
+                for (int e = 0; e < 32; e += 2)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(s[k][e]));
-                const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(s[k][e]), __uint_as_float(s[k][e + 1]));
+                const float mn = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
                 const bool grow = mn > m + slack;
+                // from here on O and P change: the product of the tile before must be complete.  With kD = 128 these scores
+                // were issued after it
+                if (kD == 64 && j > 0) {
+                    if (!(ok = warp_wait(&o_full[w], (j - 1) & 1, lane, abort_flag, p.status, kStageIdAttnFwd, 430 + w))) break;
+                    tcgen05_fence_after();
+                }
                 if (j == 0) {
                     m = mn;
                 } else if (__any_sync(0xffffffffu, grow)) {
-                    // the product of the tile before is complete: these scores were issued after it
                     const float f = grow ? ex2f((m - mn) * mul) : 1.f;
                     if (grow) m = mn;
                     l *= f;
@@ -391,14 +416,16 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
                         pk[e] = pack_bf16x2(a, d);
                     }
                     tmem_st_32x16(tP + 16 * k, pk);
+                    if (k & 1) {             // half of the keys: the product with their values can start
+                        tmem_st_wait();
+                        tcgen05_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_full[2 * w + (k >> 1)]);
+                    }
                 }
                 l += f2_hsum(f2_add(sum[0], sum[1]));
-                tmem_st_wait();
-                tcgen05_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[w]);
             }
-            if (n > 0 && ok) ok = warp_wait(&o_full[w], 0, lane, abort_flag, p.status, kStageIdAttnFwd, 420 + w);
+            if (n > 0 && ok) ok = warp_wait(&o_full[w], kD == 64 ? (n - 1) & 1 : 0, lane, abort_flag, p.status, kStageIdAttnFwd, 420 + w);
             tcgen05_fence_after();
             if (ok) {
                 const bool nothing = m == -INFINITY || n == 0;
