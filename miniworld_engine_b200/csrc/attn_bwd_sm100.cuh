@@ -59,23 +59,25 @@ struct AbQLayout {               // query-tile kernel: Q, dout, rings of key and
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-// D += A[smem, K-major] B[smem, K-major]^T over kD, both tiles as kD / 64 swizzled sub-tiles of 64 columns
+// D = A[smem, K-major] B[smem, K-major]^T over kD, both tiles as kD / 64 swizzled sub-tiles of 64 columns
 template <int kD>
 __device__ __forceinline__ void ab_scores(uint32_t d, uint32_t a, uint32_t b) {
     constexpr uint32_t idesc = umma_idesc_bf16(128, 128);
+    const uint64_t da = umma_smem_desc_sw128(a), db = umma_smem_desc_sw128(b);
 #pragma unroll
     for (int kk = 0; kk < kD / 16; ++kk) {
-        const uint32_t off = (kk >> 2) * kAfSub + (kk & 3) * 32;
-        umma_bf16_ss(d, umma_smem_desc_sw128(a + off), umma_smem_desc_sw128(b + off), idesc, kk > 0);
+        const uint64_t off = ((kk >> 2) * kAfSub + (kk & 3) * 32) >> 4;
+        umma_ss_warp(d, da + off, db + off, idesc, kk > 0);
     }
 }
 // D += A[tensor memory, 128 columns of 16 bits: 64 in columns [0, 32), 64 in [64, 96)] B[smem, 128 rows of kD]
 template <int kD>
 __device__ __forceinline__ void ab_mix(uint32_t d, uint32_t a, uint32_t b, bool add) {
     constexpr uint32_t idesc = umma_idesc_bf16(128, kD, 0, 1);
+    const uint64_t db = umma_smem_desc_mn_sw128(b, kAfSub, 1024);
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk)
-        umma_bf16_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, umma_smem_desc_mn_sw128(b + kk * 2048, kAfSub, 1024), idesc, add || kk > 0);
+        umma_ts_warp(d, a + (kk >> 2) * 64 + (kk & 3) * 8, db + ((kk * 2048) >> 4), idesc, add || kk > 0);
 }
 // 64 fp32 values as bf16 into columns [0, 32) of a tile half
 __device__ __forceinline__ void ab_put(uint32_t t, const float (&f)[64]) {
@@ -221,10 +223,10 @@ attn_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
             bool ok = true;
             auto wait = [&](uint64_t* bar, uint32_t ph, int detail) {
-                ok = ok && mbar_wait<true>(bar, ph, abort_flag, p.status, kStageIdAttnDkv, detail);
+                ok = ok && warp_wait(bar, ph, lane, abort_flag, p.status, kStageIdAttnDkv, detail);
                 tcgen05_fence_after();
                 return ok;
             };
@@ -232,10 +234,10 @@ attn_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             auto q_at = [&](int it) { return r0 + (it % kSt) * 2 * L::kTile; };
             if (wait(&kv_full[0], 0, 300) && wait(&full[0], 0, 301)) {
                 ab_scores<kD>(tS, k, q_at(0));
-                umma_commit(s_full);
+                umma_commit_warp(s_full);
                 if (wait(&kv_full[1], 0, 302)) {
                     ab_scores<kD>(tP, v, q_at(0) + L::kTile);
-                    umma_commit(dp_full);
+                    umma_commit_warp(dp_full);
                 }
             }
             for (int it = 0; ok && it < n; ++it) {
@@ -245,20 +247,19 @@ attn_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
                 if (more) {
                     if (!wait(&full[(it + 1) % kSt], ((it + 1) / kSt) & 1, 320)) break;
                     ab_scores<kD>(tS, k, q_at(it + 1));
-                    umma_commit(s_full);
+                    umma_commit_warp(s_full);
                 }
                 if (!wait(ds_full, it & 1, 330)) break;
                 ab_mix<kD>(tK, tP, q_at(it), it > 0);
-                umma_commit(&empty[it % kSt]);
+                umma_commit_warp(&empty[it % kSt]);
                 if (more) {
                     ab_scores<kD>(tP, v, q_at(it + 1) + L::kTile);
-                    umma_commit(dp_full);
+                    umma_commit_warp(dp_full);
                 } else {
-                    umma_commit(done);
+                    umma_commit_warp(done);
                 }
             }
         }
-        __syncwarp();
     } else if (warp == 2) {
         // row statistics of a query tile.  Without a bias the maximum and the sum are one number; rows behind the last
         // one get probability zero
@@ -483,10 +484,10 @@ attn_dq_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
             bool ok = true;
             auto wait = [&](uint64_t* bar, uint32_t ph, int detail) {
-                ok = ok && mbar_wait<true>(bar, ph, abort_flag, p.status, kStageIdAttnDq, detail);
+                ok = ok && warp_wait(bar, ph, lane, abort_flag, p.status, kStageIdAttnDq, detail);
                 tcgen05_fence_after();
                 return ok;
             };
@@ -495,13 +496,13 @@ attn_dq_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             auto scores = [&](int it) {
                 if (!wait(&k_ready[it % kKSt], (it / kKSt) & 1, 300)) return;
                 ab_scores<kD>(tS, q, k0 + (it % kKSt) * L::kTile);
-                umma_commit(s_full);
+                umma_commit_warp(s_full);
             };
             auto products = [&](int it) {                // dp = dout v^T
                 if (!wait(&v_full[it % kVSt], (it / kVSt) & 1, 310)) return;
                 ab_scores<kD>(tP, gq, v0 + (it % kVSt) * L::kTile);
-                umma_commit(dp_full);
-                umma_commit(&v_empty[it % kVSt]);
+                umma_commit_warp(dp_full);
+                umma_commit_warp(&v_empty[it % kVSt]);
             };
             if (wait(&q_full[0], 0, 320)) scores(0);
             if (wait(&q_full[1], 0, 321)) products(0);
@@ -509,12 +510,11 @@ attn_dq_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 if (it + 1 < n && wait(s_read, it & 1, 330)) scores(it + 1);
                 if (!wait(ds_full, it & 1, 340)) break;
                 ab_mix<kD>(tQ, tP, k0 + (it % kKSt) * L::kTile, it > 0);
-                umma_commit(&k_empty[it % kKSt]);
+                umma_commit_warp(&k_empty[it % kKSt]);
                 if (it + 1 < n) products(it + 1);
-                else umma_commit(done);
+                else umma_commit_warp(done);
             }
         }
-        __syncwarp();
     } else if (warp == 2) {
         if (bp.words != nullptr) {
             for (int it = 0; it < n; ++it) {
@@ -571,8 +571,9 @@ attn_dq_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         };
         for (int it = 0; it < n; ++it) {
             const int t = tile_at(it);
-            const uint4 w4 = bp.words != nullptr ? __ldg(reinterpret_cast<const uint4*>(bp.words) + (long long)b * bp.n_tiles + t)
-                                                 : tail_words(p.Lk - t * kAfRows);
+            uint4 w4 = make_uint4(~0u, ~0u, ~0u, ~0u);
+            if (bp.words != nullptr) w4 = __ldg(reinterpret_cast<const uint4*>(bp.words) + (long long)b * bp.n_tiles + t);
+            else if ((t + 1) * kAfRows > p.Lk) w4 = tail_words(p.Lk - t * kAfRows);
             const uint32_t w[2] = {g == 0 ? w4.x : w4.z, g == 0 ? w4.y : w4.w};
             if (!(ok = warp_wait(s_full, it & 1, lane, abort_flag, p.status, kStageIdAttnDq, 400))) break;
             tcgen05_fence_after();

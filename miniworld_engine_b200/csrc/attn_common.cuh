@@ -51,4 +51,52 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
+// ---------------------------------------------------------------------------------------
+// UMMAs issued by a whole warp.  Every lane runs the same code and one elected lane (the same each time) issues: descriptors
+// and addresses are then warp-uniform values, which the instruction takes from uniform registers as it wants them.  Under an
+// `if (lane == 0)` each operand is moved there first: 75 to 90 cycles per UMMA were measured in the attention kernels, whose
+// tensor cores then waited for the issuing thread.
+// ---------------------------------------------------------------------------------------
+__device__ __forceinline__ void umma_ss_warp(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "}\n"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+}
+__device__ __forceinline__ void umma_ts_warp(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "}\n"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit_warp(uint64_t* bar) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
+        "}\n"
+        ::"r"(smem_u32(bar))
+        : "memory");
+}
+
+// Wait of a whole warp: all lanes look once, which is all there is to it where the phase is complete; else one lane polls.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int lane, volatile int* abort_flag, int32_t* status,
+                                          int stage, int detail) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity) != 0)) return true;
+    uint32_t ok = 1;
+    if (lane == 0) ok = mbar_wait<true>(bar, parity, abort_flag, status, stage, detail);
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
 }  // namespace trimul

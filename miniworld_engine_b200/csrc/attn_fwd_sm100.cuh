@@ -96,13 +96,6 @@ __device__ __forceinline__ uint4 tail_words(int left) {      // bits of the firs
     auto w = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; };
     return make_uint4(w(left), w(left - 32), w(left - 64), w(left - 96));
 }
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int lane, volatile int* abort_flag, int32_t* status,
-                                          int stage, int detail) {
-    uint32_t ok = 1;
-    if (lane == 0) ok = mbar_wait<true>(bar, parity, abort_flag, status, stage, detail);
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
-}
-
 template <int kD, bool kBias>
 __global__ void __launch_bounds__(kAfThreads, 1)
 attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -123,7 +116,7 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     uint64_t* q_full = bars;                   // [2]
     uint64_t* s_full = q_full + 2;             // [2] scores of a key tile complete
     uint64_t* s_read = s_full + 2;             // [2] scores are in registers (kD = 64)
-    uint64_t* p_full = s_read + 2;             // [2][2] half of the probabilities in tensor memory, O rescaled where it had to be
+    uint64_t* p_full = s_read + 2;             // [2][2] probabilities in tensor memory, O rescaled where it had to be; kD = 128: by halves
     uint64_t* o_full = p_full + 4;             // [2] product complete (kD = 128: the last one)
     uint64_t* b_full = o_full + 2;             // [2][kBb]
     uint64_t* b_empty = b_full + 2 * kBb;      // [2][kBb]
@@ -203,64 +196,76 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
             constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128);
             constexpr uint32_t idesc_o = umma_idesc_bf16(128, kD, 0, 1);
             const int tiles = two ? 2 : 1;
             bool ok = true;
             auto wait = [&](uint64_t* bar, uint32_t ph, int detail) {
-                ok = ok && mbar_wait<true>(bar, ph, abort_flag, p.status, kStageIdAttnFwd, detail);
+                ok = ok && warp_wait(bar, ph, lane, abort_flag, p.status, kStageIdAttnFwd, detail);
                 tcgen05_fence_after();
                 return ok;
             };
-            auto scores = [&](int w, int j) {            // S_w = Q_w K_j^T
-                const uint32_t a = smem_u32(sQ + w * L::kTile), k = smem_u32(ring + ((2 * j) % kSt) * L::kTile);
+            const uint64_t dq = umma_smem_desc_sw128(smem_u32(sQ)), dk = umma_smem_desc_sw128(smem_u32(ring));
+            const uint64_t dv = umma_smem_desc_mn_sw128(smem_u32(ring), kAfSub, 1024);
+            auto scores = [&](int w, int slot) {         // S_w = Q_w K^T, K in ring slot `slot`
+                const uint64_t a = dq + (uint64_t)(w * (L::kTile >> 4)), k = dk + (uint64_t)(slot * (L::kTile >> 4));
 #pragma unroll
                 for (int kk = 0; kk < kD / 16; ++kk) {
-                    const uint32_t off = (kk >> 2) * kAfSub + (kk & 3) * 32;
-                    umma_bf16_ss(tmem + w * 128, umma_smem_desc_sw128(a + off), umma_smem_desc_sw128(k + off), idesc_s, kk > 0);
+                    const uint64_t off = ((kk >> 2) * kAfSub + (kk & 3) * 32) >> 4;
+                    umma_ss_warp(tmem + w * 128, a + off, k + off, idesc_s, kk > 0);
                 }
-                umma_commit(&s_full[w]);
+                umma_commit_warp(&s_full[w]);
+            };
+            auto mix = [&](int w, int slot, int half, bool add) {     // O_w += P_w V over 64 keys
+                const uint64_t v = dv + (uint64_t)(slot * (L::kTile >> 4));
+                const uint32_t pt = tmem + (kD == 128 ? w * 128 : 384 + w * 64);
+#pragma unroll
+                for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                    umma_ts_warp(tmem + 256 + w * kD, pt + kk * 8, v + ((kk * 2048) >> 4), idesc_o, add || kk > 0);
+            };
+            // ring position of the key tile that is next, and of the value tile
+            int sk = 0, sv = 1 % kSt;
+            uint32_t phk = 0, phv = 0;
+            auto step = [&](int& slot, uint32_t& ph) {
+                slot += 2;
+                if (slot >= kSt) { slot -= kSt; ph ^= 1u; }
             };
             if (wait(&full[0], 0, 300)) {
                 for (int w = 0; ok && w < tiles; ++w)
                     if (wait(&q_full[w], 0, 310 + w)) scores(w, 0);
-                umma_commit(&empty[0]);
+                umma_commit_warp(&empty[0]);
             }
-            auto mix = [&](int w, int j, int half) {     // O_w += P_w V_j over 64 keys
-                const uint32_t v = smem_u32(ring + ((2 * j + 1) % kSt) * L::kTile);
-                const uint32_t pt = tmem + (kD == 128 ? w * 128 : 384 + w * 64);
-#pragma unroll
-                for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                    umma_bf16_ts(tmem + 256 + w * kD, pt + kk * 8, umma_smem_desc_mn_sw128(v + kk * 2048, kAfSub, 1024), idesc_o,
-                                 (j | kk) != 0);
-            };
+            step(sk, phk);
             for (int j = 0; ok && j < n; ++j) {
-                const int sv = (2 * j + 1) % kSt, sk = (2 * j + 2) % kSt;
                 const bool more = j + 1 < n;
-                if (kD == 64 && more && wait(&full[sk], ((2 * j + 2) / kSt) & 1, 340)) {
+                if (kD == 64 && more && wait(&full[sk], phk, 340)) {
                     // scores have columns of their own: the next ones follow as soon as these are in registers
                     for (int w = 0; ok && w < tiles; ++w)
-                        if (wait(&s_read[w], j & 1, 350 + w)) scores(w, j + 1);
-                    umma_commit(&empty[sk]);
+                        if (wait(&s_read[w], j & 1, 350 + w)) scores(w, sk);
+                    umma_commit_warp(&empty[sk]);
                 }
                 if (fp.words != nullptr) wait(&v_ok[j % kAfClean], (j / kAfClean) & 1, 320);
-                else wait(&full[sv], ((2 * j + 1) / kSt) & 1, 321);
+                else wait(&full[sv], phv, 321);
                 for (int w = 0; ok && w < tiles; ++w) {
-                    for (int half = 0; half < 2; ++half)
-                        if (wait(&p_full[2 * w + half], j & 1, 330 + w)) mix(w, j, half);
+                    for (int half = 0; half < (kD == 64 ? 1 : 2); ++half)
+                        if (wait(&p_full[2 * w + half], j & 1, 330 + w)) {
+                            mix(w, sv, half, j > 0);
+                            if (kD == 64) mix(w, sv, 1, true);
+                        }
                     if (!ok) break;
-                    if (kD == 64 || !more) umma_commit(&o_full[w]);
-                    if (w == tiles - 1) umma_commit(&empty[sv]);
+                    if (kD == 64 || !more) umma_commit_warp(&o_full[w]);
+                    if (w == tiles - 1) umma_commit_warp(&empty[sv]);
                     if (kD == 128 && more) {
-                        if (w == 0 && !wait(&full[sk], ((2 * j + 2) / kSt) & 1, 340)) break;
-                        scores(w, j + 1);
-                        if (w == tiles - 1) umma_commit(&empty[sk]);
+                        if (w == 0 && !wait(&full[sk], phk, 340)) break;
+                        scores(w, sk);
+                        if (w == tiles - 1) umma_commit_warp(&empty[sk]);
                     }
                 }
+                step(sk, phk);
+                step(sv, phv);
             }
         }
-        __syncwarp();
     } else if (warp == 2) {
         if (fp.words != nullptr) {
             for (int j = 0; j < n; ++j) {
@@ -321,8 +326,9 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             bool ok = true;
             for (int j = 0; j < n; ++j) {
                 const int t = tile_at(j);
-                const uint4 w4 = fp.words != nullptr ? __ldg(reinterpret_cast<const uint4*>(fp.words) + (long long)b * fp.n_tiles + t)
-                                                     : tail_words(p.Lk - t * kAfRows);
+                uint4 w4 = make_uint4(~0u, ~0u, ~0u, ~0u);
+                if (fp.words != nullptr) w4 = __ldg(reinterpret_cast<const uint4*>(fp.words) + (long long)b * fp.n_tiles + t);
+                else if ((t + 1) * kAfRows > p.Lk) w4 = tail_words(p.Lk - t * kAfRows);
                 if (!(ok = warp_wait(&s_full[w], j & 1, lane, abort_flag, p.status, kStageIdAttnFwd, 400 + w))) break;
                 tcgen05_fence_after();
                 uint32_t s[4][32];
@@ -377,34 +383,14 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
                     for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(s[k][e]), __uint_as_float(s[k][e + 1]));
                 const float mn = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
                 const bool grow = mn > m + slack;
-                // from here on O and P change: the product of the tile before must be complete.  With kD = 128 these scores
-                // were issued after it
-                if (kD == 64 && j > 0) {
-                    if (!(ok = warp_wait(&o_full[w], (j - 1) & 1, lane, abort_flag, p.status, kStageIdAttnFwd, 430 + w))) break;
-                    tcgen05_fence_after();
-                }
-                if (j == 0) {
-                    m = mn;
-                } else if (__any_sync(0xffffffffu, grow)) {
-                    const float f = grow ? ex2f((m - mn) * mul) : 1.f;
-                    if (grow) m = mn;
-                    l *= f;
-#pragma unroll 1
-                    for (int cc = 0; cc < kD; cc += 16) {
-                        uint32_t o[16];
-                        tmem_ld_32x16(tO + cc, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st_32x16(tO + cc, o);
-                    }
-                }
+                const float f = j > 0 && grow ? ex2f((m - mn) * mul) : 1.f;
+                if (j == 0 || grow) m = mn;
+                const bool rescale = j > 0 && __any_sync(0xffffffffu, grow);
+                l *= f;
                 const float base = m == -INFINITY ? 0.f : m;
                 f32x2 sum[2] = {0ull, 0ull};
                 const f32x2 mul2 = f2_pack(mul, mul), off2 = f2_pack(-base * mul, -base * mul), nb2 = f2_pack(-base, -base);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    uint32_t pk[16];
+                auto exponentiate = [&](int k, uint32_t (&pk)[16]) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const f32x2 x = f2_pack(__uint_as_float(s[k][2 * e]), __uint_as_float(s[k][2 * e + 1]));
@@ -415,12 +401,46 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
                         sum[e & 1] = f2_add(sum[e & 1], f2_pack(a, d));
                         pk[e] = pack_bf16x2(a, d);
                     }
-                    tmem_st_32x16(tP + 16 * k, pk);
-                    if (k & 1) {             // half of the keys: the product with their values can start
-                        tmem_st_wait();
-                        tcgen05_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&p_full[2 * w + (k >> 1)]);
+                };
+                auto rescale_o = [&] {
+#pragma unroll 1
+                    for (int cc = 0; cc < kD; cc += 16) {
+                        uint32_t o[16];
+                        tmem_ld_32x16(tO + cc, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st_32x16(tO + cc, o);
+                    }
+                };
+                auto hand_over = [&](int half) {
+                    tmem_st_wait();
+                    tcgen05_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * w + half]);
+                };
+                if constexpr (kD == 64) {
+                    // the product of the tile before may still run: all exponentials first, then O and P change
+                    uint32_t pk[4][16];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) exponentiate(k, pk[k]);
+                    if (j > 0) {
+                        if (!(ok = warp_wait(&o_full[w], (j - 1) & 1, lane, abort_flag, p.status, kStageIdAttnFwd, 430 + w))) break;
+                        tcgen05_fence_after();
+                        if (rescale) rescale_o();
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tmem_st_32x16(tP + 16 * k, pk[k]);
+                    hand_over(0);
+                } else {
+                    // these scores were issued after the product of the tile before
+                    if (rescale) rescale_o();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t pk[16];
+                        exponentiate(k, pk);
+                        tmem_st_32x16(tP + 16 * k, pk);
+                        if (k & 1) hand_over(k >> 1);     // half of the keys: the product with their values can start
                     }
                 }
                 l += f2_hsum(f2_add(sum[0], sum[1]));
