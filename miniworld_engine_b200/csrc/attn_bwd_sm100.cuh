@@ -43,6 +43,7 @@ struct AbKvLayout {              // key-tile kernel: K, V, a ring of (Q, dout) p
     static constexpr int kStats = kBias && kD == 128 ? 1 : 2;    // buffers of 3 x 128 floats
     static constexpr int kOffBars = kOffStat + kStats * 3 * 128 * 4;
     static constexpr int kSmem = kOffBars + 256;
+    static_assert((15 + 2 * kStages) * 8 + 8 <= 256, "barriers");
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 template <int kD, bool kBias>
@@ -56,6 +57,7 @@ struct AbQLayout {               // query-tile kernel: Q, dout, rings of key and
     static constexpr int kOffBias = kOffV + kVSt * kTile;
     static constexpr int kOffBars = kOffBias + kBiasBufs * 2 * kAfSub;
     static constexpr int kSmem = kOffBars + 256;
+    static_assert((11 + 3 * kKSt + 2 * kVSt) * 8 + 8 <= 256, "barriers");
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -155,7 +157,7 @@ attn_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty + kSt);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int tile = blockIdx.x, j0 = tile * kAfRows, hk = blockIdx.y, b = blockIdx.z;
     const int group = p.H / p.Hk, nq = (p.Lq + kAfRows - 1) / kAfRows;
 
@@ -191,14 +193,14 @@ attn_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = warp_uniform(*tmem_slot);
     const uint32_t tS = tmem, tP = tmem + 128, tV = tmem + 256, tK = tmem + 256 + kD;
     griddep_wait();
     griddep_launch_dependents();
 
     const uint4 w4 = bp.words != nullptr ? __ldg(reinterpret_cast<const uint4*>(bp.words) + (long long)b * bp.n_tiles + tile)
                                          : make_uint4(~0u, ~0u, ~0u, ~0u);
-    const int n = (w4.x | w4.y | w4.z | w4.w) != 0u ? group * nq : 0;       // query tiles, head after head
+    const int n = warp_uniform((w4.x | w4.y | w4.z | w4.w) != 0u ? group * nq : 0);       // query tiles, head after head
     auto head_of = [&](int it) { return hk * group + it / nq; };
     auto row_of = [&](int it) { return (it % nq) * kAfRows; };
 
@@ -418,7 +420,7 @@ attn_dq_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_empty + kVSt);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int i0 = blockIdx.x * kAfRows, h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hk);
 
     if (threadIdx.x == 0) {
@@ -456,13 +458,13 @@ attn_dq_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = warp_uniform(*tmem_slot);
     const uint32_t tS = tmem, tP = tmem + 128, tQ = tmem + 256;
     griddep_wait();
     griddep_launch_dependents();
 
     const int* list = bp.list != nullptr ? bp.list + (long long)b * (bp.n_tiles + 1) : nullptr;
-    const int n = list != nullptr ? list[0] : bp.n_tiles;
+    const int n = warp_uniform(list != nullptr ? list[0] : bp.n_tiles);
     auto tile_at = [&](int it) { return list != nullptr ? __ldg(list + 1 + it) : it; };
 
     if (warp == 0) {

@@ -57,6 +57,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // `if (lane == 0)` each operand is moved there first: 75 to 90 cycles per UMMA were measured in the attention kernels, whose
 // tensor cores then waited for the issuing thread.
 // ---------------------------------------------------------------------------------------
+__device__ __forceinline__ int warp_uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }      // known to be, from here on
+__device__ __forceinline__ uint32_t warp_uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ void umma_ss_warp(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
     asm volatile(
         "{\n\t"
@@ -90,10 +92,28 @@ __device__ __forceinline__ void umma_commit_warp(uint64_t* bar) {
         : "memory");
 }
 
-// Wait of a whole warp: all lanes look once, which is all there is to it where the phase is complete; else one lane polls.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+// Wait of a whole warp.  All lanes look once (where the phase is complete that is all there is to it), then wait suspended for
+// up to the hint's 20 us, from which the warp wakes at once (with a sleeping poller instead, a wait took up to 3000 cycles
+// longer); after that one lane polls, with the limit of every wait.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int lane, volatile int* abort_flag, int32_t* status,
                                           int stage, int detail) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity) != 0)) return true;
+    if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
+#pragma unroll 1
+    for (int t = 0; t < 256; ++t)
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity) != 0)) return true;
     uint32_t ok = 1;
     if (lane == 0) ok = mbar_wait<true>(bar, parity, abort_flag, status, stage, detail);
     return __shfl_sync(0xffffffffu, ok, 0) != 0;

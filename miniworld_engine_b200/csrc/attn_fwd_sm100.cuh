@@ -126,7 +126,7 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_ok + kAfClean);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int i0 = blockIdx.x * 2 * kAfRows, h = blockIdx.y, b = blockIdx.z / fp.splits, split = blockIdx.z % fp.splits;
     const int hk = h / (p.H / p.Hk);
     const bool two = i0 + kAfRows < p.Lq;
@@ -163,13 +163,13 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = warp_uniform(*tmem_slot);
     griddep_wait();
     griddep_launch_dependents();
 
     // the key tiles of this block
     const int* list = fp.list != nullptr ? fp.list + (long long)b * (fp.n_tiles + 1) : nullptr;
-    const int kept = list != nullptr ? list[0] : fp.n_tiles;
+    const int kept = warp_uniform(list != nullptr ? list[0] : fp.n_tiles);
     const int t_first = split * fp.tiles_per_split;
     const int n = max(0, min(fp.tiles_per_split, kept - t_first));
     auto tile_at = [&](int j) { return list != nullptr ? __ldg(list + 1 + t_first + j) : t_first + j; };
