@@ -407,6 +407,10 @@ typedef struct trimul_attn_tensor {
  * gives zeros, and zero gradients.  Masked keys and values may hold anything, NaN included.
  */
 #define TRIMUL_ATTN_FLAG_PLAIN 1u         /* the CUDA-core kernels also where tensor-core ones exist  */
+#define TRIMUL_ATTN_FLAG_COPY_BIAS 2u     /* the bias's rows do not start on 16 bytes (or an axis of it is
+                                             repeated in place): the tensor-core kernels, which fetch it in
+                                             tiles, work on a copy in the workspace.  Without the flag such a
+                                             bias takes the CUDA-core kernels                         */
 typedef struct trimul_attn_desc {
     uint32_t struct_bytes;
     int32_t  dtype;                       /* of every tensor: TRIMUL_DTYPE_*                          */

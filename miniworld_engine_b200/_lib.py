@@ -54,7 +54,7 @@ EXPORTED_SYMBOLS = (
 BUCKETS_CLIPPED, BUCKETS_LOG, BUCKETS_CAUSAL = 0, 1, 2
 MAX_THRESHOLDS, MAX_BUCKETS, MAX_LUT = 250, 1024, 8192
 RELPOS_HEADS, RELPOS_PAIR = 0, 1
-ATTN_FLAG_PLAIN = 1
+ATTN_FLAG_PLAIN, ATTN_FLAG_COPY_BIAS = 1, 2
 
 
 class Desc(C.Structure):

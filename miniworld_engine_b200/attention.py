@@ -85,7 +85,7 @@ class _Call:
         scale = D ** -0.5 if scale is None else float(scale)
         if not math.isfinite(scale):
             raise ValueError(f"scale must be finite, got {scale}")
-        self.head = (_lib.ATTN_DESC.size, code, B, Lq, Lk, H, Hk, D, scale, _lib.ATTN_FLAG_PLAIN if plain_kernels else 0)
+        flags = _lib.ATTN_FLAG_PLAIN if plain_kernels else 0
         self.bias = self.bias_shape = self.mask = None
         self.bias_args, self.mask_args = (0, 0, 0, 0, 0, 0), (0, 0)
         if bias is not None:
@@ -99,7 +99,10 @@ class _Call:
             bias = bias.detach() if bias.requires_grad else bias
             bias = bias[(None,) * (4 - len(shape))] if len(shape) < 4 else bias
             if not self.empty and Lk:
-                bias = _bias_rows(bias, tc)
+                if (bias.shape[3] > 1 and bias.stride(3) != 1) or min(bias.stride()) < 0:
+                    bias = bias.contiguous()
+                if tc and not _on_16_bytes(bias):
+                    flags |= _lib.ATTN_FLAG_COPY_BIAS
             b, h, i, _ = bias.stride()
             self.bias, self.bias_args = bias, (bias.data_ptr(), b, h, i, full[0], full[1])
         if key_mask is not None:
@@ -109,6 +112,7 @@ class _Call:
                 raise ValueError(f"key_mask is on {key_mask.device}, q on {device}")
             m = _mask_bytes(key_mask)
             self.mask, self.mask_args = m, (m.data_ptr(), m.stride(0))
+        self.head = (_lib.ATTN_DESC.size, code, B, Lq, Lk, H, Hk, D, scale, flags)
 
     def pack(self, o, stats, o_lo, dout=_NONE, dq=_NONE, dk=_NONE, dv=_NONE, dbias=_NONE) -> bytes:
         """``trimul_attn_desc``; ``o`` ... ``dv`` as ``_tensor`` gives them."""
@@ -136,18 +140,12 @@ class _Call:
         return torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
 
 
-def _bias_rows(bias, tensor_cores):
-    """The bias with contiguous rows; for the tensor-core kernels, which fetch it in tiles, with rows on 16-byte
-    boundaries (a copy where they are not, as ``relative_position_bias_b200`` never needs)."""
-    rows_ok = bias.shape[3] == 1 or bias.stride(3) == 1
-    if tensor_cores:
-        if rows_ok and bias.data_ptr() % 16 == 0 and all(
-                n == 1 or (s % 8 == 0 and s > 0) for n, s in zip(bias.shape[:3], bias.stride()[:3])):
-            return bias
-        wide = _rows_of(bias.shape, bias.dtype, bias.device)
-        wide.copy_(bias)
-        return wide
-    return bias if rows_ok and all(s >= 0 for s in bias.stride()) else bias.contiguous()
+def _on_16_bytes(bias) -> bool:
+    """Whether the tensor-core kernels can fetch this bf16 bias where it is."""
+    if bias.data_ptr() % 16:
+        return False
+    (b, h, i, _), (sb, sh, si, _) = bias.shape, bias.stride()
+    return (i == 1 or (si % 8 == 0 and si > 0)) and (h == 1 or (sh % 8 == 0 and sh > 0)) and (b == 1 or (sb % 8 == 0 and sb > 0))
 
 
 def _rows_of(shape, dtype, device):

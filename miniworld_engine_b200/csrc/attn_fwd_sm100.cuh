@@ -54,6 +54,34 @@ struct AttnFwdParams {
     int bias_b1, bias_h1;        // bias shared along the batch / the heads
 };
 
+// A bias whose rows do not start on 16 bytes, as rows that do: two neighbouring values a thread, so that a warp reads and
+// writes 128 bytes in a row.
+__global__ void __launch_bounds__(256)
+attn_bias_rows_kernel(const __nv_bfloat16* src, long long src_b, long long src_h, long long src_i, uint32_t* dst, int H, int Lq, int Lk,
+                      long long rows, int pitch) {
+    constexpr int kU = 4;
+    griddep_wait();
+    griddep_launch_dependents();
+    const int words = pitch / 2;
+    for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (long long)gridDim.x * 8) {
+        const int i = (int)(r % Lq);
+        const long long bh = r / Lq;
+        const __nv_bfloat16* s = src + bh / H * src_b + bh % H * src_h + i * src_i;
+        for (int w0 = threadIdx.x & 31; w0 < words; w0 += 32 * kU) {
+            __nv_bfloat162 v[kU];
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int j = 2 * (w0 + 32 * u);
+                v[u].x = j < Lk ? s[j] : __nv_bfloat16();
+                v[u].y = j + 1 < Lk ? s[j + 1] : __nv_bfloat16();
+            }
+#pragma unroll
+            for (int u = 0; u < kU; ++u)
+                if (w0 + 32 * u < words) dst[r * words + w0 + 32 * u] = *reinterpret_cast<const uint32_t*>(&v[u]);
+        }
+    }
+}
+
 // Key mask as bits, and the list of tiles that keep something.  One block per batch element.
 constexpr int kMaskPrepThreads = 256;
 __global__ void __launch_bounds__(kMaskPrepThreads)

@@ -21,16 +21,53 @@ template <int kT> inline int ap_smem(int D, int tiles, int scores) {
     return (tiles * kT * ap_pitch(D) + scores * kT * ap_ppitch<kT>() + 3 * kT) * 4;
 }
 
-// kT rows of a tensor into shared memory as fp32, zeros behind the last row, in masked rows and behind column D.
-template <typename T, int kT>
-__device__ __forceinline__ void ap_load(float* dst, const T* src, long long stride, int row0, int rows, int D,
-                                        const uint8_t* keep) {
-    const int pitch = ap_pitch(D), cols = pitch - 4;
-    for (int e = threadIdx.x; e < kT * cols; e += kApThreads) {
-        const int r = e / cols, d = e - r * cols;
-        const bool in = row0 + r < rows && d < D && (keep == nullptr || keep[row0 + r] != 0);
-        dst[r * pitch + d] = in ? at_float(src[(long long)(row0 + r) * stride + d]) : 0.f;
+// kT rows of a tensor on their way into shared memory as fp32, with zeros behind the last row, in masked rows and behind
+// column D.  `fetch` issues the loads (four consecutive columns a piece where rows allow it), `put` stores what came: between
+// the two a tile's loads run behind the arithmetic of the tile before.
+template <typename T> struct ApRaw;
+template <> struct ApRaw<float> { using V = float4; };
+template <> struct ApRaw<__nv_bfloat16> { using V = uint2; };
+__device__ __forceinline__ float4 ap_wide(const float4& v) { return v; }
+__device__ __forceinline__ float4 ap_wide(const uint2& v) { return make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y)); }
+
+template <typename T, int kT, int kC>
+struct ApTile {
+    static constexpr int kPieces = kT * kC * 4 / kApThreads;      // of four columns, per thread, D = 16 kC
+    float4 v[kPieces];
+    __device__ __forceinline__ void fetch(const T* src, long long stride, int row0, int rows, int D, const uint8_t* keep, bool vec) {
+        const int cols = (ap_pitch(D) - 4) >> 2, total = kT * cols;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+            const int e = threadIdx.x + k * kApThreads;
+            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (e >= total) continue;
+            const int r = e / cols, d = (e - r * cols) * 4;
+            if (row0 + r >= rows || (keep != nullptr && keep[row0 + r] == 0)) continue;
+            const T* p = src + (long long)(row0 + r) * stride + d;
+            if (vec) {
+                v[k] = ap_wide(*reinterpret_cast<const typename ApRaw<T>::V*>(p));
+            } else {
+                v[k].x = at_float(p[0]);
+                if (d + 1 < D) v[k].y = at_float(p[1]);
+                if (d + 2 < D) v[k].z = at_float(p[2]);
+                if (d + 3 < D) v[k].w = at_float(p[3]);
+            }
+        }
     }
+    __device__ __forceinline__ void put(float* dst, int D) const {
+        const int pitch = ap_pitch(D), cols = (pitch - 4) >> 2, total = kT * cols;
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+            const int e = threadIdx.x + k * kApThreads;
+            if (e >= total) continue;
+            const int r = e / cols;
+            *reinterpret_cast<float4*>(dst + r * pitch + (e - r * cols) * 4) = v[k];
+        }
+    }
+};
+// Rows of four-column pieces at the alignment their loads need
+template <typename T> __device__ __forceinline__ bool ap_vec(const AttnTensor& t, int D) {
+    return (D & 3) == 0 && ((t.b | t.l | t.h) & 3) == 0 && (reinterpret_cast<uintptr_t>(t.p) & (4 * sizeof(T) - 1)) == 0;
 }
 
 // acc[r][c] = A[ty kR + r] . B[tx + 16 c]
@@ -94,23 +131,33 @@ __device__ __forceinline__ float ap_row_sum(float v) {
     return v;
 }
 
-// Scores of a tile: scale and bias, -inf at masked keys and behind the last one.
+// Bias values and kept keys of a tile, fetched ahead of the products; then scores: scale and bias, -inf at masked keys and
+// behind the last one.
 template <typename T, int kR>
-__device__ __forceinline__ void ap_scores(float (&s)[kR][kR], const AttnParams& p, int b, int h, int i0, int j0, int ty, int tx) {
-    const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
-    const T* bias = p.bias != nullptr ? static_cast<const T*>(p.bias) + b * p.bias_b + h * p.bias_h : nullptr;
+struct ApBias {
+    float v[kR][kR];
+    bool kept[kR];
+    __device__ __forceinline__ void fetch(const AttnParams& p, int b, int h, int i0, int j0, int ty, int tx) {
+        const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
+        const T* bias = p.bias != nullptr ? static_cast<const T*>(p.bias) + b * p.bias_b + h * p.bias_h : nullptr;
 #pragma unroll
-    for (int c = 0; c < kR; ++c) {
-        const int j = j0 + tx + 16 * c;
-        const bool kept = j < p.Lk && (keep == nullptr || keep[j] != 0);
+        for (int c = 0; c < kR; ++c) {
+            const int j = j0 + tx + 16 * c;
+            kept[c] = j < p.Lk && (keep == nullptr || keep[j] != 0);
 #pragma unroll
-        for (int r = 0; r < kR; ++r) {
-            const int i = i0 + ty * kR + r;
-            s[r][c] = !kept ? -INFINITY
-                            : fmaf(s[r][c], p.scale, bias != nullptr && i < p.Lq ? at_float(bias[i * p.bias_i + j]) : 0.f);
+            for (int r = 0; r < kR; ++r) {
+                const int i = i0 + ty * kR + r;
+                v[r][c] = bias != nullptr && i < p.Lq && j < p.Lk ? at_float(bias[i * p.bias_i + j]) : 0.f;
+            }
         }
     }
-}
+    __device__ __forceinline__ void apply(float (&s)[kR][kR], float scale) const {
+#pragma unroll
+        for (int c = 0; c < kR; ++c)
+#pragma unroll
+            for (int r = 0; r < kR; ++r) s[r][c] = kept[c] ? fmaf(s[r][c], scale, v[r][c]) : -INFINITY;
+    }
+};
 
 // ---------------------------------------------------------------------------------------
 // forward: grid (query tiles, H, B)
@@ -128,7 +175,12 @@ __global__ void __launch_bounds__(kApThreads) attn_plain_fwd_kernel(const __grid
     const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
     const T* k = static_cast<const T*>(p.k.p) + b * p.k.b + hk * p.k.h;
     const T* v = static_cast<const T*>(p.v.p) + b * p.v.b + hk * p.v.h;
-    ap_load<T, kT>(Q, static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h, p.q.l, i0, p.Lq, p.D, nullptr);
+    const bool vk = ap_vec<T>(p.k, p.D), vv = ap_vec<T>(p.v, p.D);
+    ApTile<T, kT, kC> tk, tv;
+    tk.fetch(static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h, p.q.l, i0, p.Lq, p.D, nullptr, ap_vec<T>(p.q, p.D));
+    tk.put(Q, p.D);
+    tk.fetch(k, p.k.l, 0, p.Lk, p.D, keep, vk);
+    tv.fetch(v, p.v.l, 0, p.Lk, p.D, keep, vv);
     float o[kR][kC], m[kR], l[kR];
 #pragma unroll
     for (int r = 0; r < kR; ++r) {
@@ -139,12 +191,18 @@ __global__ void __launch_bounds__(kApThreads) attn_plain_fwd_kernel(const __grid
     }
     for (int j0 = 0; j0 < p.Lk; j0 += kT) {
         __syncthreads();
-        ap_load<T, kT>(K, k, p.k.l, j0, p.Lk, p.D, keep);
-        ap_load<T, kT>(V, v, p.v.l, j0, p.Lk, p.D, keep);
+        tk.put(K, p.D);
+        tv.put(V, p.D);
         __syncthreads();
+        ApBias<T, kR> bias;
+        bias.fetch(p, b, h, i0, j0, ty, tx);
+        if (j0 + kT < p.Lk) {
+            tk.fetch(k, p.k.l, j0 + kT, p.Lk, p.D, keep, vk);
+            tv.fetch(v, p.v.l, j0 + kT, p.Lk, p.D, keep, vv);
+        }
         float s[kR][kR];
         ap_dot<kR>(s, Q, K, p.D, ty, tx);
-        ap_scores<T, kR>(s, p, b, h, i0, j0, ty, tx);
+        bias.apply(s, p.scale);
 #pragma unroll
         for (int r = 0; r < kR; ++r) {
             float mx = s[r][0];
@@ -194,53 +252,74 @@ __global__ void __launch_bounds__(kApThreads) attn_plain_fwd_kernel(const __grid
     }
 }
 
-// delta_i = sum_d dout_id o_id, a warp per row.  With 16-bit outputs the part that rounding took off o is added back:
-// where the probabilities' gradients nearly cancel against delta, half a step of o would be all that is left.
-template <typename T>
+// delta_i = sum_d dout_id o_id, kLanes lanes per row (four columns a piece where rows allow it).  With 16-bit outputs the part
+// that rounding took off o is added back: where the probabilities' gradients nearly cancel against delta, half a step of o
+// would be all that is left.
+template <typename T, int kLanes>
 __global__ void __launch_bounds__(kApThreads) attn_delta_kernel(const __grid_constant__ AttnParams p) {
     griddep_wait();
     griddep_launch_dependents();
-    const long long row = (long long)blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5);
-    if (row >= (long long)p.B * p.Lq * p.H) return;
-    const int lane = threadIdx.x & 31;
-    const int h = (int)(row % p.H);
-    const long long bi = row / p.H;
-    const int i = (int)(bi % p.Lq), b = (int)(bi / p.Lq);
-    const T* o = static_cast<const T*>(p.o.p) + b * p.o.b + (long long)i * p.o.l + h * p.o.h;
-    const T* g = static_cast<const T*>(p.dout.p) + b * p.dout.b + (long long)i * p.dout.l + h * p.dout.h;
+    const long long row = ((long long)blockIdx.x * kApThreads + threadIdx.x) / kLanes;
+    const int lane = threadIdx.x % kLanes;
+    const bool in = row < (long long)p.B * p.Lq * p.H;
     float t = 0.f;
-    for (int d = lane; d < p.D; d += 32) {
-        float y = at_float(o[d]);
-        if constexpr (sizeof(T) == 2) {
-            if (p.o_lo != nullptr) y += __bfloat162float(static_cast<const __nv_bfloat16*>(p.o_lo)[row * p.D + d]);
+    int h = 0, i = 0, b = 0;
+    if (in) {
+        h = (int)(row % p.H);
+        const long long bi = row / p.H;
+        i = (int)(bi % p.Lq);
+        b = (int)(bi / p.Lq);
+        const T* o = static_cast<const T*>(p.o.p) + b * p.o.b + (long long)i * p.o.l + h * p.o.h;
+        const T* g = static_cast<const T*>(p.dout.p) + b * p.dout.b + (long long)i * p.dout.l + h * p.dout.h;
+        const T* lo = sizeof(T) == 2 && p.o_lo != nullptr ? static_cast<const T*>(p.o_lo) + row * p.D : nullptr;
+        if (ap_vec<T>(p.o, p.D) && ap_vec<T>(p.dout, p.D) && (lo == nullptr || (reinterpret_cast<uintptr_t>(lo) & 7) == 0)) {
+            using V = typename ApRaw<T>::V;
+            for (int d = lane * 4; d < p.D; d += kLanes * 4) {
+                float4 y = ap_wide(*reinterpret_cast<const V*>(o + d));
+                const float4 x = ap_wide(*reinterpret_cast<const V*>(g + d));
+                if (lo != nullptr) {
+                    const float4 z = ap_wide(*reinterpret_cast<const V*>(lo + d));
+                    y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+                }
+                t = fmaf(y.x, x.x, fmaf(y.y, x.y, fmaf(y.z, x.z, fmaf(y.w, x.w, t))));
+            }
+        } else {
+            for (int d = lane; d < p.D; d += kLanes) t = fmaf(at_float(o[d]) + (lo != nullptr ? at_float(lo[d]) : 0.f), at_float(g[d]), t);
         }
-        t = fmaf(y, at_float(g[d]), t);
     }
 #pragma unroll
-    for (int s = 16; s >= 1; s >>= 1) t += __shfl_xor_sync(0xffffffffu, t, s);
-    if (lane == 0) p.delta[((long long)b * p.H + h) * p.Lq + i] = t;
+    for (int s = kLanes / 2; s >= 1; s >>= 1) t += __shfl_xor_sync(0xffffffffu, t, s);
+    if (in && lane == 0) p.delta[((long long)b * p.H + h) * p.Lq + i] = t;
 }
 
-// Probabilities and score gradients of a tile from its scores s and products g = dout . v.
+// Statistics of a thread's rows; then probabilities and score gradients from scores s and products g = dout . v.
 template <int kR>
-__device__ __forceinline__ void ap_probs(float (&s)[kR][kR], float (&g)[kR][kR], const AttnParams& p, int b, int h, int i0, int ty) {
+struct ApStats {
+    float2 st[kR];
+    float delta[kR];
+    __device__ __forceinline__ void fetch(const AttnParams& p, int b, int h, int i0, int ty) {
 #pragma unroll
-    for (int r = 0; r < kR; ++r) {
-        const int i = i0 + ty * kR + r;
-        float2 st = make_float2(0.f, INFINITY);
-        float delta = 0.f;
-        if (i < p.Lq) {
-            st = p.stats[((long long)b * p.H + h) * p.Lq + i];
-            delta = p.delta[((long long)b * p.H + h) * p.Lq + i];
-        }
-#pragma unroll
-        for (int c = 0; c < kR; ++c) {
-            const float e = exp2f(fmaf(s[r][c] - st.x, kLog2e, -st.y));
-            s[r][c] = e;
-            g[r][c] = e == 0.f ? 0.f : e * (g[r][c] - delta);
+        for (int r = 0; r < kR; ++r) {
+            const int i = i0 + ty * kR + r;
+            st[r] = make_float2(0.f, INFINITY);
+            delta[r] = 0.f;
+            if (i < p.Lq) {
+                st[r] = p.stats[((long long)b * p.H + h) * p.Lq + i];
+                delta[r] = p.delta[((long long)b * p.H + h) * p.Lq + i];
+            }
         }
     }
-}
+    __device__ __forceinline__ void apply(float (&s)[kR][kR], float (&g)[kR][kR]) const {
+#pragma unroll
+        for (int r = 0; r < kR; ++r)
+#pragma unroll
+            for (int c = 0; c < kR; ++c) {
+                const float e = exp2f(fmaf(s[r][c] - st[r].x, kLog2e, -st[r].y));
+                s[r][c] = e;
+                g[r][c] = e == 0.f ? 0.f : e * (g[r][c] - delta[r]);
+            }
+    }
+};
 
 // ---------------------------------------------------------------------------------------
 // gradient of q, and of the scores where the bias wants one: grid (query tiles, H, B)
@@ -258,8 +337,16 @@ __global__ void __launch_bounds__(kApThreads) attn_plain_dq_kernel(const __grid_
     const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
     const T* k = static_cast<const T*>(p.k.p) + b * p.k.b + hk * p.k.h;
     const T* v = static_cast<const T*>(p.v.p) + b * p.v.b + hk * p.v.h;
-    ap_load<T, kT>(Q, static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h, p.q.l, i0, p.Lq, p.D, nullptr);
-    ap_load<T, kT>(G, static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h, p.dout.l, i0, p.Lq, p.D, nullptr);
+    const bool vk = ap_vec<T>(p.k, p.D), vv = ap_vec<T>(p.v, p.D);
+    ApTile<T, kT, kC> tk, tv;
+    tk.fetch(static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h, p.q.l, i0, p.Lq, p.D, nullptr, ap_vec<T>(p.q, p.D));
+    tv.fetch(static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h, p.dout.l, i0, p.Lq, p.D, nullptr, ap_vec<T>(p.dout, p.D));
+    tk.put(Q, p.D);
+    tv.put(G, p.D);
+    tk.fetch(k, p.k.l, 0, p.Lk, p.D, keep, vk);
+    tv.fetch(v, p.v.l, 0, p.Lk, p.D, keep, vv);
+    ApStats<kR> st;
+    st.fetch(p, b, h, i0, ty);
     float o[kR][kC];
 #pragma unroll
     for (int r = 0; r < kR; ++r)
@@ -267,14 +354,20 @@ __global__ void __launch_bounds__(kApThreads) attn_plain_dq_kernel(const __grid_
         for (int c = 0; c < kC; ++c) o[r][c] = 0.f;
     for (int j0 = 0; j0 < p.Lk; j0 += kT) {
         __syncthreads();
-        ap_load<T, kT>(K, k, p.k.l, j0, p.Lk, p.D, keep);
-        ap_load<T, kT>(V, v, p.v.l, j0, p.Lk, p.D, keep);
+        tk.put(K, p.D);
+        tv.put(V, p.D);
         __syncthreads();
+        ApBias<T, kR> bias;
+        bias.fetch(p, b, h, i0, j0, ty, tx);
+        if (j0 + kT < p.Lk) {
+            tk.fetch(k, p.k.l, j0 + kT, p.Lk, p.D, keep, vk);
+            tv.fetch(v, p.v.l, j0 + kT, p.Lk, p.D, keep, vv);
+        }
         float s[kR][kR], g[kR][kR];
         ap_dot<kR>(s, Q, K, p.D, ty, tx);
-        ap_scores<T, kR>(s, p, b, h, i0, j0, ty, tx);
         ap_dot<kR>(g, G, V, p.D, ty, tx);
-        ap_probs<kR>(s, g, p, b, h, i0, ty);
+        bias.apply(s, p.scale);
+        st.apply(s, g);
 #pragma unroll
         for (int r = 0; r < kR; ++r) {
             const int i = i0 + ty * kR + r;
@@ -317,37 +410,50 @@ __global__ void __launch_bounds__(kApThreads) attn_plain_dkv_kernel(const __grid
     griddep_wait();
     griddep_launch_dependents();
     const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
-    ap_load<T, kT>(K, static_cast<const T*>(p.k.p) + b * p.k.b + hk * p.k.h, p.k.l, j0, p.Lk, p.D, keep);
-    ap_load<T, kT>(V, static_cast<const T*>(p.v.p) + b * p.v.b + hk * p.v.h, p.v.l, j0, p.Lk, p.D, keep);
+    const bool vq = ap_vec<T>(p.q, p.D), vg = ap_vec<T>(p.dout, p.D);
+    const int nq = (p.Lq + kT - 1) / kT;
+    ApTile<T, kT, kC> tq, tg;
+    tq.fetch(static_cast<const T*>(p.k.p) + b * p.k.b + hk * p.k.h, p.k.l, j0, p.Lk, p.D, keep, ap_vec<T>(p.k, p.D));
+    tg.fetch(static_cast<const T*>(p.v.p) + b * p.v.b + hk * p.v.h, p.v.l, j0, p.Lk, p.D, keep, ap_vec<T>(p.v, p.D));
+    tq.put(K, p.D);
+    tg.put(V, p.D);
+    auto fetch = [&](int it) {
+        const int h = hk * group + it / nq, i0 = it % nq * kT;
+        tq.fetch(static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h, p.q.l, i0, p.Lq, p.D, nullptr, vq);
+        tg.fetch(static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h, p.dout.l, i0, p.Lq, p.D, nullptr, vg);
+    };
+    fetch(0);
     float dk[kR][kC], dv[kR][kC];
 #pragma unroll
     for (int r = 0; r < kR; ++r)
 #pragma unroll
         for (int c = 0; c < kC; ++c) dk[r][c] = dv[r][c] = 0.f;
-    for (int h = hk * group; h < (hk + 1) * group; ++h) {
-        const T* q = static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h;
-        const T* go = static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h;
-        for (int i0 = 0; i0 < p.Lq; i0 += kT) {
-            __syncthreads();
-            ap_load<T, kT>(Q, q, p.q.l, i0, p.Lq, p.D, nullptr);
-            ap_load<T, kT>(G, go, p.dout.l, i0, p.Lq, p.D, nullptr);
-            __syncthreads();
-            float s[kR][kR], g[kR][kR];
-            ap_dot<kR>(s, Q, K, p.D, ty, tx);
-            ap_scores<T, kR>(s, p, b, h, i0, j0, ty, tx);
-            ap_dot<kR>(g, G, V, p.D, ty, tx);
-            ap_probs<kR>(s, g, p, b, h, i0, ty);
+    for (int it = 0; it < group * nq; ++it) {
+        const int h = hk * group + it / nq, i0 = it % nq * kT;
+        __syncthreads();
+        tq.put(Q, p.D);
+        tg.put(G, p.D);
+        __syncthreads();
+        ApBias<T, kR> bias;
+        bias.fetch(p, b, h, i0, j0, ty, tx);
+        ApStats<kR> st;
+        st.fetch(p, b, h, i0, ty);
+        if (it + 1 < group * nq) fetch(it + 1);
+        float s[kR][kR], g[kR][kR];
+        ap_dot<kR>(s, Q, K, p.D, ty, tx);
+        ap_dot<kR>(g, G, V, p.D, ty, tx);
+        bias.apply(s, p.scale);
+        st.apply(s, g);
 #pragma unroll
-            for (int r = 0; r < kR; ++r)
+        for (int r = 0; r < kR; ++r)
 #pragma unroll
-                for (int c = 0; c < kR; ++c) {          // transposed: rows of keys
-                    P[(tx + 16 * c) * pp + ty * kR + r] = s[r][c];
-                    S[(tx + 16 * c) * pp + ty * kR + r] = g[r][c];
-                }
-            __syncthreads();
-            ap_mix<kT, kR, kC>(dv, P, G, p.D, ty, tx);
-            ap_mix<kT, kR, kC>(dk, S, Q, p.D, ty, tx);
-        }
+            for (int c = 0; c < kR; ++c) {              // transposed: rows of keys
+                P[(tx + 16 * c) * pp + ty * kR + r] = s[r][c];
+                S[(tx + 16 * c) * pp + ty * kR + r] = g[r][c];
+            }
+        __syncthreads();
+        ap_mix<kT, kR, kC>(dv, P, G, p.D, ty, tx);
+        ap_mix<kT, kR, kC>(dk, S, Q, p.D, ty, tx);
     }
 #pragma unroll
     for (int r = 0; r < kR; ++r) {

@@ -237,11 +237,14 @@ bool tensor_cores(const trimul_attn_desc* d) {
     if (d->dtype != TRIMUL_DTYPE_BF16 || (d->flags & TRIMUL_ATTN_FLAG_PLAIN) != 0) return false;
     return (d->D % 8) == 0 && d->D <= 128;
 }
+bool copies_bias(const trimul_attn_desc* d) {
+    return tensor_cores(d) && d->bias != nullptr && (d->flags & TRIMUL_ATTN_FLAG_COPY_BIAS) != 0;
+}
 bool tensor_core_forward(const trimul_attn_desc* d) {
     if (!tensor_cores(d) || !tma_rows(d->q, d->Lq, d->H, d->B) || !tma_rows(d->k, d->Lk, d->Hk, d->B) ||
         !tma_rows(d->v, d->Lk, d->Hk, d->B) || !tma_rows(d->o, d->Lq, d->H, d->B) || !aligned(d->o_lo, 16))
         return false;
-    if (d->bias == nullptr) return true;
+    if (d->bias == nullptr || copies_bias(d)) return true;
     return tma_rows(trimul_attn_tensor{const_cast<void*>(d->bias), d->bias_b, d->bias_i, d->bias_h}, d->Lq, d->bias_heads, d->bias_batch);
 }
 
@@ -293,7 +296,7 @@ int forward_splits(const trimul_attn_desc* d) {
 // delta, then the scores' gradients where the bias's gradient sums them.  Depends on sizes, type, flags, the shape of the bias and
 // on whether there are a mask and a gradient of the bias, not on addresses or strides.
 struct AttnWorkspace {
-    int64_t words, list, part_o, part_ml, delta, ds, ds_pitch, total;
+    int64_t words, list, bias, part_o, part_ml, delta, ds, ds_pitch, total;
 };
 AttnWorkspace attn_workspace(const trimul_attn_desc* d, bool backward) {
     AttnWorkspace w = {};
@@ -305,6 +308,10 @@ AttnWorkspace attn_workspace(const trimul_attn_desc* d, bool backward) {
         at += align_up(d->B * tiles * 16, 256);
         w.list = at;
         at += align_up(d->B * (tiles + 1) * 4, 256);
+    }
+    if (copies_bias(d)) {
+        w.bias = at;
+        at += align_up((int64_t)d->bias_batch * d->bias_heads * d->Lq * align_up(d->Lk, 8) * 2, 256);
     }
     // by sizes alone, so that a caller may keep the answer: room for either kernel's parts
     const int splits = backward ? 1 : std::max(short_sizes(d) ? short_splits(d) : 1, tc ? forward_splits(d) : 1);
@@ -389,6 +396,21 @@ int run_short(const trimul_attn_desc* d, const AttnParams& p, const AttnWorkspac
     return run_combine<T>(p, sp.part_o, sp.part_ml, sp.splits, st);
 }
 
+// `d` with the bias where the tensor-core kernels can fetch it
+int run_bias_rows(trimul_attn_desc* d, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
+    if (!copies_bias(d)) return TRIMUL_OK;
+    const int64_t rows = (int64_t)d->bias_batch * d->bias_heads * d->Lq, pitch = align_up(d->Lk, 8);
+    const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, 8), 16 * (int64_t)sm_count()));
+    const int rc = launch_stage(attn_bias_rows_kernel, grid, 256, 0, st, true, static_cast<const __nv_bfloat16*>(d->bias),
+                                (long long)d->bias_b, (long long)d->bias_h, (long long)d->bias_i,
+                                reinterpret_cast<uint32_t*>(ws + w.bias), d->bias_heads, d->Lq, d->Lk, (long long)rows, (int)pitch);
+    d->bias = ws + w.bias;
+    d->bias_i = pitch;
+    d->bias_h = pitch * d->Lq;
+    d->bias_b = d->bias_h * d->bias_heads;
+    return rc;
+}
+
 template <int kD, bool kBias>
 int launch_fwd(const AttnFwdParams& fp, const CUtensorMap (&m)[4], cudaStream_t st) {
     using L = AfLayout<kD, kBias>;
@@ -397,7 +419,11 @@ int launch_fwd(const AttnFwdParams& fp, const CUtensorMap (&m)[4], cudaStream_t 
     const dim3 grid((unsigned)ceil_div(fp.a.Lq, 2 * kAfRows), (unsigned)fp.a.H, (unsigned)(fp.a.B * fp.splits));
     return launch_stage(kernel, grid, kAfThreads, L::kSmem, st, true, m[0], m[1], m[2], m[3], fp);
 }
-int run_fwd(const trimul_attn_desc* d, const AttnParams& p, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
+int run_fwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
+    trimul_attn_desc copy = *given;
+    const trimul_attn_desc* d = &copy;
+    int rc = run_bias_rows(&copy, w, ws, st);
+    if (rc != TRIMUL_OK) return rc;
     AttnFwdParams fp = {};
     fp.a = p;
     fp.n_tiles = (int)ceil_div(d->Lk, kAfRows);
@@ -418,12 +444,11 @@ int run_fwd(const trimul_attn_desc* d, const AttnParams& p, const AttnWorkspace&
     if (d->mask != nullptr) {
         uint32_t* words = reinterpret_cast<uint32_t*>(ws + w.words);
         int* list = reinterpret_cast<int*>(ws + w.list);
-        const int rc = run_mask(d, words, list, st);
+        rc = run_mask(d, words, list, st);
         if (rc != TRIMUL_OK) return rc;
         fp.words = words;
         fp.list = list;
     }
-    int rc;
     if (d->D <= 64) rc = d->bias != nullptr ? launch_fwd<64, true>(fp, m, st) : launch_fwd<64, false>(fp, m, st);
     else rc = d->bias != nullptr ? launch_fwd<128, true>(fp, m, st) : launch_fwd<128, false>(fp, m, st);
     if (rc != TRIMUL_OK || fp.splits == 1) return rc;
@@ -444,7 +469,11 @@ int launch_bwd(const AttnBwdParams& bp, const CUtensorMap (&m)[5], cudaStream_t 
     return launch_stage(dq, dim3((unsigned)ceil_div(p.Lq, kAfRows), (unsigned)p.H, (unsigned)p.B), kAbThreads, Q::kSmem, st, true,
                         m[0], m[1], m[2], m[3], m[4], bp);
 }
-int run_bwd(const trimul_attn_desc* d, const AttnParams& p, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
+int run_bwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
+    trimul_attn_desc copy = *given;
+    const trimul_attn_desc* d = &copy;
+    int rc = run_bias_rows(&copy, w, ws, st);
+    if (rc != TRIMUL_OK) return rc;
     AttnBwdParams bp = {};
     bp.a = p;
     bp.n_tiles = (int)ceil_div(d->Lk, kAfRows);
@@ -459,7 +488,7 @@ int run_bwd(const trimul_attn_desc* d, const AttnParams& p, const AttnWorkspace&
     if (d->mask != nullptr) {
         uint32_t* words = reinterpret_cast<uint32_t*>(ws + w.words);
         int* list = reinterpret_cast<int*>(ws + w.list);
-        const int rc = run_mask(d, words, list, st);
+        rc = run_mask(d, words, list, st);
         if (rc != TRIMUL_OK) return rc;
         bp.words = words;
         bp.list = list;
@@ -568,9 +597,11 @@ int trimul_b200_attn_backward(const trimul_attn_desc* d, void* workspace, size_t
     }
     const bool bf16 = d->dtype == TRIMUL_DTYPE_BF16;
     const int64_t rows = (int64_t)d->B * d->Lq * d->H;
-    const dim3 grid((unsigned)ceil_div(rows, kApThreads / 32));
-    if (bf16) rc = launch_stage(attn_delta_kernel<__nv_bfloat16>, grid, kApThreads, 0, st, true, p);
-    else rc = launch_stage(attn_delta_kernel<float>, grid, kApThreads, 0, st, true, p);
+    const int lanes = d->D <= 64 ? 16 : 32;
+    const dim3 grid((unsigned)ceil_div(rows, kApThreads / lanes));
+    auto delta = bf16 ? (lanes == 16 ? attn_delta_kernel<__nv_bfloat16, 16> : attn_delta_kernel<__nv_bfloat16, 32>)
+                      : (lanes == 16 ? attn_delta_kernel<float, 16> : attn_delta_kernel<float, 32>);
+    rc = launch_stage(delta, grid, kApThreads, 0, st, true, p);
     if (rc != TRIMUL_OK) return rc;
     if (tensor_core_backward(d)) rc = run_bwd(d, p, w, ws, st);
     else rc = bf16 ? run_plain_bwd<__nv_bfloat16>(p, st) : run_plain_bwd<float>(p, st);
