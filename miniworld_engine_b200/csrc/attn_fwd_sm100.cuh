@@ -546,7 +546,8 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     }
 }
 
-// Joins the parts of a row: grid over rows, a warp per row.
+// Joins the parts of a row, a warp per row.  Lane s holds the weight of part s (and of s + 32, ...: all blocks of a row fit
+// into a wave, so there are a few hundred parts at most).
 template <typename T>
 __global__ void __launch_bounds__(256)
 attn_combine_kernel(const __grid_constant__ AttnParams p, const float* part_o, const float2* part_ml, int splits) {
@@ -557,32 +558,44 @@ attn_combine_kernel(const __grid_constant__ AttnParams p, const float* part_o, c
     if (r >= rows) return;
     const int lane = threadIdx.x & 31;
     float m = -INFINITY;
-    for (int s = lane; s < splits; s += 32) m = fmaxf(m, part_ml[s * rows + r].x);
+    for (int s = lane; s < splits; s += 32) m = fmaxf(m, __ldg(part_ml + s * rows + r).x);
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int s = lane; s < splits; s += 32) {
-        const float2 ml = part_ml[s * rows + r];
-        l += ml.y * ex2f((ml.x - base) * kLog2e);
+    const bool nothing = m == -INFINITY;
+    const float base = nothing ? 0.f : m;
+    float l = 0.f, y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = 0.f;
+    for (int s0 = 0; s0 < splits; s0 += 32) {
+        const float2 ml = s0 + lane < splits ? __ldg(part_ml + (s0 + lane) * rows + r) : make_float2(-INFINITY, 0.f);
+        const float w = ex2f((ml.x - base) * kLog2e);
+        l = fmaf(ml.y, w, l);
+        const int n = min(32, splits - s0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {           // columns lane + 32 k
+            const int d = lane + 32 * k;
+            if (32 * k >= p.D) break;
+            const float* o = part_o + (s0 * rows + r) * p.D + min(d, p.D - 1);
+#pragma unroll 8
+            for (int s = 0; s < n; ++s) y[k] = fmaf(__ldg(o + s * rows * p.D), __shfl_sync(0xffffffffu, w, s), y[k]);
+        }
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    const bool nothing = m == -INFINITY;
     const float inv = nothing ? 0.f : 1.f / l;
     const int i = (int)(r % p.Lq), h = (int)((r / p.Lq) % p.H), b = (int)(r / p.Lq / p.H);
     if (lane == 0 && p.stats != nullptr) p.stats[r] = nothing ? make_float2(0.f, INFINITY) : make_float2(m, log2f(l));
     T* dst = static_cast<T*>(p.o.p) + b * p.o.b + (long long)i * p.o.l + h * p.o.h;
     const long long lo = (((long long)b * p.Lq + i) * p.H + h) * p.D;
-    for (int d = lane; d < p.D; d += 32) {
-        float y = 0.f;
-        for (int s = 0; s < splits; ++s)
-            y = fmaf(part_o[(s * rows + r) * p.D + d], ex2f((part_ml[s * rows + r].x - base) * kLog2e), y);
-        y = nothing ? 0.f : y * inv;
-        at_store(dst + d, y);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int d = lane + 32 * k;
+        if (d >= p.D) break;
+        const float v = nothing ? 0.f : y[k] * inv;
+        at_store(dst + d, v);
         if constexpr (sizeof(T) == 2) {
             if (p.o_lo != nullptr)
-                static_cast<__nv_bfloat16*>(p.o_lo)[lo + d] = __float2bfloat16_rn(y - __bfloat162float(__float2bfloat16_rn(y)));
+                static_cast<__nv_bfloat16*>(p.o_lo)[lo + d] = __float2bfloat16_rn(v - __bfloat162float(__float2bfloat16_rn(v)));
         }
     }
 }

@@ -86,14 +86,21 @@ attn_short_kernel(const __grid_constant__ AttnShortParams sp) {
     const T* v = static_cast<const T*>(p.v.p) + b * p.v.b + hk * p.v.h + d0;
     const uint8_t* mask = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
     const int k_end = min(p.Lk, (split + 1) * sp.keys_per_split);
-    for (int j0 = split * sp.keys_per_split + warp * kChunk; j0 < k_end; j0 += kAsWarps * kChunk) {
-        // keep[u]: this lane's key of load u counts
-        uint32_t keep = 0;
+    // bit u: this lane's key of load u counts
+    auto kept = [&](int j0) {
+        uint32_t bits = 0;
 #pragma unroll
         for (int u = 0; u < kAsLoads; ++u) {
             const int j = j0 + u * kKeys + sub;
-            keep |= (uint32_t)(j < k_end && (mask == nullptr || mask[j] != 0)) << u;
+            bits |= (uint32_t)(j < k_end && (mask == nullptr || __ldg(mask + j) != 0)) << u;
         }
+        return bits;
+    };
+    const int j_first = split * sp.keys_per_split + warp * kChunk;
+    uint32_t next = kept(j_first);
+    for (int j0 = j_first; j0 < k_end; j0 += kAsWarps * kChunk) {
+        const uint32_t keep = next;
+        next = kept(j0 + kAsWarps * kChunk);         // a step ahead: the loads below do not wait for the mask
         if (mask != nullptr && __all_sync(0xffffffffu, keep == 0u)) continue;
         uint4 kv[kAsLoads], vv[kAsLoads];
 #pragma unroll
@@ -125,11 +132,11 @@ attn_short_kernel(const __grid_constant__ AttnShortParams sp) {
         }
 #pragma unroll
         for (int u = 0; u < kAsLoads; ++u) {
-            const bool kept = (keep >> u) & 1u;
+            const bool counts = (keep >> u) & 1u;
 #pragma unroll
             for (int r = 0; r < kR; ++r) {
-                if (biased && kept) s[u][r] += at_float(bias[r][j0 + u * kKeys + sub]);
-                if (!kept) s[u][r] = -INFINITY;
+                if (biased && counts) s[u][r] += at_float(bias[r][j0 + u * kKeys + sub]);
+                if (!counts) s[u][r] = -INFINITY;
             }
         }
 #pragma unroll

@@ -127,9 +127,11 @@ RelposGradPlan plan_relpos_grad(const trimul_relpos_desc* d, const trimul_bucket
     const int rows = b->count + (b->segments != 0), lut = lut_bytes(lut_reach(b));
     const int kN = d->dtype == TRIMUL_DTYPE_BF16 ? 8 : 4;
     if (d->layout == TRIMUL_RELPOS_HEADS) {
-        // four heads a block where three blocks' sums fit into an SM's shared memory, two where that holds for them
+        // four heads a block where three blocks' sums fit into an SM's shared memory, two where that holds for them; one head
+        // (and more rows at once) where there is little to do
         g.threads = 128;
-        g.heads = d->channels >= 4 && rows * 4 * 128 * 4 <= 72 * 1024 ? 4 : d->channels >= 2 && rows * 2 * 128 * 4 <= 72 * 1024 ? 2 : 1;
+        const int64_t all = (int64_t)d->B * d->Lq * d->Lk * d->channels;
+        g.heads = all < (8 << 20) ? 1 : d->channels >= 4 && rows * 4 * 128 * 4 <= 72 * 1024 ? 4 : d->channels >= 2 && rows * 2 * 128 * 4 <= 72 * 1024 ? 2 : 1;
         while (g.threads > 32 && rows * g.threads * 4 > 96 * 1024) g.threads /= 2;
         // as many blocks as are resident at once, parts of at least four steps and at most 1024 rows (whose positions a
         // block keeps)

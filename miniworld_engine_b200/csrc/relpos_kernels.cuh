@@ -49,6 +49,10 @@ __device__ __forceinline__ int rp_rule(const trimul_buckets& b, int d) {
     const int half = b.kind == TRIMUL_BUCKETS_LOG ? b.count / 2 : b.count;
     const int n = b.kind == TRIMUL_BUCKETS_LOG ? abs(d) : max(d, 0);
     int lo = 0, hi = b.n_thresholds;
+    if (hi <= 32) {          // all threads read the same threshold at a time: no divergent reads of the parameter space
+        for (int t = 0; t < b.n_thresholds; ++t) lo += b.thresholds[t] <= n;
+        hi = lo;
+    }
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (b.thresholds[mid] <= n) lo = mid + 1; else hi = mid;
@@ -412,13 +416,24 @@ relpos_heads_grad_kernel(const __grid_constant__ RelposParams p, const __grid_co
     __syncthreads();
     // a warp per sum: lanes over the threads' columns
     const int warp = tid >> 5, lane = tid & 31, warps = nt >> 5;
-    for (int x = warp; x < p.rows * kH; x += warps) {
-        float t = 0.f;
-        for (int e = lane; e < nt; e += 32) t += acc[x * nt + e];
+    constexpr int kX = 4;                   // sums of a warp at a time
+    for (int x0 = warp * kX; x0 < p.rows * kH; x0 += warps * kX) {
+        float t[kX];
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-        const int u = x / kH, h = h0 + x % kH;
-        if (lane == 0 && h < p.C) partial[((long long)blockIdx.x * p.rows + u) * p.C + h] = t;
+        for (int k = 0; k < kX; ++k) {
+            t[k] = 0.f;
+            if (x0 + k < p.rows * kH)
+                for (int e = lane; e < nt; e += 32) t[k] += acc[(x0 + k) * nt + e];
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1)
+#pragma unroll
+            for (int k = 0; k < kX; ++k) t[k] += __shfl_xor_sync(0xffffffffu, t[k], o);
+#pragma unroll
+        for (int k = 0; k < kX; ++k) {
+            const int u = (x0 + k) / kH, h = h0 + (x0 + k) % kH;
+            if (lane == 0 && u < p.rows && h < p.C) partial[((long long)blockIdx.x * p.rows + u) * p.C + h] = t[k];
+        }
     }
 }
 
@@ -443,6 +458,15 @@ template <typename T, int kL, int kRun>
 struct RpRun {
     typename RpLane<T, kL>::V g[kRun];
     int u, n;
+    static __device__ __forceinline__ void move_to(float* acc, int& run, float (&sum)[kL], int to) {
+        if (to == run) return;
+#pragma unroll
+        for (int e = 0; e < kL; ++e) {
+            acc[run * 32 * kL + e] += sum[e];
+            sum[e] = 0.f;
+        }
+        run = to;
+    }
     __device__ __forceinline__ void load(const RelposParams& p, const uint16_t* lut, const T* grad, long long pos, long long last, int c0,
                                          int lane, RpCursor& cur) {
         n = (int)max(0ll, min((long long)kRun, last - pos));
@@ -459,18 +483,24 @@ struct RpRun {
         }
     }
     __device__ __forceinline__ void add(float* acc, int& run, float (&sum)[kL]) const {
+        // most runs have one bucket (a whole one, at the end of a warp's share maybe less): no test per position then
+        const int u0 = __shfl_sync(0xffffffffu, u, 0);
+        if (n == kRun && __all_sync(0xffffffffu, u == u0 || (int)(threadIdx.x & 31) >= kRun)) {
+            move_to(acc, run, sum, u0);
+#pragma unroll
+            for (int s = 0; s < kRun; ++s) {
+                float f[kL];
+                rp_lane(g[s], f);
+#pragma unroll
+                for (int e = 0; e < kL; ++e) sum[e] += f[e];
+            }
+            return;
+        }
 #pragma unroll
         for (int s = 0; s < kRun; ++s) {
             if (s >= n) break;
             const int us = __shfl_sync(0xffffffffu, u, s);
-            if (us != run) {
-#pragma unroll
-                for (int e = 0; e < kL; ++e) {
-                    acc[run * 32 * kL + e] += sum[e];
-                    sum[e] = 0.f;
-                }
-                run = us;
-            }
+            move_to(acc, run, sum, us);
             float f[kL];
             rp_lane(g[s], f);
 #pragma unroll
