@@ -445,12 +445,34 @@ relpos_heads_grad_kernel(const __grid_constant__ RelposParams p, const __grid_co
 template <typename T, int kL> struct RpLane { using V = T; };             // kL channels of a lane
 template <> struct RpLane<__nv_bfloat16, 4> { using V = uint2; };
 template <> struct RpLane<float, 4> { using V = float4; };
-__device__ __forceinline__ void rp_lane(const __nv_bfloat16& v, float (&f)[1]) { f[0] = __bfloat162float(v); }
-__device__ __forceinline__ void rp_lane(const float& v, float (&f)[1]) { f[0] = v; }
-__device__ __forceinline__ void rp_lane(const uint2& v, float (&f)[4]) {
-    f[0] = bf16_lo(v.x); f[1] = bf16_hi(v.x); f[2] = bf16_lo(v.y); f[3] = bf16_hi(v.y);
+template <int kL> struct RpSum { f32x2 v[(kL + 1) / 2]; };                // kL sums as packed pairs
+__device__ __forceinline__ void rp_add(RpSum<1>& s, const __nv_bfloat16& v) { s.v[0] = f2_add(s.v[0], f2_pack(__bfloat162float(v), 0.f)); }
+__device__ __forceinline__ void rp_add(RpSum<1>& s, const float& v) { s.v[0] = f2_add(s.v[0], f2_pack(v, 0.f)); }
+__device__ __forceinline__ void rp_add(RpSum<4>& s, const uint2& v) {
+    s.v[0] = f2_add(s.v[0], f2_from_bf16x2(v.x));
+    s.v[1] = f2_add(s.v[1], f2_from_bf16x2(v.y));
 }
-__device__ __forceinline__ void rp_lane(const float4& v, float (&f)[4]) { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+__device__ __forceinline__ void rp_add(RpSum<4>& s, const float4& v) {
+    s.v[0] = f2_add(s.v[0], f2_pack(v.x, v.y));
+    s.v[1] = f2_add(s.v[1], f2_pack(v.z, v.w));
+}
+// the sums to their bucket's row in shared memory, and back to zero
+template <int kL> __device__ __forceinline__ void rp_flush(float* acc, int row, RpSum<kL>& s) {
+    float f[(kL + 1) / 2 * 2];
+#pragma unroll
+    for (int e = 0; e < (kL + 1) / 2; ++e) {
+        f2_unpack(s.v[e], f[2 * e], f[2 * e + 1]);
+        s.v[e] = 0ull;
+    }
+    float* a = acc + row * 32 * kL;
+    if constexpr (kL == 4) {
+        float4 x = *reinterpret_cast<float4*>(a);
+        x.x += f[0]; x.y += f[1]; x.z += f[2]; x.w += f[3];
+        *reinterpret_cast<float4*>(a) = x;
+    } else {
+        a[0] += f[0];
+    }
+}
 
 // `kRun` positions of one warp (their channels of this lane, and a bucket per lane).  Two of them live in registers: one is
 // added up while the other is in flight.
@@ -458,53 +480,44 @@ template <typename T, int kL, int kRun>
 struct RpRun {
     typename RpLane<T, kL>::V g[kRun];
     int u, n;
-    static __device__ __forceinline__ void move_to(float* acc, int& run, float (&sum)[kL], int to) {
-        if (to == run) return;
-#pragma unroll
-        for (int e = 0; e < kL; ++e) {
-            acc[run * 32 * kL + e] += sum[e];
-            sum[e] = 0.f;
-        }
-        run = to;
-    }
     __device__ __forceinline__ void load(const RelposParams& p, const uint16_t* lut, const T* grad, long long pos, long long last, int c0,
                                          int lane, RpCursor& cur) {
+        using V = typename RpLane<T, kL>::V;
         n = (int)max(0ll, min((long long)kRun, last - pos));
-        const T* src = grad + pos * p.C + c0;
+        const char* src = reinterpret_cast<const char*>(grad + pos * p.C + c0);
+        const uint32_t step = (uint32_t)p.C * (uint32_t)sizeof(T);
+        if (n == kRun && c0 < p.C) {
 #pragma unroll
-        for (int s = 0; s < kRun; ++s) {
-            g[s] = typename RpLane<T, kL>::V();
-            if (s < n && c0 < p.C) g[s] = __ldcs(reinterpret_cast<const typename RpLane<T, kL>::V*>(src + (long long)s * p.C));
+            for (int s = 0; s < kRun; ++s) g[s] = __ldcs(reinterpret_cast<const V*>(src + s * step));
+        } else {
+#pragma unroll
+            for (int s = 0; s < kRun; ++s) {
+                g[s] = V();
+                if (s < n && c0 < p.C) g[s] = __ldcs(reinterpret_cast<const V*>(src + s * step));
+            }
         }
-        u = 0;
+        u = -1;
         if (lane < n) {
             u = cur.bucket(p, lut);
             cur.step(p, kRun);
         }
     }
-    __device__ __forceinline__ void add(float* acc, int& run, float (&sum)[kL]) const {
-        // most runs have one bucket (a whole one, at the end of a warp's share maybe less): no test per position then
-        const int u0 = __shfl_sync(0xffffffffu, u, 0);
-        if (n == kRun && __all_sync(0xffffffffu, u == u0 || (int)(threadIdx.x & 31) >= kRun)) {
-            move_to(acc, run, sum, u0);
+    __device__ __forceinline__ void add(float* acc, int& run, RpSum<kL>& sum, int lane) const {
+        // bit s: position s starts another bucket than the one before it
+        const int before = __shfl_up_sync(0xffffffffu, u, 1);
+        const uint32_t starts = __ballot_sync(0xffffffffu, lane < n && u != (lane == 0 ? run : before));
+        if (n == kRun && starts == 0u) {               // most runs: no test per position
 #pragma unroll
-            for (int s = 0; s < kRun; ++s) {
-                float f[kL];
-                rp_lane(g[s], f);
-#pragma unroll
-                for (int e = 0; e < kL; ++e) sum[e] += f[e];
-            }
+            for (int s = 0; s < kRun; ++s) rp_add(sum, g[s]);
             return;
         }
 #pragma unroll
         for (int s = 0; s < kRun; ++s) {
-            if (s >= n) break;
-            const int us = __shfl_sync(0xffffffffu, u, s);
-            move_to(acc, run, sum, us);
-            float f[kL];
-            rp_lane(g[s], f);
-#pragma unroll
-            for (int e = 0; e < kL; ++e) sum[e] += f[e];
+            if ((starts >> s) & 1u) {
+                rp_flush(acc, run, sum);
+                run = __shfl_sync(0xffffffffu, u, s);
+            }
+            rp_add(sum, g[s]);                         // zero behind the last position
         }
     }
 };
@@ -528,21 +541,18 @@ relpos_pair_grad_kernel(const __grid_constant__ RelposParams p, const __grid_con
     const long long total = (long long)p.B * p.Lq * p.Lk;
     const long long first = ((long long)blockIdx.x * warps + warp) * pos_per_warp, last = min(first + pos_per_warp, total);
     int run = 0;
-    float sum[kL];
-#pragma unroll
-    for (int e = 0; e < kL; ++e) sum[e] = 0.f;
+    RpSum<kL> sum = {};
     RpCursor cur;
     if (first < last) cur.init(p, min(first + lane, total - 1));
     RpRun<T, kL, kRun> a, b;
     a.load(p, lut, grad, first, last, c0, lane, cur);
     for (long long pos = first; pos < last; pos += 2 * kRun) {
         b.load(p, lut, grad, pos + kRun, last, c0, lane, cur);
-        a.add(acc, run, sum);
+        a.add(acc, run, sum, lane);
         a.load(p, lut, grad, pos + 2 * kRun, last, c0, lane, cur);
-        b.add(acc, run, sum);
+        b.add(acc, run, sum, lane);
     }
-#pragma unroll
-    for (int e = 0; e < kL; ++e) acc[run * 32 * kL + e] += sum[e];
+    rp_flush(acc, run, sum);
     __syncthreads();
     const int width = min(32 * kL, p.C - (int)blockIdx.y * 32 * kL);
     for (int e = tid; e < p.rows * 32 * kL; e += nt) {
