@@ -83,7 +83,7 @@ attn_bias_rows_kernel(const __nv_bfloat16* src, long long src_b, long long src_h
 }
 
 // Key mask as bits, and the list of tiles that keep something.  One block per batch element.
-constexpr int kMaskPrepThreads = 256;
+constexpr int kMaskPrepThreads = 1024;
 __global__ void __launch_bounds__(kMaskPrepThreads)
 attn_mask_kernel(const uint8_t* mask, long long mask_b, int Lk, int n_tiles, uint32_t* words, int* list) {
     __shared__ int any[kMaskPrepThreads / 32];

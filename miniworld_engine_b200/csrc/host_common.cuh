@@ -71,7 +71,7 @@ inline int sm_count() {
 // attribute call is not free and these entry points sit on latency-sensitive host paths.
 inline bool ensure_smem_once(const void* fn, int bytes) {
     struct Entry { const void* fn; uint64_t devices; };
-    static Entry table[64];
+    static Entry table[256];
     static int used = 0;
     static std::mutex mu;
     int dev = 0;
@@ -82,7 +82,7 @@ inline bool ensure_smem_once(const void* fn, int bytes) {
         if (table[i].fn == fn) e = &table[i];
     if (e != nullptr && dev < 64 && ((e->devices >> dev) & 1u)) return true;
     if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
-    if (e == nullptr && used < 64) { e = &table[used++]; e->fn = fn; e->devices = 0; }
+    if (e == nullptr && used < 256) { e = &table[used++]; e->fn = fn; e->devices = 0; }
     if (e != nullptr && dev < 64) e->devices |= 1ull << dev;
     return true;
 }

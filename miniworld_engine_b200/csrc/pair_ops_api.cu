@@ -159,13 +159,17 @@ RelposGradPlan plan_relpos_grad(const trimul_relpos_desc* d, const trimul_bucket
     return g;
 }
 
+// whether a lane of the pair gradient may take four channels at a time
+bool wide_lanes(const trimul_relpos_desc* d, const void* grad) {
+    return (d->channels % 4) == 0 && aligned(grad, 4 * elem_size(d->dtype));
+}
+
 template <typename T>
 int run_relpos_grad(const trimul_relpos_desc* d, const trimul_buckets* b, const RelposParams& p, const void* grad,
                     void* dtable, float* partial, cudaStream_t st) {
     constexpr int kN = RpVec<T>::kN;
     int rc;
-    const bool wide = (d->channels % 4) == 0 && aligned(grad, 4 * sizeof(T));
-    const RelposGradPlan g = plan_relpos_grad(d, b, wide);
+    const RelposGradPlan g = plan_relpos_grad(d, b, wide_lanes(d, grad));
     if (d->layout == TRIMUL_RELPOS_HEADS) {
         const bool vec = aligned(grad, 16) && (p.sB % kN) == 0 && (p.sH % kN) == 0 && (p.sI % kN) == 0;
         auto kernel = g.heads == 4 ? (vec ? relpos_heads_grad_kernel<T, true, 4> : relpos_heads_grad_kernel<T, false, 4>)
@@ -180,7 +184,7 @@ int run_relpos_grad(const trimul_relpos_desc* d, const trimul_buckets* b, const 
         rc = launch_stage(kernel, dim3((unsigned)g.parts, (unsigned)g.column_blocks), g.threads, g.smem, st, true, p, *b,
                           static_cast<const T*>(grad), partial, (long long)g.per_part);
     }
-    if (rc != TRIMUL_OK) return rc;
+    if (rc != TRIMUL_OK || partial == dtable) return rc;
     const int n = p.rows * p.C;
     return launch_stage(relpos_reduce_kernel, dim3((unsigned)ceil_div(n, 32)), kRpReduceThreads, 0, st, true,
                         static_cast<const float*>(partial), dtable, p.table_bf16, g.parts, n);
@@ -545,7 +549,9 @@ int trimul_b200_relpos_bias_grad(const trimul_relpos_desc* d, const trimul_bucke
     if (!aligned(workspace, 16)) return TRIMUL_E_INVALID;
     const RelposParams p = relpos_params(d, b, nullptr, q_pos, k_pos, q_seg, k_seg);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    float* partial = static_cast<float*>(workspace);
+    // a single part is the result
+    const int parts = plan_relpos_grad(d, b, wide_lanes(d, grad)).parts;
+    float* partial = static_cast<float*>(parts == 1 && !p.table_bf16 ? dtable : workspace);
     return d->dtype == TRIMUL_DTYPE_BF16 ? run_relpos_grad<__nv_bfloat16>(d, b, p, grad, dtable, partial, st)
                                          : run_relpos_grad<float>(d, b, p, grad, dtable, partial, st);
 }

@@ -287,3 +287,41 @@ def test_learned_bias_and_attention_together():
     value, bound = (sums(t) for t in want["dbias"])
     n = torch.bincount(u.flatten(), minlength=33)[:, None] * 2.0 ** -24
     check(mod.weight.grad, (value, bound + n * sums(want["dbias"][0].abs())), "table")
+
+
+@pytest.mark.parametrize("Lq", [1, 40])
+def test_offsets_beyond_32_bits(Lq):
+    """Keys, values and a bias whose rows lie more than 2^31 elements apart in all."""
+    step = 1 << 26
+    Lk, H, D = 40, 2, 64
+    big = torch.empty(Lk * step, dtype=BF16, device="cuda")                # 5.4 GB
+    q, k, v, g, b, m = _inputs(1, Lq, Lk, H, H, D, "1H", "holes", BF16)
+    far = lambda t, at: torch.as_strided(big, t.shape, (Lk * step, step, D, 1), at).copy_(t)
+    k2, v2 = far(k, 0), far(v, 1024)
+    rows = torch.as_strided(big, b.shape, (Lk * step, Lq * step, step, 1), 4096) if Lq <= 20 else b
+    if rows is not b:
+        rows.copy_(b)
+    got, bare = _both(q, k2, v2, g, rows, m)
+    want, wb = _both(q, k, v, g, b, m)
+    assert torch.equal(bare, wb) and all(torch.equal(got[n], want[n]) for n in want)
+
+
+def test_first_calls_inside_a_capture_and_backward_twice():
+    """Gradients accumulate as autograd has it, and the explicit calls may be captured without a call before."""
+    from miniworld_engine_b200 import cross_attention_b200
+    q, k, v, g, b, m = _inputs(1, 77, 93, 2, 2, 40, "1H", "tail", BF16)       # a head dimension no other test has
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, bare = _both(q, k, v, g, b, m)
+    graph.replay()
+    torch.cuda.synchronize()
+    want = attention64(q, k, v, b, m, None, g)
+    for name in want:
+        check(got[name], want[name], name)
+    leaves = [t.float().requires_grad_(True) for t in (q, k, v, b)]
+    for _ in range(2):
+        cross_attention_b200(*leaves[:3], bias=leaves[3], key_mask=m).backward(g.float())
+    once = [t.clone().requires_grad_(True) for t in (x.detach() for x in leaves)]
+    cross_attention_b200(*once[:3], bias=once[3], key_mask=m).backward(g.float())
+    for a, c in zip(leaves, once):
+        assert torch.equal(a.grad, 2 * c.grad)

@@ -215,3 +215,29 @@ def test_streams_and_graphs():
     torch.cuda.synchronize()
     for o, w in zip(outs, want):
         assert torch.equal(o[0], w[0]) and torch.equal(o[1], w[1])
+
+
+@pytest.mark.parametrize("layout", ["heads", "pair"])
+def test_offsets_beyond_32_bits(layout):
+    """Results and gradients of more than 2^31 elements: the last rows are right, and every element is counted."""
+    from miniworld_engine_b200 import relative_position_bias_b200, relative_position_bias_backward_b200
+    n, c = (12000, 16) if layout == "heads" else (4200, 128)
+    pos = torch.arange(n, device="cuda")
+    buckets = _rule("clip32", False)
+    table = torch.randn(65, c, device="cuda")
+    out = relative_position_bias_b200(table, buckets, pos, layout=layout, dtype=torch.bfloat16)
+    assert out.numel() > 2 ** 31
+    last = bucket_matrix(pos[-3:], pos, "clip", 65, 32).cuda()
+    if layout == "heads":
+        assert torch.equal(out[:, -3:], table[last].bfloat16().movedim(-1, 0))
+    else:
+        assert torch.equal(out[-3:], table[last].bfloat16())
+    out.fill_(2.0 ** -10)
+    got = relative_position_bias_backward_b200(out, buckets, pos, layout=layout)
+    d = torch.arange(-32, 33, device="cuda")
+    pairs = n - d.abs()
+    pairs[0] = pairs[-1] = (n - 32) * (n - 31) // 2
+    # counts up to 7e7 do not fit into 24 bits: exact within a part (less than 2^24 elements), then at most 2^10 parts are
+    # added, each addition off by 2^-24 of the sum.  A row left out would be 2^-13.6 of it
+    want = (pairs.double() * 2.0 ** -10)[:, None]
+    assert ((got.double() - want).abs() <= 2.0 ** -14 * want).all()
