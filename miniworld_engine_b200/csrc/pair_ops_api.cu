@@ -12,6 +12,7 @@
 
 #include "host_common.cuh"
 #include "attn_bwd_sm100.cuh"
+#include "attn_fwd64_sm100.cuh"
 #include "attn_fwd_sm100.cuh"
 #include "attn_plain.cuh"
 #include "attn_short.cuh"
@@ -425,6 +426,13 @@ int launch_fwd(const AttnFwdParams& fp, const CUtensorMap (&m)[4], cudaStream_t 
     const dim3 grid((unsigned)ceil_div(fp.a.Lq, 2 * kAfRows), (unsigned)fp.a.H, (unsigned)(fp.a.B * fp.splits));
     return launch_stage(kernel, grid, kAfThreads, L::kSmem, st, true, m[0], m[1], m[2], m[3], fp);
 }
+template <bool kBias>
+int launch_fwd64(const AttnFwdParams& fp, const CUtensorMap (&m)[4], cudaStream_t st) {
+    auto kernel = attn_fwd64_sm100_kernel<kBias>;
+    if (!ensure_smem(kernel, A6Layout<kBias>::kSmem)) return TRIMUL_E_CUDA;
+    const dim3 grid((unsigned)ceil_div(fp.a.Lq, 2 * kAfRows), (unsigned)fp.a.H, (unsigned)(fp.a.B * fp.splits));
+    return launch_stage(kernel, grid, kA6Threads, A6Layout<kBias>::kSmem, st, true, m[0], m[1], m[2], m[3], fp);
+}
 int run_fwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
     trimul_attn_desc copy = *given;
     const trimul_attn_desc* d = &copy;
@@ -455,7 +463,7 @@ int run_fwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorksp
         fp.words = words;
         fp.list = list;
     }
-    if (d->D <= 64) rc = d->bias != nullptr ? launch_fwd<64, true>(fp, m, st) : launch_fwd<64, false>(fp, m, st);
+    if (d->D <= 64) rc = d->bias != nullptr ? launch_fwd64<true>(fp, m, st) : launch_fwd64<false>(fp, m, st);
     else rc = d->bias != nullptr ? launch_fwd<128, true>(fp, m, st) : launch_fwd<128, false>(fp, m, st);
     if (rc != TRIMUL_OK || fp.splits == 1) return rc;
     return run_combine<__nv_bfloat16>(p, fp.part_o, fp.part_ml, fp.splits, st);
