@@ -5,10 +5,11 @@
 // tile w, half p of every tile of 128 keys), each with its own softmax warps (a thread owns a row), its own running maximum
 // and sum and its own O in tensor memory; while one chain loads scores or waits for its products, the other three
 // exponentiate.  At the end the two chains of a query tile are joined through shared memory.  Two chains over whole key
-// tiles (as for wider heads) left the exponentials idle for two fifths of the time: 71 us instead of FIG_NOBIAS for 2048 x 4096,
+// tiles (as for wider heads) left the exponentials idle for two fifths of the time: 71 us instead of 62 for 2048 x 4096,
 // 18 heads of 64.
-// 640 threads: warp 0 TMA producer, warp 1 UMMA issuer, warp 2 cleans value rows of masked keys, warp 3 bias producer,
-// warps 4 + 4 c ... the softmax warps of chain c = 2 p + w.
+// 640 threads: warp 0 TMA producer, warps 1 and 3 UMMA issuers of query tiles 0 and 1 (one warp for all four chains was busy
+// for longer than the exponentials take), warp 2 cleans value rows of masked keys, warps 4 + 4 c ... the softmax warps of
+// chain c = 2 p + w.
 // Tensor memory of chain c: S (64 columns, P overlays the first 32) at 128 c, O (64 columns) after it.  The next scores of a
 // chain are issued after the product that reads its P, and tcgen05.mma of one thread run in the order of issue.
 #pragma once
@@ -88,7 +89,7 @@ attn_fwd64_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         }
         for (int s = 0; s < kSt; ++s) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+            mbar_init(&empty[s], two ? 2 : 1);       // one commit per issuer
         }
         for (int s = 0; s < kAfClean; ++s) mbar_init(&v_ok[s], 1);
         *abort_flag = 0;
@@ -128,31 +129,44 @@ attn_fwd64_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 mbar_arrive_expect_tx(&full[s], L::kTile);
                 tma_load_4d(ring + s * L::kTile, (it & 1) ? &tmV : &tmK, &full[s], 0, tile_at(it >> 1) * kAfRows, hk, b);
                 if (it == 0 && two) load_q(1);
+                if (kBias && (it & 1) == 0) {            // the chains' bias tiles between keys and values
+                    const int j = it >> 1, buf = j % kBb;
+                    bool ok = true;
+                    for (int c = 0; ok && c < 4; ++c) {
+                        if ((c & 1) != 0 && !two) continue;
+                        ok = mbar_wait<true>(&b_empty[c * 2 + buf], ((j / kBb) & 1) ^ 1, abort_flag, p.status, kStageIdAttnFwd64, 600 + c);
+                        if (!ok) break;
+                        mbar_arrive_expect_tx(&b_full[c * 2 + buf], L::kTile);
+                        tma_load_4d(sBias + (c * kBb + buf) * L::kTile, &tmBias, &b_full[c * 2 + buf], tile_at(j) * kAfRows + (c >> 1) * 64,
+                                    i0 + (c & 1) * kAfRows, fp.bias_h1 ? 0 : h, fp.bias_b1 ? 0 : b);
+                    }
+                    if (!ok) break;
+                }
             }
         }
         __syncwarp();
-    } else if (warp == 1) {
-        if (n > 0) {
+    } else if (warp == 1 || warp == 3) {
+        const int w = warp == 3;
+        if (n > 0 && (w == 0 || two)) {
             constexpr uint32_t idesc_s = umma_idesc_bf16(128, 64);
             constexpr uint32_t idesc_o = umma_idesc_bf16(128, 64, 0, 1);
-            const int tiles = two ? 2 : 1;
             bool ok = true;
             auto wait = [&](uint64_t* bar, uint32_t ph, int detail) {
                 ok = ok && warp_wait(bar, ph, lane, abort_flag, p.status, kStageIdAttnFwd64, detail);
                 tcgen05_fence_after();
                 return ok;
             };
-            const uint64_t dq = umma_smem_desc_sw128(smem_u32(sQ)), dk = umma_smem_desc_sw128(smem_u32(ring));
+            const uint64_t dq = umma_smem_desc_sw128(smem_u32(sQ + w * L::kTile)), dk = umma_smem_desc_sw128(smem_u32(ring));
             const uint64_t dv = umma_smem_desc_mn_sw128(smem_u32(ring), kAfSub, 1024);
             constexpr uint64_t kHalf = (64 * 128) >> 4;          // 64 rows of a tile
-            auto scores = [&](int half, int w, int slot) {
-                const uint64_t a = dq + (uint64_t)(w * (L::kTile >> 4)), k = dk + (uint64_t)(slot * (L::kTile >> 4)) + half * kHalf;
+            auto scores = [&](int half, int slot) {
+                const uint64_t k = dk + (uint64_t)(slot * (L::kTile >> 4)) + half * kHalf;
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
-                    umma_ss_warp(tmem + (2 * half + w) * 128, a + kk * kDescKStep, k + kk * kDescKStep, idesc_s, kk > 0);
+                    umma_ss_warp(tmem + (2 * half + w) * 128, dq + kk * kDescKStep, k + kk * kDescKStep, idesc_s, kk > 0);
                 umma_commit_warp(&s_full[2 * half + w]);
             };
-            auto mix = [&](int half, int w, int slot, bool add) {
+            auto mix = [&](int half, int slot, bool add) {
                 const uint64_t v = dv + (uint64_t)(slot * (L::kTile >> 4)) + half * kHalf;
                 const uint32_t t = tmem + (2 * half + w) * 128;
 #pragma unroll
@@ -164,12 +178,9 @@ attn_fwd64_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 slot += 2;
                 if (slot >= kSt) { slot -= kSt; ph ^= 1u; }
             };
-            if (wait(&full[0], 0, 300)) {
-                for (int w = 0; ok && w < tiles; ++w)
-                    if (wait(&q_full[w], 0, 310 + w)) {
-                        scores(0, w, 0);
-                        scores(1, w, 0);
-                    }
+            if (wait(&full[0], 0, 300) && wait(&q_full[w], 0, 310 + w)) {
+                scores(0, 0);
+                scores(1, 0);
                 umma_commit_warp(&empty[0]);
             }
             step(sk, phk);
@@ -178,14 +189,13 @@ attn_fwd64_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 if (fp.words != nullptr) wait(&v_ok[j % kAfClean], (j / kAfClean) & 1, 320);
                 else wait(&full[sv], phv, 321);
                 if (more) wait(&full[sk], phk, 340);
-                for (int half = 0; ok && half < 2; ++half)
-                    for (int w = 0; ok && w < tiles; ++w) {
-                        const int c = 2 * half + w;
-                        if (!wait(&p_full[c], j & 1, 330 + c)) break;
-                        mix(half, w, sv, j > 0);
-                        if (more) scores(half, w, sk);
-                        else umma_commit_warp(&o_full[c]);
-                    }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (!wait(&p_full[2 * half + w], j & 1, 330 + 2 * half + w)) break;
+                    mix(half, sv, j > 0);
+                    if (more) scores(half, sk);
+                    else umma_commit_warp(&o_full[2 * half + w]);
+                }
                 if (!ok) break;
                 umma_commit_warp(&empty[sv]);
                 if (more) umma_commit_warp(&empty[sk]);
@@ -213,23 +223,6 @@ attn_fwd64_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 if (lane == 0) mbar_arrive(&v_ok[j % kAfClean]);
             }
         }
-    } else if (warp == 3) {
-        if (kBias && lane == 0) {
-            bool ok = true;
-            for (int j = 0; ok && j < n; ++j) {
-                const int j0 = tile_at(j) * kAfRows, buf = j % kBb;
-                for (int half = 0; ok && half < 2; ++half)
-                    for (int w = 0; ok && w < (two ? 2 : 1); ++w) {
-                        const int s = (2 * half + w) * 2 + buf;
-                        ok = mbar_wait<true>(&b_empty[s], ((j / kBb) & 1) ^ 1, abort_flag, p.status, kStageIdAttnFwd64, 600 + s);
-                        if (!ok) break;
-                        mbar_arrive_expect_tx(&b_full[s], L::kTile);
-                        tma_load_4d(sBias + ((2 * half + w) * kBb + buf) * L::kTile, &tmBias, &b_full[s], j0 + half * 64, i0 + w * kAfRows,
-                                    fp.bias_h1 ? 0 : h, fp.bias_b1 ? 0 : b);
-                    }
-            }
-        }
-        __syncwarp();
     } else {
         const int c = (warp - 4) >> 2, w = c & 1, half = c >> 1, q = warp & 3, row = q * 32 + lane, i = i0 + w * kAfRows + row;
         if (w == 0 || two) {

@@ -1,22 +1,25 @@
-// Cross attention, forward, on the tensor cores (bf16, head dimension a multiple of 8 up to 128).
+// Cross attention, forward, on the tensor cores (bf16) for head dimensions of 72 to 128, and what the tensor-core kernels
+// share.  Narrower heads: attn_fwd64_sm100.cuh.
 //
 // One pass over the keys with a running maximum and sum: S = Q K^T and O += P V are tcgen05.mma with accumulators in
 // tensor memory, P goes back to tensor memory as the A operand of the second product and never touches shared memory.
 // A block owns two tiles of 128 queries of one head.  While the softmax warps of one tile exponentiate, the tensor cores
 // work for the other.  384 threads:
 //   warp 0      TMA producer: queries once, then key and value tiles of 128 rows through one ring of slots
-//   warp 1      UMMA issuer
+//   warp 1      UMMA issuer (a second one, a warp per query tile, made it 15 % slower)
 //   warp 2      with a key mask: zeroes the value rows of masked keys in shared memory, whose probabilities are zero but
 //               which may hold infinities or NaN
-//   warp 3      TMA producer of the bias tiles [128 queries][128 keys], one buffer (kD = 64: two) per query tile
+//   warp 3      TMA producer of the bias tiles [128 queries][128 keys], one buffer per query tile
 //   warps 4-7, 8-11   softmax of one query tile each: a thread owns a row
 // The running maximum a row is scaled by lags behind the true one by up to 2^8: O is rescaled only when a row's maximum
 // has grown by more (accumulators and sums are fp32, where a common factor of 2^8 costs nothing).
-// Tensor memory: S of both tiles [0, 256), O of both from 256.  kD = 64: P has columns of its own, and the next scores are
-// issued as soon as the present ones are in registers.  kD = 128: the 512 columns are full, P overlays the first half of its
-// own S, and the next scores follow the product that reads P (tcgen05.mma of one thread run in the order of issue, so they
-// cannot overtake it).  P is handed over in halves of 64 keys, so that its product starts while the rest is exponentiated.
-// Head dimensions below kD are filled with zeros by the TMA loads.
+// Tensor memory is full: S of both tiles [0, 256), O of both from 256.  P overlays the first half of its own S, and the next
+// scores follow the product that reads P (tcgen05.mma of one thread run in the order of issue, so they cannot overtake it).
+// P is handed over in halves of 64 keys, so that its product starts while the rest is exponentiated.
+// What bounds it: softmax, product and next scores of a query tile wait for each other (3500 cycles a round for both tiles, of
+// which the tensor cores work 2100 and the exponentials 2048), and blocks of 256 queries: 4096 x 8192 with 16 heads of 128 is
+// 256 blocks for 148 SMs.  1058 TFLOP/s there (0.64 of the measured GEMM rate).  Softmax by two warps per row (each half the keys) measured the same.
+// Head dimensions below 128 are filled with zeros by the TMA loads.
 #pragma once
 
 #include "attn_common.cuh"
@@ -28,18 +31,19 @@ constexpr int kAfRows = 128;                     // rows of a query or key tile
 constexpr int kAfSub = 128 * 128;                // 128 rows x 64 bf16, swizzled
 constexpr int kAfClean = 4;                      // at least the value tiles that the ring holds at once
 constexpr int kStageIdAttnFwd = 11;
+constexpr int kAfD = 128;                        // columns of head dimension
 constexpr float kAfSlack = 8.f;                  // log2 of what a row's maximum may grow without a rescale
 
-template <int kD, bool kBias>
+template <bool kBias>
 struct AfLayout {
-    static constexpr int kTile = kD / 64 * kAfSub;                        // one query, key or value tile
-    static constexpr int kBiasBufs = kBias ? (kD == 64 ? 2 : 1) : 0;      // per query tile
-    static constexpr int kStages = kBias ? (kD == 64 ? 4 : 3) : (kD == 64 ? 8 : 5);
+    static constexpr int kTile = 2 * kAfSub;                              // one query, key or value tile
+    static constexpr int kStages = kBias ? 3 : 5;
     static_assert((kStages + 1) / 2 <= kAfClean, "a value tile must be consumed before its barrier is used again");
     static constexpr int kOffBias = 2 * kTile;
-    static constexpr int kOffRing = kOffBias + 2 * kBiasBufs * 2 * kAfSub;
+    static constexpr int kOffRing = kOffBias + (kBias ? 2 * 2 * kAfSub : 0);
     static constexpr int kOffBars = kOffRing + kStages * kTile;
-    static constexpr int kSmem = kOffBars + 512;
+    static constexpr int kSmem = kOffBars + 256;
+    static_assert((14 + 2 * kStages + kAfClean) * 8 + 8 <= 256, "barriers");
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -124,14 +128,16 @@ __device__ __forceinline__ uint4 tail_words(int left) {      // bits of the firs
     auto w = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; };
     return make_uint4(w(left), w(left - 32), w(left - 64), w(left - 96));
 }
-template <int kD, bool kBias>
+
+template <bool kBias>
 __global__ void __launch_bounds__(kAfThreads, 1)
 attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmBias,
                       const __grid_constant__ AttnFwdParams fp) {
-    using L = AfLayout<kD, kBias>;
+    using L = AfLayout<kBias>;
+    constexpr int kD = kAfD;
     const AttnParams& p = fp.a;
-    constexpr int kSt = L::kStages, kBb = L::kBiasBufs > 0 ? L::kBiasBufs : 1;
+    constexpr int kSt = L::kStages;
     extern __shared__ __align__(1024) uint8_t smem[];
     if ((smem_u32(smem) & 1023u) != 0u) {
         if (threadIdx.x == 0) report_timeout(p.status, kStageIdAttnFwd, 900);
@@ -143,12 +149,11 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBars);
     uint64_t* q_full = bars;                   // [2]
     uint64_t* s_full = q_full + 2;             // [2] scores of a key tile complete
-    uint64_t* s_read = s_full + 2;             // [2] scores are in registers (kD = 64)
-    uint64_t* p_full = s_read + 2;             // [2][2] probabilities in tensor memory, O rescaled where it had to be; kD = 128: by halves
-    uint64_t* o_full = p_full + 4;             // [2] product complete (kD = 128: the last one)
-    uint64_t* b_full = o_full + 2;             // [2][kBb]
-    uint64_t* b_empty = b_full + 2 * kBb;      // [2][kBb]
-    uint64_t* full = b_empty + 2 * kBb;        // [kSt]
+    uint64_t* p_full = s_full + 2;             // [2][2] half of the probabilities in tensor memory, O rescaled where it had to be
+    uint64_t* o_full = p_full + 4;             // [2] last product complete
+    uint64_t* b_full = o_full + 2;             // [2]
+    uint64_t* b_empty = b_full + 2;            // [2]
+    uint64_t* full = b_empty + 2;        // [kSt]
     uint64_t* empty = full + kSt;              // [kSt]
     uint64_t* v_ok = empty + kSt;              // [kAfClean] masked value rows zeroed, value tile j at j % kAfClean
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_ok + kAfClean);
@@ -163,12 +168,11 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         for (int w = 0; w < 2; ++w) {
             mbar_init(&q_full[w], 1);
             mbar_init(&s_full[w], 1);
-            mbar_init(&s_read[w], 4);
             mbar_init(&p_full[2 * w], 4);
             mbar_init(&p_full[2 * w + 1], 4);
             mbar_init(&o_full[w], 1);
         }
-        for (int s = 0; s < 2 * kBb; ++s) {
+        for (int s = 0; s < 2; ++s) {
             mbar_init(&b_full[s], 1);
             mbar_init(&b_empty[s], 4);
         }
@@ -225,9 +229,9 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         __syncwarp();
     } else if (warp == 1) {
         if (n > 0) {
+            const int tiles = two ? 2 : 1;
             constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128);
             constexpr uint32_t idesc_o = umma_idesc_bf16(128, kD, 0, 1);
-            const int tiles = two ? 2 : 1;
             bool ok = true;
             auto wait = [&](uint64_t* bar, uint32_t ph, int detail) {
                 ok = ok && warp_wait(bar, ph, lane, abort_flag, p.status, kStageIdAttnFwd, detail);
@@ -247,7 +251,7 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             };
             auto mix = [&](int w, int slot, int half, bool add) {     // O_w += P_w V over 64 keys
                 const uint64_t v = dv + (uint64_t)(slot * (L::kTile >> 4));
-                const uint32_t pt = tmem + (kD == 128 ? w * 128 : 384 + w * 64);
+                const uint32_t pt = tmem + w * 128;
 #pragma unroll
                 for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
                     umma_ts_warp(tmem + 256 + w * kD, pt + kk * 8, v + ((kk * 2048) >> 4), idesc_o, add || kk > 0);
@@ -267,24 +271,15 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             step(sk, phk);
             for (int j = 0; ok && j < n; ++j) {
                 const bool more = j + 1 < n;
-                if (kD == 64 && more && wait(&full[sk], phk, 340)) {
-                    // scores have columns of their own: the next ones follow as soon as these are in registers
-                    for (int w = 0; ok && w < tiles; ++w)
-                        if (wait(&s_read[w], j & 1, 350 + w)) scores(w, sk);
-                    umma_commit_warp(&empty[sk]);
-                }
                 if (fp.words != nullptr) wait(&v_ok[j % kAfClean], (j / kAfClean) & 1, 320);
                 else wait(&full[sv], phv, 321);
                 for (int w = 0; ok && w < tiles; ++w) {
-                    for (int half = 0; half < (kD == 64 ? 1 : 2); ++half)
-                        if (wait(&p_full[2 * w + half], j & 1, 330 + w)) {
-                            mix(w, sv, half, j > 0);
-                            if (kD == 64) mix(w, sv, 1, true);
-                        }
+                    for (int half = 0; half < 2; ++half)
+                        if (wait(&p_full[2 * w + half], j & 1, 330 + w)) mix(w, sv, half, j > 0);
                     if (!ok) break;
-                    if (kD == 64 || !more) umma_commit_warp(&o_full[w]);
+                    if (!more) umma_commit_warp(&o_full[w]);
                     if (w == tiles - 1) umma_commit_warp(&empty[sv]);
-                    if (kD == 128 && more) {
+                    if (more) {
                         if (w == 0 && !wait(&full[sk], phk, 340)) break;
                         scores(w, sk);
                         if (w == tiles - 1) umma_commit_warp(&empty[sk]);
@@ -322,15 +317,14 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         if (kBias && lane == 0) {
             bool ok = true;
             for (int j = 0; ok && j < n; ++j) {
-                const int j0 = tile_at(j) * kAfRows, buf = j % kBb;
+                const int j0 = tile_at(j) * kAfRows;
                 for (int w = 0; ok && w < (two ? 2 : 1); ++w) {
-                    const int s = w * kBb + buf;
-                    ok = mbar_wait<true>(&b_empty[s], ((j / kBb) & 1) ^ 1, abort_flag, p.status, kStageIdAttnFwd, 600 + s);
+                    ok = mbar_wait<true>(&b_empty[w], (j & 1) ^ 1, abort_flag, p.status, kStageIdAttnFwd, 600 + w);
                     if (!ok) break;
-                    mbar_arrive_expect_tx(&b_full[s], 2 * kAfSub);
+                    mbar_arrive_expect_tx(&b_full[w], 2 * kAfSub);
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
-                        tma_load_4d(sBias + (s * 2 + u) * kAfSub, &tmBias, &b_full[s], j0 + u * 64, i0 + w * kAfRows,
+                        tma_load_4d(sBias + (w * 2 + u) * kAfSub, &tmBias, &b_full[w], j0 + u * 64, i0 + w * kAfRows,
                                     fp.bias_h1 ? 0 : h, fp.bias_b1 ? 0 : b);
                 }
             }
@@ -341,8 +335,7 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         if (w == 0 || two) {
             const uint32_t lane_off = (uint32_t)(q * 32) << 16;
             const uint32_t tS = tmem + w * 128 + lane_off;
-            const uint32_t tP = tmem + (kD == 128 ? w * 128 : 384 + w * 64) + lane_off;
-            const uint32_t tO = tmem + 256 + w * kD + lane_off;
+            const uint32_t tP = tS, tO = tmem + 256 + w * kD + lane_off;
             // scores are kept in units of which `mul` makes base-2 exponents: raw products, or with a bias (or a scale that is
             // not positive) what they come to
             const float c2 = p.scale * kLog2e;
@@ -363,16 +356,10 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 #pragma unroll
                 for (int k = 0; k < 4; ++k) tmem_ld_32x32(tS + 32 * k, s[k]);
                 tmem_ld_wait();
-                if (kD == 64) {
-                    tcgen05_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&s_read[w]);
-                }
                 if constexpr (kBias) {
-                    const int bs = w * kBb + j % kBb;
-                    if (!(ok = warp_wait(&b_full[bs], (j / kBb) & 1, lane, abort_flag, p.status, kStageIdAttnFwd, 410 + w))) break;
+                    if (!(ok = warp_wait(&b_full[w], j & 1, lane, abort_flag, p.status, kStageIdAttnFwd, 410 + w))) break;
                     const f32x2 sc = f2_pack(p.scale, p.scale);
-                    const uint8_t* br = sBias + bs * 2 * kAfSub + row * 128;
+                    const uint8_t* br = sBias + w * 2 * kAfSub + row * 128;
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -389,7 +376,7 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
                             }
                         }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&b_empty[bs]);
+                    if (lane == 0) mbar_arrive(&b_empty[w]);
                 } else if (!raw) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
@@ -418,7 +405,21 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
                 const float base = m == -INFINITY ? 0.f : m;
                 f32x2 sum[2] = {0ull, 0ull};
                 const f32x2 mul2 = f2_pack(mul, mul), off2 = f2_pack(-base * mul, -base * mul), nb2 = f2_pack(-base, -base);
-                auto exponentiate = [&](int k, uint32_t (&pk)[16]) {
+                // these scores were issued after the product of the tile before: O and P may change
+                if (rescale) {
+#pragma unroll 1
+                    for (int cc = 0; cc < kD; cc += 16) {
+                        uint32_t o[16];
+                        tmem_ld_32x16(tO + cc, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st_32x16(tO + cc, o);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t pk[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const f32x2 x = f2_pack(__uint_as_float(s[k][2 * e]), __uint_as_float(s[k][2 * e + 1]));
@@ -429,51 +430,17 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
                         sum[e & 1] = f2_add(sum[e & 1], f2_pack(a, d));
                         pk[e] = pack_bf16x2(a, d);
                     }
-                };
-                auto rescale_o = [&] {
-#pragma unroll 1
-                    for (int cc = 0; cc < kD; cc += 16) {
-                        uint32_t o[16];
-                        tmem_ld_32x16(tO + cc, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st_32x16(tO + cc, o);
-                    }
-                };
-                auto hand_over = [&](int half) {
-                    tmem_st_wait();
-                    tcgen05_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[2 * w + half]);
-                };
-                if constexpr (kD == 64) {
-                    // the product of the tile before may still run: all exponentials first, then O and P change
-                    uint32_t pk[4][16];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) exponentiate(k, pk[k]);
-                    if (j > 0) {
-                        if (!(ok = warp_wait(&o_full[w], (j - 1) & 1, lane, abort_flag, p.status, kStageIdAttnFwd, 430 + w))) break;
-                        tcgen05_fence_after();
-                        if (rescale) rescale_o();
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) tmem_st_32x16(tP + 16 * k, pk[k]);
-                    hand_over(0);
-                } else {
-                    // these scores were issued after the product of the tile before
-                    if (rescale) rescale_o();
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        uint32_t pk[16];
-                        exponentiate(k, pk);
-                        tmem_st_32x16(tP + 16 * k, pk);
-                        if (k & 1) hand_over(k >> 1);     // half of the keys: the product with their values can start
+                    tmem_st_32x16(tP + 16 * k, pk);
+                    if (k & 1) {             // half of the keys: the product with their values can start
+                        tmem_st_wait();
+                        tcgen05_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_full[2 * w + (k >> 1)]);
                     }
                 }
                 l += f2_hsum(f2_add(sum[0], sum[1]));
             }
-            if (n > 0 && ok) ok = warp_wait(&o_full[w], kD == 64 ? (n - 1) & 1 : 0, lane, abort_flag, p.status, kStageIdAttnFwd, 420 + w);
+            if (n > 0 && ok) ok = warp_wait(&o_full[w], 0, lane, abort_flag, p.status, kStageIdAttnFwd, 420 + w);
             tcgen05_fence_after();
             if (ok) {
                 const bool nothing = m == -INFINITY || n == 0;

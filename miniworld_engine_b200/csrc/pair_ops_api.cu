@@ -418,10 +418,10 @@ int run_bias_rows(trimul_attn_desc* d, const AttnWorkspace& w, uint8_t* ws, cuda
     return rc;
 }
 
-template <int kD, bool kBias>
+template <bool kBias>
 int launch_fwd(const AttnFwdParams& fp, const CUtensorMap (&m)[4], cudaStream_t st) {
-    using L = AfLayout<kD, kBias>;
-    auto kernel = attn_fwd_sm100_kernel<kD, kBias>;
+    using L = AfLayout<kBias>;
+    auto kernel = attn_fwd_sm100_kernel<kBias>;
     if (!ensure_smem(kernel, L::kSmem)) return TRIMUL_E_CUDA;
     const dim3 grid((unsigned)ceil_div(fp.a.Lq, 2 * kAfRows), (unsigned)fp.a.H, (unsigned)(fp.a.B * fp.splits));
     return launch_stage(kernel, grid, kAfThreads, L::kSmem, st, true, m[0], m[1], m[2], m[3], fp);
@@ -464,7 +464,7 @@ int run_fwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorksp
         fp.list = list;
     }
     if (d->D <= 64) rc = d->bias != nullptr ? launch_fwd64<true>(fp, m, st) : launch_fwd64<false>(fp, m, st);
-    else rc = d->bias != nullptr ? launch_fwd<128, true>(fp, m, st) : launch_fwd<128, false>(fp, m, st);
+    else rc = d->bias != nullptr ? launch_fwd<true>(fp, m, st) : launch_fwd<false>(fp, m, st);
     if (rc != TRIMUL_OK || fp.splits == 1) return rc;
     return run_combine<__nv_bfloat16>(p, fp.part_o, fp.part_ml, fp.splits, st);
 }
