@@ -14,7 +14,9 @@ namespace trimul {
 
 constexpr int kAsThreads = 128;
 constexpr int kAsWarps = kAsThreads / 32;
-template <int kR> __host__ __device__ constexpr int as_loads() { return kR == 8 ? 4 : 8; }      // eight rows of sums leave registers for four
+template <int kR> __host__ __device__ constexpr int as_loads() { return kR == 1 ? 8 : 4; }      // what the rows' sums leave registers for
+// blocks on an SM at once, by the registers of the rows' sums
+__host__ __device__ constexpr int as_blocks(int rows) { return rows <= 1 ? 4 : rows <= 2 ? 5 : rows <= 4 ? 4 : 2; }
 
 struct AttnShortParams {
     AttnParams a;
@@ -40,7 +42,7 @@ template <> struct AsVec<float> {
 
 // kLanes lanes per key row; kR query rows; grid (splits, Hk, B)
 template <typename T, int kLanes, int kR>
-__global__ void __launch_bounds__(kAsThreads)
+__global__ void __launch_bounds__(kAsThreads, as_blocks(kR))
 attn_short_kernel(const __grid_constant__ AttnShortParams sp) {
     constexpr int kN = AsVec<T>::kN, kP = kN / 2;
     constexpr int kKeys = 32 / kLanes;                 // keys of one load

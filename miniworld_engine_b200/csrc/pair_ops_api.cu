@@ -285,10 +285,10 @@ bool short_rows(const trimul_attn_desc* d) {
     };
     return short_sizes(d) && ok(d->k) && ok(d->v);
 }
-// Enough blocks for four on every SM, and keys for two steps of every warp.
+// As many blocks as are resident at once, and keys for two steps of every warp.
 int short_splits(const trimul_attn_desc* d) {
     const int64_t blocks = (int64_t)d->B * d->Hk;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(4 * sm_count() / blocks, d->Lk / 256));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(as_blocks(d->Lq * (d->H / d->Hk)) * sm_count() / blocks, d->Lk / 256));
 }
 
 // Key splits of the forward pass: where the blocks leave SMs idle, each block takes a share of the key tiles (two at
