@@ -272,11 +272,16 @@ bool encode_bias(CUtensorMap* map, const trimul_attn_desc* d) {
                        d->bias_batch);
 }
 
-// Few query rows per key head: the kernel that reads keys and values once for all of them.  Its rows are 16-byte pieces.
+// Few query rows per key head: the kernel that reads keys and values once for all of them.  Its rows are 16-byte pieces.  Where
+// the tensor-core kernel is the alternative, it has to serve at least as many heads as queries with each key: 8 x 4096 keys, 16
+// key heads of 64 take it 31 / 38 / 57 / 94 us for 1 / 2 / 4 / 8 rows, the tensor-core kernel (which works on 128 rows anyway,
+// and again for every query head) 39 us for any number of queries and one query head per key head; with two query heads per
+// key head 21 against 39.  Heads of 128: 53 / 68 against 60 us for one and two queries, 39 against 60 for two heads.
 constexpr int kShortRows = 8;
 bool short_sizes(const trimul_attn_desc* d) {
-    const int n = 16 / elem_size(d->dtype);
-    return (d->flags & TRIMUL_ATTN_FLAG_PLAIN) == 0 && (int64_t)d->Lq * (d->H / d->Hk) <= kShortRows && (d->D % n) == 0 && d->D <= 32 * n;
+    const int n = 16 / elem_size(d->dtype), group = d->H / d->Hk;
+    if ((d->flags & TRIMUL_ATTN_FLAG_PLAIN) != 0 || (d->D % n) != 0 || d->D > 32 * n) return false;
+    return (int64_t)d->Lq * group <= kShortRows && (!tensor_cores(d) || d->Lq <= group);
 }
 bool short_rows(const trimul_attn_desc* d) {
     const int n = 16 / elem_size(d->dtype);
