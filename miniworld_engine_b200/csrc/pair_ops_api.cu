@@ -296,12 +296,14 @@ int short_splits(const trimul_attn_desc* d) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(as_blocks(d->Lq * (d->H / d->Hk)) * sm_count() / blocks, d->Lk / 256));
 }
 
-// Key splits of the forward pass: where the blocks leave SMs idle, each block takes a share of the key tiles (two at
-// least: a lone tile's products and exponentials do not overlap) and a second kernel joins the parts.
+// Key splits of the forward pass: where the blocks leave SMs idle, each block takes a share of the key tiles and a second kernel
+// joins the parts.  Four tiles at least, since the parts cost a launch and their way through memory: 8 heads, 64 queries of 64, us
+// with one / two / four tiles at least: 512 keys 10.4 / 10.1 / 8.5, 1024 9.8 / 11.1 / 12.2, 4096 14.7 / 13.4 / 12.9; 4 heads, 256
+// queries of 128, 8192 keys 35 / 29 / 25.
 int forward_splits(const trimul_attn_desc* d) {
     const int64_t blocks = ceil_div(d->Lq, 2 * kAfRows) * d->H * d->B, tiles = ceil_div(d->Lk, kAfRows);
     const int64_t room = sm_count() / blocks;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(room, tiles / 2));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(room, tiles / 4));
 }
 
 // Workspace.  Both directions: the key mask as bits and its list of tiles.  Forward: the parts of split rows.  Backward:
