@@ -3,9 +3,9 @@
 //   p_ij = exp(x_ij - m_i) / l_i       dp_ij = dout_i . v_j       ds_ij = p_ij (dp_ij - delta_i)
 //   dv_j = sum_i p_ij dout_i           dk_j = scale sum_i ds_ij q_i           dq_i = scale sum_j ds_ij k_j
 //
-// Two kernels, each of which recomputes the scores and owns its results, so nothing is added up across blocks and the
-// same call gives the same bits: one block per key tile walks over the queries (dk, dv), one per query tile over the
-// keys (dq, and ds where the bias wants it).  Together seven products of the scores' size instead of the five that a
+// Two kinds of blocks, each of which recomputes the scores and owns its results, so nothing is added up across blocks and the
+// same call gives the same bits: one per key tile walks over the queries (dk, dv), one per query tile over the keys (dq, and
+// ds where the bias wants it).  Together seven products of the scores' size instead of the five that a
 // single kernel would need, which would have to add up dq through memory.
 //
 // Both: 384 threads (TMA producer, UMMA issuer, a helper warp, bias producer, two groups of four softmax warps that share
@@ -30,6 +30,8 @@ struct AttnBwdParams {
     const uint32_t* words;       // as in the forward kernel
     const int* list;
     int bias_b1, bias_h1;
+    int kv_blocks, q_blocks;     // of the two kinds
+    int q_first;                 // the blocks over the keys come first
 };
 
 template <int kD, bool kBias>
@@ -123,14 +125,12 @@ __device__ __forceinline__ void ab_row_out(uint32_t t, __nv_bfloat16* dst, int D
 }
 
 // ---------------------------------------------------------------------------------------
-// dk, dv: grid (key tiles, Hk, B).  Scores transposed: a lane of tensor memory is a key, a column a query.  Masked keys
+// dk, dv: a block per (key tile, key head, batch element).  Scores transposed: a lane of tensor memory is a key, a column a query.  Masked keys
 // only ever meet their own lanes, so whatever their rows hold stays there, and their results are written as zeros.
 // ---------------------------------------------------------------------------------------
 template <int kD, bool kBias>
-__global__ void __launch_bounds__(kAbThreads, 1)
-attn_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG,
-                      const __grid_constant__ CUtensorMap tmBias, const __grid_constant__ AttnBwdParams bp) {
+__device__ __forceinline__ void attn_dkv_block(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
+                                               const CUtensorMap& tmG, const CUtensorMap& tmBias, const AttnBwdParams& bp, int block) {
     using L = AbKvLayout<kD, kBias>;
     const AttnParams& p = bp.a;
     constexpr int kSt = L::kStages, kBb = L::kBiasBufs > 0 ? L::kBiasBufs : 1;
@@ -158,7 +158,7 @@ attn_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = warp_uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int tile = blockIdx.x, j0 = tile * kAfRows, hk = blockIdx.y, b = blockIdx.z;
+    const int tile = block % bp.n_tiles, j0 = tile * kAfRows, hk = block / bp.n_tiles % p.Hk, b = block / bp.n_tiles / p.Hk;
     const int group = p.H / p.Hk, nq = (p.Lq + kAfRows - 1) / kAfRows;
 
     if (threadIdx.x == 0) {
@@ -387,14 +387,12 @@ attn_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 }
 
 // ---------------------------------------------------------------------------------------
-// dq and ds: grid (query tiles, H, B).  A lane of tensor memory is a query, a column a key.  Key rows of masked keys are
+// dq and ds: a block per (query tile, head, batch element).  A lane of tensor memory is a query, a column a key.  Key rows of masked keys are
 // zeroed in shared memory, where ds K would read them.
 // ---------------------------------------------------------------------------------------
 template <int kD, bool kBias>
-__global__ void __launch_bounds__(kAbThreads, 1)
-attn_dq_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG,
-                     const __grid_constant__ CUtensorMap tmBias, const __grid_constant__ AttnBwdParams bp) {
+__device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
+                                              const CUtensorMap& tmG, const CUtensorMap& tmBias, const AttnBwdParams& bp, int block) {
     using L = AbQLayout<kD, kBias>;
     const AttnParams& p = bp.a;
     constexpr int kKSt = L::kKSt, kVSt = L::kVSt, kBb = L::kBiasBufs > 0 ? L::kBiasBufs : 1;
@@ -421,7 +419,8 @@ attn_dq_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = warp_uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int i0 = blockIdx.x * kAfRows, h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hk);
+    const int nq = (p.Lq + kAfRows - 1) / kAfRows;
+    const int i0 = block % nq * kAfRows, h = block / nq % p.H, b = block / nq / p.H, hk = h / (p.H / p.Hk);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; ++s) {
@@ -652,6 +651,19 @@ attn_dq_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         tcgen05_fence_after();
         tmem_dealloc(tmem, 512);
     }
+}
+
+// Both kinds of blocks in one launch, the kind whose blocks take longer first: its last wave is filled with the other kind's.
+template <int kD, bool kBias>
+__global__ void __launch_bounds__(kAbThreads, 1)
+attn_bwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG,
+                      const __grid_constant__ CUtensorMap tmBias, const __grid_constant__ AttnBwdParams bp) {
+    const int first = bp.q_first ? bp.q_blocks : bp.kv_blocks;
+    const bool second = (int)blockIdx.x >= first;
+    const int block = second ? (int)blockIdx.x - first : (int)blockIdx.x;
+    if (second != (bp.q_first != 0)) attn_dq_block<kD, kBias>(tmQ, tmK, tmV, tmG, tmBias, bp, block);
+    else attn_dkv_block<kD, kBias>(tmQ, tmK, tmV, tmG, tmBias, bp, block);
 }
 
 }  // namespace trimul

@@ -477,18 +477,17 @@ int run_fwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorksp
 }
 
 template <int kD, bool kBias>
-int launch_bwd(const AttnBwdParams& bp, const CUtensorMap (&m)[5], cudaStream_t st) {
-    using KV = AbKvLayout<kD, kBias>;
-    using Q = AbQLayout<kD, kBias>;
-    auto dkv = attn_dkv_sm100_kernel<kD, kBias>;
-    auto dq = attn_dq_sm100_kernel<kD, kBias>;
-    if (!ensure_smem(dkv, KV::kSmem) || !ensure_smem(dq, Q::kSmem)) return TRIMUL_E_CUDA;
+int launch_bwd(AttnBwdParams bp, const CUtensorMap (&m)[5], cudaStream_t st) {
+    constexpr int kSmem = std::max(AbKvLayout<kD, kBias>::kSmem, AbQLayout<kD, kBias>::kSmem);
+    auto kernel = attn_bwd_sm100_kernel<kD, kBias>;
+    if (!ensure_smem(kernel, kSmem)) return TRIMUL_E_CUDA;
     const AttnParams& p = bp.a;
-    const int rc = launch_stage(dkv, dim3((unsigned)bp.n_tiles, (unsigned)p.Hk, (unsigned)p.B), kAbThreads, KV::kSmem, st, true,
-                                m[0], m[1], m[2], m[3], m[4], bp);
-    if (rc != TRIMUL_OK) return rc;
-    return launch_stage(dq, dim3((unsigned)ceil_div(p.Lq, kAfRows), (unsigned)p.H, (unsigned)p.B), kAbThreads, Q::kSmem, st, true,
-                        m[0], m[1], m[2], m[3], m[4], bp);
+    const int64_t nq = ceil_div(p.Lq, kAfRows), kv = (int64_t)bp.n_tiles * p.Hk * p.B, q = nq * p.H * p.B;
+    if (kv + q > INT32_MAX) return TRIMUL_E_UNSUPPORTED;
+    bp.kv_blocks = (int)kv;
+    bp.q_blocks = (int)q;
+    bp.q_first = bp.n_tiles * 3 > nq * (p.H / p.Hk) * 4;       // three products a key tile, four a query tile
+    return launch_stage(kernel, dim3((unsigned)(kv + q)), kAbThreads, kSmem, st, true, m[0], m[1], m[2], m[3], m[4], bp);
 }
 int run_bwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
     trimul_attn_desc copy = *given;
