@@ -369,6 +369,7 @@ template <typename T> int run_plain_fwd(const AttnParams& p, cudaStream_t st) {
 template <typename T> int run_plain_bwd(const AttnParams& p, cudaStream_t st) {
     if (p.D <= 32) return launch_plain_bwd<T, 64, 2>(p, st);
     if (p.D <= 64) return launch_plain_bwd<T, 64, 4>(p, st);
+    if (p.D <= 128) return launch_plain_bwd<T, 32, 8>(p, st);
     return launch_plain_bwd<T, 32, 16>(p, st);
 }
 
