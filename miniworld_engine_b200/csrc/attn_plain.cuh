@@ -322,18 +322,16 @@ struct ApStats {
 };
 
 // ---------------------------------------------------------------------------------------
-// gradient of q, and of the scores where the bias wants one: grid (query tiles, H, B)
+// gradient of q, and of the scores where the bias wants one: a block per query tile, head and batch element
 // ---------------------------------------------------------------------------------------
 template <typename T, int kT, int kC>
-__global__ void __launch_bounds__(kApThreads) attn_plain_dq_kernel(const __grid_constant__ AttnParams p) {
+__device__ __forceinline__ void ap_dq_block(const AttnParams& p, int tile, int h, int b) {
     constexpr int kR = kT / 16;
     extern __shared__ __align__(16) float sm[];
     const int pitch = ap_pitch(p.D), pp = ap_ppitch<kT>();
     float *Q = sm, *G = Q + kT * pitch, *K = G + kT * pitch, *V = K + kT * pitch, *P = V + kT * pitch;
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    const int i0 = blockIdx.x * kT, h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hk);
-    griddep_wait();
-    griddep_launch_dependents();
+    const int i0 = tile * kT, hk = h / (p.H / p.Hk);
     const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
     const T* k = static_cast<const T*>(p.k.p) + b * p.k.b + hk * p.k.h;
     const T* v = static_cast<const T*>(p.v.p) + b * p.v.b + hk * p.v.h;
@@ -397,18 +395,17 @@ __global__ void __launch_bounds__(kApThreads) attn_plain_dq_kernel(const __grid_
 }
 
 // ---------------------------------------------------------------------------------------
-// gradients of k and v: grid (key tiles, Hk, B); the query heads that share the key head are summed here
+// gradients of k and v: a block per key tile, key head and batch element; the query heads that share the key head are
+// summed here
 // ---------------------------------------------------------------------------------------
 template <typename T, int kT, int kC>
-__global__ void __launch_bounds__(kApThreads) attn_plain_dkv_kernel(const __grid_constant__ AttnParams p) {
+__device__ __forceinline__ void ap_dkv_block(const AttnParams& p, int tile, int hk, int b) {
     constexpr int kR = kT / 16;
     extern __shared__ __align__(16) float sm[];
     const int pitch = ap_pitch(p.D), pp = ap_ppitch<kT>();
     float *Q = sm, *G = Q + kT * pitch, *K = G + kT * pitch, *V = K + kT * pitch, *P = V + kT * pitch, *S = P + kT * pp;
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    const int j0 = blockIdx.x * kT, hk = blockIdx.y, b = blockIdx.z, group = p.H / p.Hk;
-    griddep_wait();
-    griddep_launch_dependents();
+    const int j0 = tile * kT, group = p.H / p.Hk;
     const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
     const bool vq = ap_vec<T>(p.q, p.D), vg = ap_vec<T>(p.dout, p.D);
     const int nq = (p.Lq + kT - 1) / kT;
@@ -469,6 +466,27 @@ __global__ void __launch_bounds__(kApThreads) attn_plain_dkv_kernel(const __grid
             at_store(dkp + d, kept ? dk[r][c] * p.scale : 0.f);
             at_store(dvp + d, kept ? dv[r][c] : 0.f);
         }
+    }
+}
+
+// Both kinds of blocks in one grid, the longer kind first: where neither fills the device, they run side by side.
+struct ApBwdGrid {
+    int kv_blocks, q_blocks, kv_tiles, q_tiles, q_first;
+};
+template <typename T, int kT, int kC>
+__global__ void __launch_bounds__(kApThreads)
+attn_plain_bwd_kernel(const __grid_constant__ AttnParams p, const ApBwdGrid g) {
+    const int first = g.q_first ? g.q_blocks : g.kv_blocks;
+    const bool second = (int)blockIdx.x >= first;
+    const int n = second ? (int)blockIdx.x - first : (int)blockIdx.x;
+    griddep_wait();
+    griddep_launch_dependents();
+    if (second != (g.q_first != 0)) {
+        const int head = n / g.q_tiles;
+        ap_dq_block<T, kT, kC>(p, n - head * g.q_tiles, head % p.H, head / p.H);
+    } else {
+        const int head = n / g.kv_tiles;
+        ap_dkv_block<T, kT, kC>(p, n - head * g.kv_tiles, head % p.Hk, head / p.Hk);
     }
 }
 

@@ -353,12 +353,12 @@ template <typename T, int kT, int kC> int launch_plain_fwd(const AttnParams& p, 
     return launch_stage(kernel, dim3((unsigned)ceil_div(p.Lq, kT), p.H, p.B), kApThreads, ap_smem<kT>(p.D, 3, 1), st, true, p);
 }
 template <typename T, int kT, int kC> int launch_plain_bwd(const AttnParams& p, cudaStream_t st) {
-    auto dq = attn_plain_dq_kernel<T, kT, kC>;
-    auto dkv = attn_plain_dkv_kernel<T, kT, kC>;
-    if (!ensure_smem(dq, ap_smem<kT>(16 * kC, 4, 1)) || !ensure_smem(dkv, ap_smem<kT>(16 * kC, 4, 2))) return TRIMUL_E_CUDA;
-    const int rc = launch_stage(dkv, dim3((unsigned)ceil_div(p.Lk, kT), p.Hk, p.B), kApThreads, ap_smem<kT>(p.D, 4, 2), st, true, p);
-    if (rc != TRIMUL_OK) return rc;
-    return launch_stage(dq, dim3((unsigned)ceil_div(p.Lq, kT), p.H, p.B), kApThreads, ap_smem<kT>(p.D, 4, 1), st, true, p);
+    auto kernel = attn_plain_bwd_kernel<T, kT, kC>;
+    if (!ensure_smem(kernel, ap_smem<kT>(16 * kC, 4, 2))) return TRIMUL_E_CUDA;
+    const int64_t nk = ceil_div(p.Lk, kT), nq = ceil_div(p.Lq, kT), kv = nk * p.Hk * p.B, q = nq * p.H * p.B;
+    if (kv + q > INT32_MAX) return TRIMUL_E_UNSUPPORTED;
+    const ApBwdGrid g{(int)kv, (int)q, (int)nk, (int)nq, nk * 3 > nq * (p.H / p.Hk) * 4};   // three products a key tile, four a query tile
+    return launch_stage(kernel, dim3((unsigned)(kv + q)), kApThreads, ap_smem<kT>(p.D, 4, 2), st, true, p, g);
 }
 template <typename T> int run_plain_fwd(const AttnParams& p, cudaStream_t st) {
     if (p.D <= 32) return launch_plain_fwd<T, 64, 2>(p, st);
