@@ -30,8 +30,7 @@ struct AttnBwdParams {
     const uint32_t* words;       // as in the forward kernel
     const int* list;
     int bias_b1, bias_h1;
-    int kv_blocks, q_blocks;     // of the two kinds
-    int q_first;                 // the blocks over the keys come first
+    AttnBwdSplit w;
 };
 
 template <int kD, bool kBias>
@@ -124,6 +123,27 @@ __device__ __forceinline__ void ab_row_out(uint32_t t, __nv_bfloat16* dst, int D
     }
 }
 
+// The same of a part: fp32
+template <int kD>
+__device__ __forceinline__ void ab_part_out(uint32_t t, float* dst, int D, float f, bool write, bool zero) {
+#pragma unroll 1
+    for (int cc = 0; cc < kD; cc += 16) {
+        if (cc >= D) break;
+        uint32_t o[16];
+        tmem_ld_32x16(t + cc, o);
+        tmem_ld_wait();
+        if (!write) continue;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            if (cc + 4 * g >= D) break;
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = zero ? 0.f : __uint_as_float(o[4 * g + e]) * f;
+            *reinterpret_cast<float4*>(dst + cc + 4 * g) = make_float4(y[0], y[1], y[2], y[3]);
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------
 // dk, dv: a block per (key tile, key head, batch element).  Scores transposed: a lane of tensor memory is a key, a column a query.  Masked keys
 // only ever meet their own lanes, so whatever their rows hold stays there, and their results are written as zeros.
@@ -158,7 +178,8 @@ __device__ __forceinline__ void attn_dkv_block(const CUtensorMap& tmQ, const CUt
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = warp_uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int tile = block % bp.n_tiles, j0 = tile * kAfRows, hk = block / bp.n_tiles % p.Hk, b = block / bp.n_tiles / p.Hk;
+    const int tile = block % bp.n_tiles, j0 = tile * kAfRows, hk = block / bp.n_tiles % p.Hk;
+    const int b = block / bp.n_tiles / p.Hk % p.B, split = block / bp.n_tiles / p.Hk / p.B;
     const int group = p.H / p.Hk, nq = (p.Lq + kAfRows - 1) / kAfRows;
 
     if (threadIdx.x == 0) {
@@ -200,9 +221,10 @@ __device__ __forceinline__ void attn_dkv_block(const CUtensorMap& tmQ, const CUt
 
     const uint4 w4 = bp.words != nullptr ? __ldg(reinterpret_cast<const uint4*>(bp.words) + (long long)b * bp.n_tiles + tile)
                                          : make_uint4(~0u, ~0u, ~0u, ~0u);
-    const int n = warp_uniform((w4.x | w4.y | w4.z | w4.w) != 0u ? group * nq : 0);       // query tiles, head after head
-    auto head_of = [&](int it) { return hk * group + it / nq; };
-    auto row_of = [&](int it) { return (it % nq) * kAfRows; };
+    const int first = split * bp.w.kv_share;             // of the query tiles, head after head
+    const int n = warp_uniform((w4.x | w4.y | w4.z | w4.w) != 0u ? max(0, min(bp.w.kv_share, group * nq - first)) : 0);
+    auto head_of = [&](int it) { return hk * group + (first + it) / nq; };
+    auto row_of = [&](int it) { return ((first + it) % nq) * kAfRows; };
 
     if (warp == 0) {
         if (lane == 0 && n > 0) {
@@ -369,9 +391,16 @@ __device__ __forceinline__ void attn_dkv_block(const CUtensorMap& tmQ, const CUt
         if (ok) {
             const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
             const bool zero = n == 0 || ((w[q] >> lane) & 1u) == 0u;
-            const AttnTensor& t = g == 0 ? p.dv : p.dk;
-            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(t.p) + b * t.b + (long long)j * t.l + hk * t.h;
-            ab_row_out<kD>((g == 0 ? tV : tK) + lane_off, dst, p.D, g == 0 ? 1.f : p.scale, j < p.Lk, zero);
+            const uint32_t acc = (g == 0 ? tV : tK) + lane_off;
+            const float f = g == 0 ? 1.f : p.scale;
+            if (bp.w.dk != nullptr) {
+                const long long prow = (((long long)split * p.B + b) * p.Hk + hk) * p.Lk + j;
+                ab_part_out<kD>(acc, (g == 0 ? bp.w.dv : bp.w.dk) + prow * p.D, p.D, f, j < p.Lk, zero);
+            } else {
+                const AttnTensor& t = g == 0 ? p.dv : p.dk;
+                __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(t.p) + b * t.b + (long long)j * t.l + hk * t.h;
+                ab_row_out<kD>(acc, dst, p.D, f, j < p.Lk, zero);
+            }
         }
     }
 
@@ -420,7 +449,8 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
 
     const int warp = warp_uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int nq = (p.Lq + kAfRows - 1) / kAfRows;
-    const int i0 = block % nq * kAfRows, h = block / nq % p.H, b = block / nq / p.H, hk = h / (p.H / p.Hk);
+    const int i0 = block % nq * kAfRows, h = block / nq % p.H, hk = h / (p.H / p.Hk);
+    const int b = block / nq / p.H % p.B, split = block / nq / p.H / p.B;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < 2; ++s) {
@@ -463,8 +493,10 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
     griddep_launch_dependents();
 
     const int* list = bp.list != nullptr ? bp.list + (long long)b * (bp.n_tiles + 1) : nullptr;
-    const int n = warp_uniform(list != nullptr ? list[0] : bp.n_tiles);
-    auto tile_at = [&](int it) { return list != nullptr ? __ldg(list + 1 + it) : it; };
+    // of the listed key tiles a block takes its share
+    const int listed = warp_uniform(list != nullptr ? list[0] : bp.n_tiles), share = (listed + bp.w.q_splits - 1) / bp.w.q_splits;
+    const int first = min(split * share, listed), n = min(share, listed - first);
+    auto tile_at = [&](int it) { return list != nullptr ? __ldg(list + 1 + first + it) : first + it; };
 
     if (warp == 0) {
         if (lane == 0 && n > 0) {
@@ -561,7 +593,7 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
         const float both = -fmaf(ml.x, kLog2e, ml.y);
         __nv_bfloat16* ds = p.ds != nullptr ? static_cast<__nv_bfloat16*>(p.ds) + b * p.ds_b + h * p.ds_h + i * p.ds_i : nullptr;
         bool ok = true;
-        int t_next = 0;              // first key tile whose ds is not written yet
+        int t_next = first > 0 ? tile_at(-1) + 1 : 0;      // first key tile whose ds is not written yet
         auto clear_ds = [&](int t_end) {
             if (ds != nullptr && i < p.Lq)
                 for (int t = t_next; t < t_end; ++t)
@@ -633,12 +665,17 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
                 }
             }
         }
-        if (ok) clear_ds(bp.n_tiles);
+        if (ok && split == bp.w.q_splits - 1) clear_ds(bp.n_tiles);
         if (n > 0 && ok) ok = warp_wait(done, 0, lane, abort_flag, p.status, kStageIdAttnDq, 403);
         tcgen05_fence_after();
         if (ok && g == 0) {
-            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.dq.p) + b * p.dq.b + (long long)i * p.dq.l + h * p.dq.h;
-            ab_row_out<kD>(tQ + lane_off, dst, p.D, p.scale, i < p.Lq, n == 0);
+            if (bp.w.dq != nullptr) {
+                const long long prow = (((long long)split * p.B + b) * p.H + h) * p.Lq + i;
+                ab_part_out<kD>(tQ + lane_off, bp.w.dq + prow * p.D, p.D, p.scale, i < p.Lq, n == 0);
+            } else {
+                __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.dq.p) + b * p.dq.b + (long long)i * p.dq.l + h * p.dq.h;
+                ab_row_out<kD>(tQ + lane_off, dst, p.D, p.scale, i < p.Lq, n == 0);
+            }
         }
     }
 
@@ -659,10 +696,10 @@ __global__ void __launch_bounds__(kAbThreads, 1)
 attn_bwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG,
                       const __grid_constant__ CUtensorMap tmBias, const __grid_constant__ AttnBwdParams bp) {
-    const int first = bp.q_first ? bp.q_blocks : bp.kv_blocks;
+    const int first = bp.w.q_first ? bp.w.q_blocks : bp.w.kv_blocks;
     const bool second = (int)blockIdx.x >= first;
     const int block = second ? (int)blockIdx.x - first : (int)blockIdx.x;
-    if (second != (bp.q_first != 0)) attn_dq_block<kD, kBias>(tmQ, tmK, tmV, tmG, tmBias, bp, block);
+    if (second != (bp.w.q_first != 0)) attn_dq_block<kD, kBias>(tmQ, tmK, tmV, tmG, tmBias, bp, block);
     else attn_dkv_block<kD, kBias>(tmQ, tmK, tmV, tmG, tmBias, bp, block);
 }
 

@@ -36,6 +36,16 @@ struct AttnParams {
     int32_t* status;
 };
 
+// Backward pass: how many blocks share the loop of a tile, and where their parts go ([split][row][D] in fp32, rows as
+// [B][heads][length]; null: the loop is whole and the block writes the result)
+struct AttnBwdSplit {
+    int q_splits, kv_splits;
+    int q_share, kv_share;                 // steps of a block, without masks
+    int q_blocks, kv_blocks;               // with the splits
+    int q_first;                           // the blocks over the keys come first
+    float *dq, *dk, *dv;
+};
+
 __device__ __forceinline__ float at_float(float v) { return v; }
 __device__ __forceinline__ float at_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ void at_store(float* p, float v) { *p = v; }

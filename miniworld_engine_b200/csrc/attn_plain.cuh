@@ -163,13 +163,14 @@ struct ApBias {
 // forward: grid (query tiles, H, B)
 // ---------------------------------------------------------------------------------------
 template <typename T, int kT, int kC>
-__global__ void __launch_bounds__(kApThreads) attn_plain_fwd_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kApThreads) attn_plain_fwd_kernel(const __grid_constant__ AttnParams p, int splits, int share, float* part_o, float2* part_ml) {
     constexpr int kR = kT / 16;
     extern __shared__ __align__(16) float sm[];
     const int pitch = ap_pitch(p.D), pp = ap_ppitch<kT>();
     float *Q = sm, *K = Q + kT * pitch, *V = K + kT * pitch, *P = V + kT * pitch;
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    const int i0 = blockIdx.x * kT, h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hk);
+    const int i0 = blockIdx.x * kT, h = blockIdx.y, b = blockIdx.z / splits, split = blockIdx.z % splits, hk = h / (p.H / p.Hk);
+    const int first = split * share * kT, end = min(p.Lk, first + share * kT);      // keys of this block
     griddep_wait();
     griddep_launch_dependents();
     const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
@@ -179,8 +180,8 @@ __global__ void __launch_bounds__(kApThreads) attn_plain_fwd_kernel(const __grid
     ApTile<T, kT, kC> tk, tv;
     tk.fetch(static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h, p.q.l, i0, p.Lq, p.D, nullptr, ap_vec<T>(p.q, p.D));
     tk.put(Q, p.D);
-    tk.fetch(k, p.k.l, 0, p.Lk, p.D, keep, vk);
-    tv.fetch(v, p.v.l, 0, p.Lk, p.D, keep, vv);
+    tk.fetch(k, p.k.l, first, p.Lk, p.D, keep, vk);
+    tv.fetch(v, p.v.l, first, p.Lk, p.D, keep, vv);
     float o[kR][kC], m[kR], l[kR];
 #pragma unroll
     for (int r = 0; r < kR; ++r) {
@@ -189,14 +190,14 @@ __global__ void __launch_bounds__(kApThreads) attn_plain_fwd_kernel(const __grid
 #pragma unroll
         for (int c = 0; c < kC; ++c) o[r][c] = 0.f;
     }
-    for (int j0 = 0; j0 < p.Lk; j0 += kT) {
+    for (int j0 = first; j0 < end; j0 += kT) {
         __syncthreads();
         tk.put(K, p.D);
         tv.put(V, p.D);
         __syncthreads();
         ApBias<T, kR> bias;
         bias.fetch(p, b, h, i0, j0, ty, tx);
-        if (j0 + kT < p.Lk) {
+        if (j0 + kT < end) {
             tk.fetch(k, p.k.l, j0 + kT, p.Lk, p.D, keep, vk);
             tv.fetch(v, p.v.l, j0 + kT, p.Lk, p.D, keep, vv);
         }
@@ -230,6 +231,14 @@ __global__ void __launch_bounds__(kApThreads) attn_plain_fwd_kernel(const __grid
     for (int r = 0; r < kR; ++r) {
         const int i = i0 + ty * kR + r;
         if (i >= p.Lq) continue;
+        if (part_o != nullptr) {             // not yet divided: attn_combine_kernel joins the parts
+            const long long row = (((long long)split * p.B + b) * p.H + h) * p.Lq + i;
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+                if (tx + 16 * c < p.D) part_o[row * p.D + tx + 16 * c] = o[r][c];
+            if (tx == 0) part_ml[row] = make_float2(m[r], l[r]);
+            continue;
+        }
         const bool empty = m[r] == -INFINITY;
         const float inv = empty ? 0.f : 1.f / l[r];
         T* dst = static_cast<T*>(p.o.p) + b * p.o.b + (long long)i * p.o.l + h * p.o.h;
@@ -325,13 +334,14 @@ struct ApStats {
 // gradient of q, and of the scores where the bias wants one: a block per query tile, head and batch element
 // ---------------------------------------------------------------------------------------
 template <typename T, int kT, int kC>
-__device__ __forceinline__ void ap_dq_block(const AttnParams& p, int tile, int h, int b) {
+__device__ __forceinline__ void ap_dq_block(const AttnParams& p, const AttnBwdSplit& w, int tile, int h, int b, int split) {
     constexpr int kR = kT / 16;
     extern __shared__ __align__(16) float sm[];
     const int pitch = ap_pitch(p.D), pp = ap_ppitch<kT>();
     float *Q = sm, *G = Q + kT * pitch, *K = G + kT * pitch, *V = K + kT * pitch, *P = V + kT * pitch;
     const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
     const int i0 = tile * kT, hk = h / (p.H / p.Hk);
+    const int first = split * w.q_share * kT, end = min(p.Lk, first + w.q_share * kT);      // keys of this block
     const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
     const T* k = static_cast<const T*>(p.k.p) + b * p.k.b + hk * p.k.h;
     const T* v = static_cast<const T*>(p.v.p) + b * p.v.b + hk * p.v.h;
@@ -341,8 +351,8 @@ __device__ __forceinline__ void ap_dq_block(const AttnParams& p, int tile, int h
     tv.fetch(static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h, p.dout.l, i0, p.Lq, p.D, nullptr, ap_vec<T>(p.dout, p.D));
     tk.put(Q, p.D);
     tv.put(G, p.D);
-    tk.fetch(k, p.k.l, 0, p.Lk, p.D, keep, vk);
-    tv.fetch(v, p.v.l, 0, p.Lk, p.D, keep, vv);
+    tk.fetch(k, p.k.l, first, p.Lk, p.D, keep, vk);
+    tv.fetch(v, p.v.l, first, p.Lk, p.D, keep, vv);
     ApStats<kR> st;
     st.fetch(p, b, h, i0, ty);
     float o[kR][kC];
@@ -350,14 +360,14 @@ __device__ __forceinline__ void ap_dq_block(const AttnParams& p, int tile, int h
     for (int r = 0; r < kR; ++r)
 #pragma unroll
         for (int c = 0; c < kC; ++c) o[r][c] = 0.f;
-    for (int j0 = 0; j0 < p.Lk; j0 += kT) {
+    for (int j0 = first; j0 < end; j0 += kT) {
         __syncthreads();
         tk.put(K, p.D);
         tv.put(V, p.D);
         __syncthreads();
         ApBias<T, kR> bias;
         bias.fetch(p, b, h, i0, j0, ty, tx);
-        if (j0 + kT < p.Lk) {
+        if (j0 + kT < end) {
             tk.fetch(k, p.k.l, j0 + kT, p.Lk, p.D, keep, vk);
             tv.fetch(v, p.v.l, j0 + kT, p.Lk, p.D, keep, vv);
         }
@@ -384,6 +394,13 @@ __device__ __forceinline__ void ap_dq_block(const AttnParams& p, int tile, int h
     for (int r = 0; r < kR; ++r) {
         const int i = i0 + ty * kR + r;
         if (i >= p.Lq) continue;
+        if (w.dq != nullptr) {
+            float* part = w.dq + ((((long long)split * p.B + b) * p.H + h) * p.Lq + i) * p.D;
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+                if (tx + 16 * c < p.D) part[tx + 16 * c] = o[r][c] * p.scale;
+            continue;
+        }
         T* dst = static_cast<T*>(p.dq.p) + b * p.dq.b + (long long)i * p.dq.l + h * p.dq.h;
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
@@ -399,7 +416,7 @@ __device__ __forceinline__ void ap_dq_block(const AttnParams& p, int tile, int h
 // summed here
 // ---------------------------------------------------------------------------------------
 template <typename T, int kT, int kC>
-__device__ __forceinline__ void ap_dkv_block(const AttnParams& p, int tile, int hk, int b) {
+__device__ __forceinline__ void ap_dkv_block(const AttnParams& p, const AttnBwdSplit& w, int tile, int hk, int b, int split) {
     constexpr int kR = kT / 16;
     extern __shared__ __align__(16) float sm[];
     const int pitch = ap_pitch(p.D), pp = ap_ppitch<kT>();
@@ -409,6 +426,7 @@ __device__ __forceinline__ void ap_dkv_block(const AttnParams& p, int tile, int 
     const uint8_t* keep = p.mask != nullptr ? p.mask + b * p.mask_b : nullptr;
     const bool vq = ap_vec<T>(p.q, p.D), vg = ap_vec<T>(p.dout, p.D);
     const int nq = (p.Lq + kT - 1) / kT;
+    const int first = split * w.kv_share, end = min(group * nq, first + w.kv_share);        // query tiles, head after head
     ApTile<T, kT, kC> tq, tg;
     tq.fetch(static_cast<const T*>(p.k.p) + b * p.k.b + hk * p.k.h, p.k.l, j0, p.Lk, p.D, keep, ap_vec<T>(p.k, p.D));
     tg.fetch(static_cast<const T*>(p.v.p) + b * p.v.b + hk * p.v.h, p.v.l, j0, p.Lk, p.D, keep, ap_vec<T>(p.v, p.D));
@@ -419,13 +437,13 @@ __device__ __forceinline__ void ap_dkv_block(const AttnParams& p, int tile, int 
         tq.fetch(static_cast<const T*>(p.q.p) + b * p.q.b + h * p.q.h, p.q.l, i0, p.Lq, p.D, nullptr, vq);
         tg.fetch(static_cast<const T*>(p.dout.p) + b * p.dout.b + h * p.dout.h, p.dout.l, i0, p.Lq, p.D, nullptr, vg);
     };
-    fetch(0);
+    fetch(first);
     float dk[kR][kC], dv[kR][kC];
 #pragma unroll
     for (int r = 0; r < kR; ++r)
 #pragma unroll
         for (int c = 0; c < kC; ++c) dk[r][c] = dv[r][c] = 0.f;
-    for (int it = 0; it < group * nq; ++it) {
+    for (int it = first; it < end; ++it) {
         const int h = hk * group + it / nq, i0 = it % nq * kT;
         __syncthreads();
         tq.put(Q, p.D);
@@ -435,7 +453,7 @@ __device__ __forceinline__ void ap_dkv_block(const AttnParams& p, int tile, int 
         bias.fetch(p, b, h, i0, j0, ty, tx);
         ApStats<kR> st;
         st.fetch(p, b, h, i0, ty);
-        if (it + 1 < group * nq) fetch(it + 1);
+        if (it + 1 < end) fetch(it + 1);
         float s[kR][kR], g[kR][kR];
         ap_dot<kR>(s, Q, K, p.D, ty, tx);
         ap_dot<kR>(g, G, V, p.D, ty, tx);
@@ -457,6 +475,17 @@ __device__ __forceinline__ void ap_dkv_block(const AttnParams& p, int tile, int 
         const int j = j0 + ty * kR + r;
         if (j >= p.Lk) continue;
         const bool kept = keep == nullptr || keep[j] != 0;     // zero whatever the upstream gradient holds
+        if (w.dk != nullptr) {
+            const long long row = ((((long long)split * p.B + b) * p.Hk + hk) * p.Lk + j) * p.D;
+#pragma unroll
+            for (int c = 0; c < kC; ++c) {
+                const int d = tx + 16 * c;
+                if (d >= p.D) break;
+                w.dk[row + d] = kept ? dk[r][c] * p.scale : 0.f;
+                w.dv[row + d] = kept ? dv[r][c] : 0.f;
+            }
+            continue;
+        }
         T* dkp = static_cast<T*>(p.dk.p) + b * p.dk.b + (long long)j * p.dk.l + hk * p.dk.h;
         T* dvp = static_cast<T*>(p.dv.p) + b * p.dv.b + (long long)j * p.dv.l + hk * p.dv.h;
 #pragma unroll
@@ -470,23 +499,34 @@ __device__ __forceinline__ void ap_dkv_block(const AttnParams& p, int tile, int 
 }
 
 // Both kinds of blocks in one grid, the longer kind first: where neither fills the device, they run side by side.
-struct ApBwdGrid {
-    int kv_blocks, q_blocks, kv_tiles, q_tiles, q_first;
-};
 template <typename T, int kT, int kC>
 __global__ void __launch_bounds__(kApThreads)
-attn_plain_bwd_kernel(const __grid_constant__ AttnParams p, const ApBwdGrid g) {
-    const int first = g.q_first ? g.q_blocks : g.kv_blocks;
-    const bool second = (int)blockIdx.x >= first;
+attn_plain_bwd_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ AttnBwdSplit w) {
+    const int first = w.q_first ? w.q_blocks : w.kv_blocks;
+    const bool second = (int)blockIdx.x >= first, over_keys = second != (w.q_first != 0);
     const int n = second ? (int)blockIdx.x - first : (int)blockIdx.x;
+    const int tiles = ((over_keys ? p.Lq : p.Lk) + kT - 1) / kT, heads = over_keys ? p.H : p.Hk;
+    const int tile = n % tiles, h = n / tiles % heads, b = n / tiles / heads % p.B, split = n / tiles / heads / p.B;
     griddep_wait();
     griddep_launch_dependents();
-    if (second != (g.q_first != 0)) {
-        const int head = n / g.q_tiles;
-        ap_dq_block<T, kT, kC>(p, n - head * g.q_tiles, head % p.H, head / p.H);
-    } else {
-        const int head = n / g.kv_tiles;
-        ap_dkv_block<T, kT, kC>(p, n - head * g.kv_tiles, head % p.Hk, head / p.Hk);
+    if (over_keys) ap_dq_block<T, kT, kC>(p, w, tile, h, b, split);
+    else ap_dkv_block<T, kT, kC>(p, w, tile, h, b, split);
+}
+
+// The parts of a gradient added up, in order: a thread per element; blockIdx.y: which of two tensors of one shape
+template <typename T>
+__global__ void __launch_bounds__(kApThreads)
+attn_join_kernel(const float* part0, const float* part1, AttnTensor t0, AttnTensor t1, int splits, int L, int heads, int D, long long n) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const float* part = blockIdx.y ? part1 : part0;
+    const AttnTensor& t = blockIdx.y ? t1 : t0;
+    for (long long e = (long long)blockIdx.x * kApThreads + threadIdx.x; e < n; e += (long long)gridDim.x * kApThreads) {
+        float y = 0.f;
+#pragma unroll 8
+        for (int s = 0; s < splits; ++s) y += part[s * n + e];
+        const long long row = e / D, bh = row / L;
+        at_store(static_cast<T*>(t.p) + bh / heads * t.b + (row - bh * L) * t.l + bh % heads * t.h + (e - row * D), y);
     }
 }
 

@@ -306,11 +306,51 @@ int forward_splits(const trimul_attn_desc* d) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(room, tiles / 4));
 }
 
+// The CUDA-core kernels: rows of a tile, and key splits of the forward pass as above, up to three blocks for two SMs (a step takes
+// long enough that one less pays for joining: 2 x 60 queries of 96, 1000 keys 188 -> 23 us, 2 x 256 of 32, 320 keys 27 -> 21).
+int plain_rows(const trimul_attn_desc* d, bool backward) { return d->D <= (backward ? 64 : 128) ? 64 : 32; }
+int plain_splits(const trimul_attn_desc* d) {
+    const int rows = plain_rows(d, false);
+    const int64_t blocks = ceil_div(d->Lq, rows) * d->H * d->B, tiles = ceil_div(d->Lk, rows);
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(sm_count() * 3 / 2 / blocks, tiles));
+    return (int)ceil_div(tiles, ceil_div(tiles, splits));
+}
+
+// Backward pass: a block's loop is split among several, whose parts a second kernel adds up, where it is twice as long as a
+// block slot's share of all steps: few queries against many keys leave dq to a few long loops, many queries against few keys dk and dv.
+// Tensor cores, 8 heads, us whole / split: 61 x 4096 of 64 41 / 20, of 128 46 / 29, 100 x 1024 of 64 13.8 / 10.8, 2048 x 100 of
+// 128 37 / 22; a loop just over twice the share (700 x 1400, 4 heads of 128) 21.6 / 24.2, hence `margin`; shares of four steps at
+// least instead of two 100 x 1024 12.2, 2048 x 100 25.1.  CUDA cores, where a step takes longer and two blocks fit on an SM: 2 x
+// 60 x 1000, 4 heads of 96 208 / 75, 500 x 60, 4 heads of 64 128 / 25, 188 x 169, 8 heads of 128 69 / 59.
+AttnBwdSplit backward_split(const trimul_attn_desc* d, int rows, int least, int margin, int slots) {
+    const int64_t nq = ceil_div(d->Lq, rows), nk = ceil_div(d->Lk, rows), q = nq * d->H * d->B, kv = nk * d->Hk * d->B;
+    const int64_t kv_loop = nq * (d->H / d->Hk), share = std::max<int64_t>(least, ceil_div(q * nk + kv * kv_loop, slots));
+    auto split = [&](int64_t loop) { return loop >= 2 * share + margin ? ceil_div(loop, ceil_div(loop, loop / share)) : 1; };
+    AttnBwdSplit w = {};
+    w.q_splits = (int)split(nk);
+    w.kv_splits = (int)split(kv_loop);
+    w.q_share = (int)ceil_div(nk, w.q_splits);
+    w.kv_share = (int)ceil_div(kv_loop, w.kv_splits);
+    const int64_t q_blocks = q * w.q_splits, kv_blocks = kv * w.kv_splits;
+    const bool fits = q_blocks + kv_blocks <= INT32_MAX;          // one grid; 0 blocks: too many
+    w.q_blocks = fits ? (int)q_blocks : 0;
+    w.kv_blocks = fits ? (int)kv_blocks : 0;
+    w.q_first = w.q_share * 3LL > w.kv_share * 4LL;                // three products a key tile, four a query tile
+    return w;
+}
+AttnBwdSplit backward_split(const trimul_attn_desc* d, bool tensor) {
+    return tensor ? backward_split(d, kAfRows, 2, 4, sm_count()) : backward_split(d, plain_rows(d, true), 1, 0, 2 * sm_count());
+}
+int64_t part_bytes(const trimul_attn_desc* d, const AttnBwdSplit& w, bool q) {
+    if ((q ? w.q_splits : w.kv_splits) == 1) return 0;
+    return align_up((q ? (int64_t)w.q_splits * d->H * d->Lq : (int64_t)w.kv_splits * d->Hk * d->Lk) * d->B * d->D * 4, 256);
+}
+
 // Workspace.  Both directions: the key mask as bits and its list of tiles.  Forward: the parts of split rows.  Backward:
 // delta, then the scores' gradients where the bias's gradient sums them.  Depends on sizes, type, flags, the shape of the bias and
 // on whether there are a mask and a gradient of the bias, not on addresses or strides.
 struct AttnWorkspace {
-    int64_t words, list, bias, part_o, part_ml, delta, ds, ds_pitch, total;
+    int64_t words, list, bias, part_o, part_ml, delta, dq, dk, dv, ds, ds_pitch, total;
 };
 AttnWorkspace attn_workspace(const trimul_attn_desc* d, bool backward) {
     AttnWorkspace w = {};
@@ -328,7 +368,7 @@ AttnWorkspace attn_workspace(const trimul_attn_desc* d, bool backward) {
         at += align_up((int64_t)d->bias_batch * d->bias_heads * d->Lq * align_up(d->Lk, 8) * 2, 256);
     }
     // by sizes alone, so that a caller may keep the answer: room for either kernel's parts
-    const int splits = backward ? 1 : std::max(short_sizes(d) ? short_splits(d) : 1, tc ? forward_splits(d) : 1);
+    const int splits = backward ? 1 : std::max({short_sizes(d) ? short_splits(d) : 1, tc ? forward_splits(d) : 1, plain_splits(d)});
     if (splits > 1) {
         const int64_t rows = (int64_t)splits * d->B * d->H * d->Lq;
         w.part_o = at;
@@ -339,6 +379,17 @@ AttnWorkspace attn_workspace(const trimul_attn_desc* d, bool backward) {
     if (backward) {
         w.delta = at;
         at += align_up((int64_t)d->B * d->H * d->Lq * 4, 256);
+        int64_t q = 0, kv = 0;
+        for (bool tensor : {false, true})
+            if (!tensor || tc) {
+                const AttnBwdSplit split = backward_split(d, tensor);
+                q = std::max(q, part_bytes(d, split, true));
+                kv = std::max(kv, part_bytes(d, split, false));
+            }
+        w.dq = at;
+        w.dk = w.dq + q;
+        w.dv = w.dk + kv;
+        at = w.dv + kv;
         w.ds = at;
         w.ds_pitch = align_up(d->Lk, 16 / elem_size(d->dtype));
         if (sums_bias(d)) at += align_up((int64_t)d->B * d->H * d->Lq * w.ds_pitch * elem_size(d->dtype), 256);
@@ -347,41 +398,56 @@ AttnWorkspace attn_workspace(const trimul_attn_desc* d, bool backward) {
     return w;
 }
 
-template <typename T, int kT, int kC> int launch_plain_fwd(const AttnParams& p, cudaStream_t st) {
+template <typename T>
+int run_combine(const AttnParams& p, const float* part_o, const float2* part_ml, int splits, cudaStream_t st) {
+    const int64_t rows = (int64_t)p.B * p.H * p.Lq;
+    return launch_stage(attn_combine_kernel<T>, dim3((unsigned)ceil_div(rows, 8)), 256, 0, st, true, p, part_o, part_ml, splits);
+}
+
+template <typename T, int kT, int kC>
+int launch_plain_fwd(const AttnParams& p, int splits, float* part_o, float2* part_ml, cudaStream_t st) {
     auto kernel = attn_plain_fwd_kernel<T, kT, kC>;
     if (!ensure_smem(kernel, ap_smem<kT>(16 * kC, 3, 1))) return TRIMUL_E_CUDA;
-    return launch_stage(kernel, dim3((unsigned)ceil_div(p.Lq, kT), p.H, p.B), kApThreads, ap_smem<kT>(p.D, 3, 1), st, true, p);
+    const int rc = launch_stage(kernel, dim3((unsigned)ceil_div(p.Lq, kT), p.H, p.B * splits), kApThreads, ap_smem<kT>(p.D, 3, 1), st, true,
+                                p, splits, (int)ceil_div(ceil_div(p.Lk, kT), splits), part_o, part_ml);
+    return rc != TRIMUL_OK || splits == 1 ? rc : run_combine<T>(p, part_o, part_ml, splits, st);
 }
-template <typename T, int kT, int kC> int launch_plain_bwd(const AttnParams& p, cudaStream_t st) {
+template <typename T, int kT, int kC> int launch_plain_bwd(const AttnParams& p, const AttnBwdSplit& w, cudaStream_t st) {
     auto kernel = attn_plain_bwd_kernel<T, kT, kC>;
     if (!ensure_smem(kernel, ap_smem<kT>(16 * kC, 4, 2))) return TRIMUL_E_CUDA;
-    const int64_t nk = ceil_div(p.Lk, kT), nq = ceil_div(p.Lq, kT), kv = nk * p.Hk * p.B, q = nq * p.H * p.B;
-    if (kv + q > INT32_MAX) return TRIMUL_E_UNSUPPORTED;
-    const ApBwdGrid g{(int)kv, (int)q, (int)nk, (int)nq, nk * 3 > nq * (p.H / p.Hk) * 4};   // three products a key tile, four a query tile
-    return launch_stage(kernel, dim3((unsigned)(kv + q)), kApThreads, ap_smem<kT>(p.D, 4, 2), st, true, p, g);
+    return launch_stage(kernel, dim3((unsigned)(w.kv_blocks + w.q_blocks)), kApThreads, ap_smem<kT>(p.D, 4, 2), st, true, p, w);
 }
-template <typename T> int run_plain_fwd(const AttnParams& p, cudaStream_t st) {
-    if (p.D <= 32) return launch_plain_fwd<T, 64, 2>(p, st);
-    if (p.D <= 64) return launch_plain_fwd<T, 64, 4>(p, st);
-    if (p.D <= 128) return launch_plain_fwd<T, 64, 8>(p, st);
-    return launch_plain_fwd<T, 32, 16>(p, st);
+template <typename T> int run_plain_fwd(const trimul_attn_desc* d, const AttnParams& p, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
+    const int splits = plain_splits(d);
+    float* o = splits > 1 ? reinterpret_cast<float*>(ws + w.part_o) : nullptr;
+    float2* ml = reinterpret_cast<float2*>(ws + w.part_ml);
+    if (p.D <= 32) return launch_plain_fwd<T, 64, 2>(p, splits, o, ml, st);
+    if (p.D <= 64) return launch_plain_fwd<T, 64, 4>(p, splits, o, ml, st);
+    if (p.D <= 128) return launch_plain_fwd<T, 64, 8>(p, splits, o, ml, st);
+    return launch_plain_fwd<T, 32, 16>(p, splits, o, ml, st);
 }
-template <typename T> int run_plain_bwd(const AttnParams& p, cudaStream_t st) {
-    if (p.D <= 32) return launch_plain_bwd<T, 64, 2>(p, st);
-    if (p.D <= 64) return launch_plain_bwd<T, 64, 4>(p, st);
-    if (p.D <= 128) return launch_plain_bwd<T, 32, 8>(p, st);
-    return launch_plain_bwd<T, 32, 16>(p, st);
+template <typename T> int run_plain_bwd(const AttnParams& p, const AttnBwdSplit& w, cudaStream_t st) {
+    if (p.D <= 32) return launch_plain_bwd<T, 64, 2>(p, w, st);
+    if (p.D <= 64) return launch_plain_bwd<T, 64, 4>(p, w, st);
+    if (p.D <= 128) return launch_plain_bwd<T, 32, 8>(p, w, st);
+    return launch_plain_bwd<T, 32, 16>(p, w, st);
+}
+// The split loops' parts to their results
+template <typename T> int run_join(const AttnParams& p, const AttnBwdSplit& w, cudaStream_t st) {
+    auto join = [&](const float* a, const float* b, const AttnTensor& ta, const AttnTensor& tb, int splits, int L, int heads) {
+        const int64_t n = (int64_t)p.B * heads * L * p.D;
+        const dim3 grid((unsigned)std::min<int64_t>(ceil_div(n, kApThreads), 16 * (int64_t)sm_count()), b != nullptr ? 2 : 1);
+        return launch_stage(attn_join_kernel<T>, grid, kApThreads, 0, st, true, a, b, ta, tb, splits, L, heads, p.D, (long long)n);
+    };
+    int rc = TRIMUL_OK;
+    if (w.dq != nullptr) rc = join(w.dq, nullptr, p.dq, p.dq, w.q_splits, p.Lq, p.H);
+    if (rc == TRIMUL_OK && w.dk != nullptr) rc = join(w.dk, w.dv, p.dk, p.dv, w.kv_splits, p.Lk, p.Hk);
+    return rc;
 }
 
 int run_mask(const trimul_attn_desc* d, uint32_t* words, int* list, cudaStream_t st) {
     return launch_stage(attn_mask_kernel, dim3((unsigned)d->B), kMaskPrepThreads, 0, st, true, d->mask, (long long)d->mask_b, d->Lk,
                         (int)ceil_div(d->Lk, kAfRows), words, list);
-}
-
-template <typename T>
-int run_combine(const AttnParams& p, const float* part_o, const float2* part_ml, int splits, cudaStream_t st) {
-    const int64_t rows = (int64_t)p.B * p.H * p.Lq;
-    return launch_stage(attn_combine_kernel<T>, dim3((unsigned)ceil_div(rows, 8)), 256, 0, st, true, p, part_o, part_ml, splits);
 }
 
 template <typename T, int kLanes>
@@ -478,25 +544,22 @@ int run_fwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorksp
 }
 
 template <int kD, bool kBias>
-int launch_bwd(AttnBwdParams bp, const CUtensorMap (&m)[5], cudaStream_t st) {
+int launch_bwd(const AttnBwdParams& bp, const CUtensorMap (&m)[5], cudaStream_t st) {
     constexpr int kSmem = std::max(AbKvLayout<kD, kBias>::kSmem, AbQLayout<kD, kBias>::kSmem);
     auto kernel = attn_bwd_sm100_kernel<kD, kBias>;
     if (!ensure_smem(kernel, kSmem)) return TRIMUL_E_CUDA;
-    const AttnParams& p = bp.a;
-    const int64_t nq = ceil_div(p.Lq, kAfRows), kv = (int64_t)bp.n_tiles * p.Hk * p.B, q = nq * p.H * p.B;
-    if (kv + q > INT32_MAX) return TRIMUL_E_UNSUPPORTED;
-    bp.kv_blocks = (int)kv;
-    bp.q_blocks = (int)q;
-    bp.q_first = bp.n_tiles * 3 > nq * (p.H / p.Hk) * 4;       // three products a key tile, four a query tile
-    return launch_stage(kernel, dim3((unsigned)(kv + q)), kAbThreads, kSmem, st, true, m[0], m[1], m[2], m[3], m[4], bp);
+    const dim3 grid((unsigned)(bp.w.kv_blocks + bp.w.q_blocks));
+    return launch_stage(kernel, grid, kAbThreads, kSmem, st, true, m[0], m[1], m[2], m[3], m[4], bp);
 }
-int run_bwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
+int run_bwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorkspace& w, const AttnBwdSplit& split, uint8_t* ws,
+            cudaStream_t st) {
     trimul_attn_desc copy = *given;
     const trimul_attn_desc* d = &copy;
     int rc = run_bias_rows(&copy, w, ws, st);
     if (rc != TRIMUL_OK) return rc;
     AttnBwdParams bp = {};
     bp.a = p;
+    bp.w = split;
     bp.n_tiles = (int)ceil_div(d->Lk, kAfRows);
     bp.bias_b1 = d->bias_batch == 1;
     bp.bias_h1 = d->bias_heads == 1;
@@ -593,7 +656,8 @@ int trimul_b200_attn_forward(const trimul_attn_desc* d, void* workspace, size_t 
         return d->dtype == TRIMUL_DTYPE_BF16 ? run_short<__nv_bfloat16>(d, p, w, static_cast<uint8_t*>(workspace), st)
                                              : run_short<float>(d, p, w, static_cast<uint8_t*>(workspace), st);
     if (tensor_core_forward(d)) return run_fwd(d, p, w, static_cast<uint8_t*>(workspace), st);
-    return d->dtype == TRIMUL_DTYPE_BF16 ? run_plain_fwd<__nv_bfloat16>(p, st) : run_plain_fwd<float>(p, st);
+    return d->dtype == TRIMUL_DTYPE_BF16 ? run_plain_fwd<__nv_bfloat16>(d, p, w, static_cast<uint8_t*>(workspace), st)
+                                         : run_plain_fwd<float>(d, p, w, static_cast<uint8_t*>(workspace), st);
 }
 
 int trimul_b200_attn_backward(const trimul_attn_desc* d, void* workspace, size_t workspace_bytes, void* stream,
@@ -626,8 +690,17 @@ int trimul_b200_attn_backward(const trimul_attn_desc* d, void* workspace, size_t
                       : (lanes == 16 ? attn_delta_kernel<float, 16> : attn_delta_kernel<float, 32>);
     rc = launch_stage(delta, grid, kApThreads, 0, st, true, p);
     if (rc != TRIMUL_OK) return rc;
-    if (tensor_core_backward(d)) rc = run_bwd(d, p, w, ws, st);
-    else rc = bf16 ? run_plain_bwd<__nv_bfloat16>(p, st) : run_plain_bwd<float>(p, st);
+    const bool tensor = tensor_core_backward(d);
+    AttnBwdSplit split = backward_split(d, tensor);
+    if (split.q_blocks == 0) return TRIMUL_E_UNSUPPORTED;
+    if (split.q_splits > 1) split.dq = reinterpret_cast<float*>(ws + w.dq);
+    if (split.kv_splits > 1) {
+        split.dk = reinterpret_cast<float*>(ws + w.dk);
+        split.dv = reinterpret_cast<float*>(ws + w.dv);
+    }
+    if (tensor) rc = run_bwd(d, p, w, split, ws, st);
+    else rc = bf16 ? run_plain_bwd<__nv_bfloat16>(p, split, st) : run_plain_bwd<float>(p, split, st);
+    if (rc == TRIMUL_OK) rc = bf16 ? run_join<__nv_bfloat16>(p, split, st) : run_join<float>(p, split, st);
     if (rc != TRIMUL_OK || !sums_bias(d)) return rc;
     const int n = 16 / elem_size(d->dtype);
     const int64_t items = (int64_t)d->bias_batch * d->bias_heads * d->Lq * ceil_div(d->Lk, n);

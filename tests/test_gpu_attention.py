@@ -325,3 +325,27 @@ def test_first_calls_inside_a_capture_and_backward_twice():
     cross_attention_b200(*once[:3], bias=once[3], key_mask=m).backward(g.float())
     for a, c in zip(leaves, once):
         assert torch.equal(a.grad, 2 * c.grad)
+
+
+@pytest.mark.parametrize("dtype,plain", [(BF16, False), (BF16, True), (FP32, False)])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hk,D,bias", [
+    (1, 61, 2100, 2, 2, 64, "1H"),
+    (1, 2100, 61, 4, 2, 128, None),
+    (2, 40, 1500, 2, 1, 96, "BH"),
+    (1, 900, 10, 2, 2, 32, "11"),
+    (1, 1030, 1700, 1, 1, 40, "BH"),
+    (2, 9, 700, 1, 1, 136, "1H"),
+])
+def test_loops_that_several_blocks_share(B, Lq, Lk, H, Hk, D, bias, dtype, plain):
+    """Few tiles on one side and many on the other; masks that leave some blocks' shares without a key."""
+    q, k, v, g, b, _ = _inputs(B, Lq, Lk, H, Hk, D, bias, None, dtype, seed=Lk)
+    _check_all(q, k, v, g, b, None, plain_kernels=plain)
+    mask = torch.zeros(B, Lk, dtype=torch.bool, device="cuda")
+    mask[:, Lk // 2:Lk // 2 + 3] = True
+    mask[0, -1] = True
+    first = _check_all(q, k, v, g, b, mask, plain_kernels=plain)
+    again, _ = _both(q, k, v, g, b, mask, plain_kernels=plain)
+    for name in first:
+        assert torch.equal(first[name], again[name]), name
+    mask[-1] = False
+    _check_all(q, k, v, g, b, mask, plain_kernels=plain)
