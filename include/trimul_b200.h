@@ -424,7 +424,7 @@ typedef struct trimul_attn_desc {
     int32_t  bias_batch, bias_heads;      /* 1 (serves all), or B / H                                 */
     const uint8_t* mask;                  /* NULL or [B, Lk] bytes, mask_b apart; 0 = masked          */
     int64_t  mask_b;
-    float*   stats;                       /* [B, H, Lq, 2]: row maximum and log2 of the row's sum;
+    float*   stats;                       /* [B, H, Lq, 2], on 8 bytes: row maximum and log2 of the sum;
                                              forward: may be NULL; backward: what forward wrote       */
     void*    o_lo;                        /* bf16 only, [B, Lq, H, D] dense: the rounding of o; may be
                                              NULL in forward; backward: what forward wrote, or NULL   */

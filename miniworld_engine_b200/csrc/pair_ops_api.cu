@@ -200,6 +200,7 @@ int check_attn(const trimul_attn_desc* d) {
     if (d->B <= 0 || d->Lq <= 0 || d->Lk <= 0 || d->H <= 0 || d->Hk <= 0 || d->D <= 0) return TRIMUL_E_INVALID;
     if ((d->H % d->Hk) != 0) return TRIMUL_E_INVALID;
     if (d->D > 256 || d->B > 65535 || d->H > 65535) return TRIMUL_E_UNSUPPORTED;
+    if (!aligned(d->stats, 8)) return TRIMUL_E_INVALID;         // read and written as pairs
     if (d->Lq > (1 << 24) || d->Lk > (1 << 24)) return TRIMUL_E_UNSUPPORTED;
     if ((d->bias != nullptr || d->dbias != nullptr) &&
         ((d->bias_batch != 1 && d->bias_batch != d->B) || (d->bias_heads != 1 && d->bias_heads != d->H)))

@@ -201,3 +201,17 @@ def test_c_abi_checks_attention(lib):
     d.stats = 4096
     assert need(d) == 0
     assert lib.trimul_b200_attn_backward(C.byref(d), 4096, n.value - 1, None, None) == _lib.E_WORKSPACE
+
+
+def test_c_abi_wants_the_statistics_on_eight_bytes(lib):
+    d = _lib.AttnDesc()
+    d.struct_bytes, d.dtype, d.scale = C.sizeof(_lib.AttnDesc), 0, 1.0
+    d.B, d.Lq, d.Lk, d.H, d.Hk, d.D = 1, 4, 4, 1, 1, 8
+    for t in ("q", "k", "v", "o", "dout", "dq", "dk", "dv"):
+        getattr(d, t).p = 4096
+    n = C.c_size_t()
+    for stats, rc in ((4096, 0), (4100, _lib.E_INVALID)):
+        d.stats = stats
+        assert lib.trimul_b200_attn_workspace_bytes(C.byref(d), 1, C.byref(n)) == rc
+    assert lib.trimul_b200_attn_forward(C.byref(d), 4096, 1 << 20, None, None) == _lib.E_INVALID
+    assert lib.trimul_b200_attn_backward(C.byref(d), 4096, 1 << 20, None, None) == _lib.E_INVALID
