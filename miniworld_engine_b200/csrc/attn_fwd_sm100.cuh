@@ -58,72 +58,6 @@ struct AttnFwdParams {
     int bias_b1, bias_h1;        // bias shared along the batch / the heads
 };
 
-// A bias whose rows do not start on 16 bytes, as rows that do: two neighbouring values a thread, so that a warp reads and
-// writes 128 bytes in a row.
-__global__ void __launch_bounds__(256)
-attn_bias_rows_kernel(const __nv_bfloat16* src, long long src_b, long long src_h, long long src_i, uint32_t* dst, int H, int Lq, int Lk,
-                      long long rows, int pitch) {
-    constexpr int kU = 4;
-    griddep_wait();
-    griddep_launch_dependents();
-    const int words = pitch / 2;
-    for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (long long)gridDim.x * 8) {
-        const int i = (int)(r % Lq);
-        const long long bh = r / Lq;
-        const __nv_bfloat16* s = src + bh / H * src_b + bh % H * src_h + i * src_i;
-        for (int w0 = threadIdx.x & 31; w0 < words; w0 += 32 * kU) {
-            __nv_bfloat162 v[kU];
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int j = 2 * (w0 + 32 * u);
-                v[u].x = j < Lk ? s[j] : __nv_bfloat16();
-                v[u].y = j + 1 < Lk ? s[j + 1] : __nv_bfloat16();
-            }
-#pragma unroll
-            for (int u = 0; u < kU; ++u)
-                if (w0 + 32 * u < words) dst[r * words + w0 + 32 * u] = *reinterpret_cast<const uint32_t*>(&v[u]);
-        }
-    }
-}
-
-// Key mask as bits, and the list of tiles that keep something.  One block per batch element.
-constexpr int kMaskPrepThreads = 1024;
-__global__ void __launch_bounds__(kMaskPrepThreads)
-attn_mask_kernel(const uint8_t* mask, long long mask_b, int Lk, int n_tiles, uint32_t* words, int* list) {
-    __shared__ int any[kMaskPrepThreads / 32];
-    griddep_wait();
-    griddep_launch_dependents();
-    const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint8_t* m = mask + b * mask_b;
-    int* out = list + (long long)b * (n_tiles + 1);
-    int count = 0;
-    for (int t0 = 0; t0 < n_tiles; t0 += kMaskPrepThreads / 32) {
-        const int t = t0 + warp;
-        uint32_t all = 0;
-        if (t < n_tiles) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int j = t * kAfRows + k * 32 + lane;
-                w[k] = __ballot_sync(0xffffffffu, j < Lk && m[min(j, Lk - 1)] != 0);
-                all |= w[k];
-            }
-            if (lane == 0) *reinterpret_cast<uint4*>(words + ((long long)b * n_tiles + t) * 4) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        if (lane == 0) any[warp] = all != 0;
-        __syncthreads();
-        int before = 0, total = 0;
-        for (int k = 0; k < kMaskPrepThreads / 32; ++k) {
-            if (k < warp) before += any[k];
-            total += any[k];
-        }
-        if (lane == 0 && all != 0) out[1 + count + before] = t;
-        count += total;
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) out[0] = count;
-}
-
 __device__ __forceinline__ uint4 tail_words(int left) {      // bits of the first `left` of 128 keys
     auto w = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; };
     return make_uint4(w(left), w(left - 32), w(left - 64), w(left - 96));

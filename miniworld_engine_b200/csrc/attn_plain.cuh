@@ -261,46 +261,6 @@ __global__ void __launch_bounds__(kApThreads) attn_plain_fwd_kernel(const __grid
     }
 }
 
-// delta_i = sum_d dout_id o_id, kLanes lanes per row (four columns a piece where rows allow it).  With 16-bit outputs the part
-// that rounding took off o is added back: where the probabilities' gradients nearly cancel against delta, half a step of o
-// would be all that is left.
-template <typename T, int kLanes>
-__global__ void __launch_bounds__(kApThreads) attn_delta_kernel(const __grid_constant__ AttnParams p) {
-    griddep_wait();
-    griddep_launch_dependents();
-    const long long row = ((long long)blockIdx.x * kApThreads + threadIdx.x) / kLanes;
-    const int lane = threadIdx.x % kLanes;
-    const bool in = row < (long long)p.B * p.Lq * p.H;
-    float t = 0.f;
-    int h = 0, i = 0, b = 0;
-    if (in) {
-        h = (int)(row % p.H);
-        const long long bi = row / p.H;
-        i = (int)(bi % p.Lq);
-        b = (int)(bi / p.Lq);
-        const T* o = static_cast<const T*>(p.o.p) + b * p.o.b + (long long)i * p.o.l + h * p.o.h;
-        const T* g = static_cast<const T*>(p.dout.p) + b * p.dout.b + (long long)i * p.dout.l + h * p.dout.h;
-        const T* lo = sizeof(T) == 2 && p.o_lo != nullptr ? static_cast<const T*>(p.o_lo) + row * p.D : nullptr;
-        if (ap_vec<T>(p.o, p.D) && ap_vec<T>(p.dout, p.D) && (lo == nullptr || (reinterpret_cast<uintptr_t>(lo) & 7) == 0)) {
-            using V = typename ApRaw<T>::V;
-            for (int d = lane * 4; d < p.D; d += kLanes * 4) {
-                float4 y = ap_wide(*reinterpret_cast<const V*>(o + d));
-                const float4 x = ap_wide(*reinterpret_cast<const V*>(g + d));
-                if (lo != nullptr) {
-                    const float4 z = ap_wide(*reinterpret_cast<const V*>(lo + d));
-                    y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
-                }
-                t = fmaf(y.x, x.x, fmaf(y.y, x.y, fmaf(y.z, x.z, fmaf(y.w, x.w, t))));
-            }
-        } else {
-            for (int d = lane; d < p.D; d += kLanes) t = fmaf(at_float(o[d]) + (lo != nullptr ? at_float(lo[d]) : 0.f), at_float(g[d]), t);
-        }
-    }
-#pragma unroll
-    for (int s = kLanes / 2; s >= 1; s >>= 1) t += __shfl_xor_sync(0xffffffffu, t, s);
-    if (in && lane == 0) p.delta[((long long)b * p.H + h) * p.Lq + i] = t;
-}
-
 // Statistics of a thread's rows; then probabilities and score gradients from scores s and products g = dout . v.
 template <int kR>
 struct ApStats {

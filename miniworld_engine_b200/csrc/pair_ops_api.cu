@@ -15,6 +15,7 @@
 #include "attn_fwd64_sm100.cuh"
 #include "attn_fwd_sm100.cuh"
 #include "attn_plain.cuh"
+#include "attn_prep.cuh"
 #include "attn_short.cuh"
 #include "relpos_kernels.cuh"
 
@@ -446,9 +447,36 @@ template <typename T> int run_join(const AttnParams& p, const AttnBwdSplit& w, c
     return rc;
 }
 
-int run_mask(const trimul_attn_desc* d, uint32_t* words, int* list, cudaStream_t st) {
-    return launch_stage(attn_mask_kernel, dim3((unsigned)d->B), kMaskPrepThreads, 0, st, true, d->mask, (long long)d->mask_b, d->Lk,
-                        (int)ceil_div(d->Lk, kAfRows), words, list);
+// What the main kernel needs prepared; `d` gets the bias where the tensor-core kernels can fetch it
+AttnPrep prepare(trimul_attn_desc* d, const AttnWorkspace& w, uint8_t* ws) {
+    AttnPrep r = {};
+    if (copies_bias(d)) {
+        r.bias = reinterpret_cast<uint32_t*>(ws + w.bias);
+        r.bias_heads = d->bias_heads;
+        r.bias_pitch = (int)align_up(d->Lk, 8);
+        r.bias_rows = (int64_t)d->bias_batch * d->bias_heads * d->Lq;
+        r.bias_blocks = (int)std::min<int64_t>(ceil_div(r.bias_rows, kPrepWarps), 4 * (int64_t)sm_count());
+        d->bias = r.bias;
+        d->bias_i = r.bias_pitch;
+        d->bias_h = d->bias_i * d->Lq;
+        d->bias_b = d->bias_h * d->bias_heads;
+    }
+    if (d->mask != nullptr) {
+        r.mask_blocks = d->B;
+        r.n_tiles = (int)ceil_div(d->Lk, kAfRows);
+        r.words = reinterpret_cast<uint32_t*>(ws + w.words);
+        r.list = reinterpret_cast<int*>(ws + w.list);
+    }
+    return r;
+}
+int run_prep(const AttnParams& p, const AttnPrep& w, bool bf16, bool backward, cudaStream_t st) {
+    const int lanes = p.D <= 64 ? 16 : 32;
+    const int64_t delta = backward ? ceil_div((int64_t)p.B * p.Lq * p.H, kPrepThreads / lanes) : 0, blocks = w.mask_blocks + w.bias_blocks + delta;
+    if (blocks == 0) return TRIMUL_OK;
+    if (blocks > INT32_MAX) return TRIMUL_E_UNSUPPORTED;
+    auto kernel = bf16 ? (lanes == 16 ? attn_prep_kernel<__nv_bfloat16, 16> : attn_prep_kernel<__nv_bfloat16, 32>)
+                       : (lanes == 16 ? attn_prep_kernel<float, 16> : attn_prep_kernel<float, 32>);
+    return launch_stage(kernel, dim3((unsigned)blocks), kPrepThreads, 0, st, true, p, w);
 }
 
 template <typename T, int kLanes>
@@ -478,21 +506,6 @@ int run_short(const trimul_attn_desc* d, const AttnParams& p, const AttnWorkspac
     return run_combine<T>(p, sp.part_o, sp.part_ml, sp.splits, st);
 }
 
-// `d` with the bias where the tensor-core kernels can fetch it
-int run_bias_rows(trimul_attn_desc* d, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
-    if (!copies_bias(d)) return TRIMUL_OK;
-    const int64_t rows = (int64_t)d->bias_batch * d->bias_heads * d->Lq, pitch = align_up(d->Lk, 8);
-    const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, 8), 16 * (int64_t)sm_count()));
-    const int rc = launch_stage(attn_bias_rows_kernel, grid, 256, 0, st, true, static_cast<const __nv_bfloat16*>(d->bias),
-                                (long long)d->bias_b, (long long)d->bias_h, (long long)d->bias_i,
-                                reinterpret_cast<uint32_t*>(ws + w.bias), d->bias_heads, d->Lq, d->Lk, (long long)rows, (int)pitch);
-    d->bias = ws + w.bias;
-    d->bias_i = pitch;
-    d->bias_h = pitch * d->Lq;
-    d->bias_b = d->bias_h * d->bias_heads;
-    return rc;
-}
-
 template <bool kBias>
 int launch_fwd(const AttnFwdParams& fp, const CUtensorMap (&m)[4], cudaStream_t st) {
     using L = AfLayout<kBias>;
@@ -511,13 +524,16 @@ int launch_fwd64(const AttnFwdParams& fp, const CUtensorMap (&m)[4], cudaStream_
 int run_fwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorkspace& w, uint8_t* ws, cudaStream_t st) {
     trimul_attn_desc copy = *given;
     const trimul_attn_desc* d = &copy;
-    int rc = run_bias_rows(&copy, w, ws, st);
+    const AttnPrep prep = prepare(&copy, w, ws);
+    int rc = run_prep(p, prep, true, false, st);
     if (rc != TRIMUL_OK) return rc;
     AttnFwdParams fp = {};
     fp.a = p;
     fp.n_tiles = (int)ceil_div(d->Lk, kAfRows);
     fp.splits = forward_splits(d);
     fp.tiles_per_split = (int)ceil_div(fp.n_tiles, fp.splits);
+    fp.words = prep.words;
+    fp.list = prep.list;
     fp.bias_b1 = d->bias_batch == 1;
     fp.bias_h1 = d->bias_heads == 1;
     if (fp.splits > 1) {
@@ -530,14 +546,6 @@ int run_fwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorksp
         return TRIMUL_E_CUDA;
     m[3] = m[0];
     if (d->bias != nullptr && !encode_bias(&m[3], d)) return TRIMUL_E_CUDA;
-    if (d->mask != nullptr) {
-        uint32_t* words = reinterpret_cast<uint32_t*>(ws + w.words);
-        int* list = reinterpret_cast<int*>(ws + w.list);
-        rc = run_mask(d, words, list, st);
-        if (rc != TRIMUL_OK) return rc;
-        fp.words = words;
-        fp.list = list;
-    }
     if (d->D <= 64) rc = d->bias != nullptr ? launch_fwd64<true>(fp, m, st) : launch_fwd64<false>(fp, m, st);
     else rc = d->bias != nullptr ? launch_fwd<true>(fp, m, st) : launch_fwd<false>(fp, m, st);
     if (rc != TRIMUL_OK || fp.splits == 1) return rc;
@@ -556,12 +564,15 @@ int run_bwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorksp
             cudaStream_t st) {
     trimul_attn_desc copy = *given;
     const trimul_attn_desc* d = &copy;
-    int rc = run_bias_rows(&copy, w, ws, st);
+    const AttnPrep prep = prepare(&copy, w, ws);
+    const int rc = run_prep(p, prep, true, true, st);
     if (rc != TRIMUL_OK) return rc;
     AttnBwdParams bp = {};
     bp.a = p;
     bp.w = split;
     bp.n_tiles = (int)ceil_div(d->Lk, kAfRows);
+    bp.words = prep.words;
+    bp.list = prep.list;
     bp.bias_b1 = d->bias_batch == 1;
     bp.bias_h1 = d->bias_heads == 1;
     CUtensorMap m[5];
@@ -570,14 +581,6 @@ int run_bwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorksp
         return TRIMUL_E_CUDA;
     m[4] = m[0];
     if (d->bias != nullptr && !encode_bias(&m[4], d)) return TRIMUL_E_CUDA;
-    if (d->mask != nullptr) {
-        uint32_t* words = reinterpret_cast<uint32_t*>(ws + w.words);
-        int* list = reinterpret_cast<int*>(ws + w.list);
-        rc = run_mask(d, words, list, st);
-        if (rc != TRIMUL_OK) return rc;
-        bp.words = words;
-        bp.list = list;
-    }
     if (d->D <= 64) return d->bias != nullptr ? launch_bwd<64, true>(bp, m, st) : launch_bwd<64, false>(bp, m, st);
     return d->bias != nullptr ? launch_bwd<128, true>(bp, m, st) : launch_bwd<128, false>(bp, m, st);
 }
@@ -684,13 +687,6 @@ int trimul_b200_attn_backward(const trimul_attn_desc* d, void* workspace, size_t
         }
     }
     const bool bf16 = d->dtype == TRIMUL_DTYPE_BF16;
-    const int64_t rows = (int64_t)d->B * d->Lq * d->H;
-    const int lanes = d->D <= 64 ? 16 : 32;
-    const dim3 grid((unsigned)ceil_div(rows, kApThreads / lanes));
-    auto delta = bf16 ? (lanes == 16 ? attn_delta_kernel<__nv_bfloat16, 16> : attn_delta_kernel<__nv_bfloat16, 32>)
-                      : (lanes == 16 ? attn_delta_kernel<float, 16> : attn_delta_kernel<float, 32>);
-    rc = launch_stage(delta, grid, kApThreads, 0, st, true, p);
-    if (rc != TRIMUL_OK) return rc;
     const bool tensor = tensor_core_backward(d);
     AttnBwdSplit split = backward_split(d, tensor);
     if (split.q_blocks == 0) return TRIMUL_E_UNSUPPORTED;
@@ -699,6 +695,8 @@ int trimul_b200_attn_backward(const trimul_attn_desc* d, void* workspace, size_t
         split.dk = reinterpret_cast<float*>(ws + w.dk);
         split.dv = reinterpret_cast<float*>(ws + w.dv);
     }
+    if (!tensor) rc = run_prep(p, AttnPrep{}, bf16, true, st);
+    if (rc != TRIMUL_OK) return rc;
     if (tensor) rc = run_bwd(d, p, w, split, ws, st);
     else rc = bf16 ? run_plain_bwd<__nv_bfloat16>(p, split, st) : run_plain_bwd<float>(p, split, st);
     if (rc == TRIMUL_OK) rc = bf16 ? run_join<__nv_bfloat16>(p, split, st) : run_join<float>(p, split, st);
