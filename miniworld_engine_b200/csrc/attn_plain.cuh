@@ -6,9 +6,9 @@
 // tx + 16 c of a kT x kT tile of scores, r, c < kR = kT / 16, both operands read from shared memory in four-element
 // pieces along the head dimension (pitch D rounded up to 4, plus 4: the sixteen rows that a half warp reads at once then
 // lie in different banks).  What bounds it is the shared-memory pipe: 2 kR reads of 16 bytes for 4 kR^2 multiply-adds, and where
-there are few blocks their latency (fp32, 2 x 256 x 320, 8 heads of 32: forward 21 us in 192 blocks of two or fewer steps, backward
-39 in 144 of four or five).  Backward above 64 columns on 32-row tiles, whose accumulators and operands leave registers and shared
-memory for two blocks an SM.
+// there are few blocks their latency (fp32, 2 x 256 x 320, 8 heads of 32: forward 21 us in 192 blocks of two or fewer steps, backward
+// 39 in 144 of four or five).  Backward above 64 columns on 32-row tiles: the accumulators of dk and dv of 64 rows would not fit
+// into the registers.
 #pragma once
 
 #include "attn_common.cuh"
