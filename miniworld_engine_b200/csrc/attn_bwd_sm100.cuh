@@ -424,7 +424,7 @@ __device__ __forceinline__ void attn_dkv_block(const CUtensorMap& tmQ, const CUt
 // dq and ds: a block per (query tile, head, batch element).  A lane of tensor memory is a query, a column a key.  Key rows of masked keys are
 // zeroed in shared memory, where ds K would read them.
 // ---------------------------------------------------------------------------------------
-template <int kD, bool kBias>
+template <int kD, bool kBias, typename Ds>
 __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
                                               const CUtensorMap& tmG, const CUtensorMap& tmBias, const AttnBwdParams& bp, int block) {
     using L = AbQLayout<kD, kBias>;
@@ -596,13 +596,14 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
         const float2 ml = i < p.Lq ? __ldg(p.stats + srow) : make_float2(0.f, INFINITY);
         const float delta = i < p.Lq ? __ldg(p.delta + srow) : 0.f;
         const float both = -fmaf(ml.x, kLog2e, ml.y);
-        __nv_bfloat16* ds = p.ds != nullptr ? static_cast<__nv_bfloat16*>(p.ds) + b * p.ds_b + h * p.ds_h + i * p.ds_i : nullptr;
+        constexpr int kVec = 16 / (int)sizeof(Ds);
+        Ds* ds = p.ds != nullptr ? static_cast<Ds*>(p.ds) + b * p.ds_b + h * p.ds_h + i * p.ds_i : nullptr;
         bool ok = true;
         int t_next = first > 0 ? tile_at(-1) + 1 : 0;      // first key tile whose ds is not written yet
         auto clear_ds = [&](int t_end) {
             if (ds != nullptr && i < p.Lq)
                 for (int t = t_next; t < t_end; ++t)
-                    for (int e = 0; e < 64; e += 8)
+                    for (int e = 0; e < 64; e += kVec)
                         if (t * kAfRows + g * 64 + e < p.Lk)
                             *reinterpret_cast<uint4*>(ds + t * kAfRows + g * 64 + e) = make_uint4(0u, 0u, 0u, 0u);
             t_next = t_end + 1;
@@ -662,11 +663,15 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
                 clear_ds(t);
                 if (i < p.Lq) {
 #pragma unroll
-                    for (int e = 0; e < 64; e += 8)
-                        if (t * kAfRows + g * 64 + e < p.Lk)
-                            *reinterpret_cast<uint4*>(ds + t * kAfRows + g * 64 + e) =
-                                make_uint4(pack_bf16x2(x[e], x[e + 1]), pack_bf16x2(x[e + 2], x[e + 3]),
-                                           pack_bf16x2(x[e + 4], x[e + 5]), pack_bf16x2(x[e + 6], x[e + 7]));
+                    for (int e = 0; e < 64; e += kVec)
+                        if (t * kAfRows + g * 64 + e < p.Lk) {
+                            if constexpr (sizeof(Ds) == 2)
+                                *reinterpret_cast<uint4*>(ds + t * kAfRows + g * 64 + e) =
+                                    make_uint4(pack_bf16x2(x[e], x[e + 1]), pack_bf16x2(x[e + 2], x[e + 3]),
+                                               pack_bf16x2(x[e + 4], x[e + 5]), pack_bf16x2(x[e + 6], x[e + 7]));
+                            else
+                                *reinterpret_cast<float4*>(ds + t * kAfRows + g * 64 + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                        }
                 }
             }
         }
@@ -696,7 +701,8 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
 }
 
 // Both kinds of blocks in one launch, the kind whose blocks take longer first: its last wave is filled with the other kind's.
-template <int kD, bool kBias>
+// Ds: how the scores' gradients are written, where they are.
+template <int kD, bool kBias, typename Ds>
 __global__ void __launch_bounds__(kAbThreads, 1)
 attn_bwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG,
@@ -704,7 +710,7 @@ attn_bwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     const int first = bp.w.q_first ? bp.w.q_blocks : bp.w.kv_blocks;
     const bool second = (int)blockIdx.x >= first;
     const int block = second ? (int)blockIdx.x - first : (int)blockIdx.x;
-    if (second != (bp.w.q_first != 0)) attn_dq_block<kD, kBias>(tmQ, tmK, tmV, tmG, tmBias, bp, block);
+    if (second != (bp.w.q_first != 0)) attn_dq_block<kD, kBias, Ds>(tmQ, tmK, tmV, tmG, tmBias, bp, block);
     else attn_dkv_block<kD, kBias>(tmQ, tmK, tmV, tmG, tmBias, bp, block);
 }
 

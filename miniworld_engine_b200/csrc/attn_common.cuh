@@ -33,6 +33,7 @@ struct AttnParams {
     float* delta;                          // [B][H][Lq]: sum_d dout o
     void* ds;                              // gradient of x, or null: written with the strides below
     long long ds_b, ds_h, ds_i;
+    int ds_wide;                           // ds is fp32 whatever the inputs are: it is going to be summed
     int32_t* status;
 };
 

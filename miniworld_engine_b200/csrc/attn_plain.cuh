@@ -346,8 +346,11 @@ __device__ __forceinline__ void ap_dq_block(const AttnParams& p, const AttnBwdSp
             for (int c = 0; c < kR; ++c) {
                 const int j = j0 + tx + 16 * c;
                 P[(ty * kR + r) * pp + tx + 16 * c] = g[r][c];
-                if (p.ds != nullptr && i < p.Lq && j < p.Lk)
-                    at_store(static_cast<T*>(p.ds) + b * p.ds_b + h * p.ds_h + i * p.ds_i + j, g[r][c]);
+                if (p.ds != nullptr && i < p.Lq && j < p.Lk) {
+                    const long long at = b * p.ds_b + h * p.ds_h + i * p.ds_i + j;
+                    if (p.ds_wide) static_cast<float*>(p.ds)[at] = g[r][c];
+                    else at_store(static_cast<T*>(p.ds) + at, g[r][c]);
+                }
             }
         }
         __syncwarp();
@@ -493,13 +496,13 @@ attn_join_kernel(const float* part0, const float* part1, AttnTensor t0, AttnTens
     }
 }
 
-// Gradient of a bias that serves several batch elements or heads: the scores' gradients [B][H][Lq][pitch] summed over
-// the broadcast axes, in fp32 and in a fixed order.
-template <typename T>
+// Gradient of a bias that serves several batch elements or heads: the scores' gradients [B][H][Lq][pitch] (TS: as they were
+// written) summed over the broadcast axes, in fp32 and in a fixed order.
+template <typename T, typename TS>
 __global__ void __launch_bounds__(kApThreads)
-attn_bias_sum_kernel(const T* ds, long long ds_b, long long ds_h, long long ds_i, T* out, long long out_b, long long out_h,
+attn_bias_sum_kernel(const TS* ds, long long ds_b, long long ds_h, long long ds_i, T* out, long long out_b, long long out_h,
                      long long out_i, int B, int H, int Lq, int Lk, int sum_b, int sum_h) {
-    constexpr int kN = 16 / (int)sizeof(T);
+    constexpr int kN = 16 / (int)sizeof(T), kLoads = kN * (int)sizeof(TS) / 16;
     griddep_wait();
     griddep_launch_dependents();
     const int nch = (Lk + kN - 1) / kN;
@@ -518,17 +521,20 @@ attn_bias_sum_kernel(const T* ds, long long ds_b, long long ds_h, long long ds_i
 #pragma unroll 4
         for (int s = 0; s < nb * nh; ++s) {
             const int b = b0 + s / nh, h = h0 + s % nh;
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(ds + b * ds_b + h * ds_h + i * ds_i) + c);
-            if constexpr (sizeof(T) == 2) {
+            const uint4* src = reinterpret_cast<const uint4*>(ds + b * ds_b + h * ds_h + i * ds_i) + (long long)c * kLoads;
+#pragma unroll
+            for (int l = 0; l < kLoads; ++l) {
+                const uint4 v = __ldg(src + l);
                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    acc[2 * e] += bf16_lo(w[e]);
-                    acc[2 * e + 1] += bf16_hi(w[e]);
+                    if constexpr (sizeof(TS) == 2) {
+                        acc[2 * e] += bf16_lo(w[e]);
+                        acc[2 * e + 1] += bf16_hi(w[e]);
+                    } else {
+                        acc[4 * l + e] += __uint_as_float(w[e]);
+                    }
                 }
-            } else {
-                acc[0] += __uint_as_float(v.x); acc[1] += __uint_as_float(v.y);
-                acc[2] += __uint_as_float(v.z); acc[3] += __uint_as_float(v.w);
             }
         }
         uint4 v;

@@ -349,3 +349,22 @@ def test_loops_that_several_blocks_share(B, Lq, Lk, H, Hk, D, bias, dtype, plain
         assert torch.equal(first[name], again[name]), name
     mask[-1] = False
     _check_all(q, k, v, g, b, mask, plain_kernels=plain)
+
+
+@pytest.mark.parametrize("Lq,D", [(1, 96), (9, 64), (40, 20)])
+def test_shared_bias_gradient_of_a_small_call_is_rounded_once(Lq, D):
+    """Half a bf16 step of the sum (2^-8), and of every summand the fp32 arithmetic and the 16 bits of ``o`` in delta: far
+    below 2^-12 of p (|dout . v| + |delta|).  Rounding every summand to bf16 first would be off by up to 2^-8 of those.
+    delta is taken from the result that the forward pass returned: its probabilities are rounded to bf16 on their way into
+    the product with v, which moves delta by up to 2^-8 of sum p |dout . v| and is no part of this rounding."""
+    from miniworld_engine_b200 import cross_attention_backward_b200, cross_attention_forward_b200
+    q, k, v, g, b, _ = _inputs(4, Lq, 70, 2, 2, D, "1H", None, BF16, seed=Lq)
+    out, state = cross_attention_forward_b200(q, k, v, bias=b)
+    got = cross_attention_backward_b200(g, q, k, v, out, state, bias=b)[3].double()
+    o = out.double() + state.rounding.double()
+    q, k, v, g, o = (t.double().transpose(1, 2) for t in (q, k, v, g, o))
+    p = (q @ k.mT * D ** -0.5 + b.double()).softmax(-1)
+    dp = g @ v.mT
+    delta = (g * o).sum(-1, keepdim=True)
+    want, size = (p * (dp - delta)).sum(0), (p * (dp.abs() + delta.abs())).sum(0)
+    assert (((got - want).abs() - 2.0 ** -8 * want.abs()) <= 2.0 ** -12 * size).all()
