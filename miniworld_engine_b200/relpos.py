@@ -48,7 +48,12 @@ class PositionBuckets:
             raise NotImplementedError(f"at most {_lib.MAX_THRESHOLDS} shared buckets a side are supported, got {len(thresholds)}")
         self._struct = _lib.Buckets(kind, count, max_distance, int(self.segments), len(thresholds),
                                     (C.c_int32 * _lib.MAX_THRESHOLDS)(*thresholds))
-        self._address = C.addressof(self._struct)
+
+    @property
+    def _address(self) -> int:
+        """Where the library reads the rule; asked for at every call, since a copy (``copy.deepcopy``, pickle) has a
+        structure of its own."""
+        return C.addressof(self._struct)
 
     @staticmethod
     @functools.lru_cache(maxsize=256)

@@ -215,3 +215,64 @@ def test_c_abi_wants_the_statistics_on_eight_bytes(lib):
         assert lib.trimul_b200_attn_workspace_bytes(C.byref(d), 1, C.byref(n)) == rc
     assert lib.trimul_b200_attn_forward(C.byref(d), 4096, 1 << 20, None, None) == _lib.E_INVALID
     assert lib.trimul_b200_attn_backward(C.byref(d), 4096, 1 << 20, None, None) == _lib.E_INVALID
+
+
+# what a process does with a rule that came to it: the library reads it (here for the size of a workspace)
+_READ_RULE = """
+import ctypes as C, pickle, sys
+from miniworld_engine_b200 import _lib
+rules = pickle.loads(bytes.fromhex(sys.stdin.read()))
+for rule in rules:
+    desc = _lib.RelposDesc(C.sizeof(_lib.RelposDesc), 0, 0, 1, 1, 8, 8, 4, 0, 0, 0, 0, 0, 0, 0, 64, 8)
+    n = C.c_size_t()
+    rc = _lib.load().trimul_b200_relpos_bias_grad_workspace_bytes(C.byref(desc), rule._address, C.byref(n))
+    print(rc, rule.rows, n.value)
+"""
+
+
+def _read_rule(lib, rule):
+    desc = _lib.RelposDesc(C.sizeof(_lib.RelposDesc), 0, 0, 1, 1, 8, 8, 4, 0, 0, 0, 0, 0, 0, 0, 64, 8)
+    n = C.c_size_t()
+    return lib.trimul_b200_relpos_bias_grad_workspace_bytes(C.byref(desc), rule._address, C.byref(n)), rule.rows, n.value
+
+
+def test_rules_survive_another_process(lib):
+    import os
+    import pickle
+    import subprocess
+    import sys
+    rules = [PositionBuckets.clipped(20, segments=True), PositionBuckets.logarithmic(32, 128),
+             RelativePositionBiasB200(PositionBuckets.clipped(7), 4).buckets]
+    want = [_read_rule(lib, r) for r in rules]
+    got = subprocess.run([sys.executable, "-c", _READ_RULE], input=pickle.dumps(rules).hex(), capture_output=True, text=True,
+                         cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), timeout=600)
+    assert got.returncode == 0, got.stderr[-2000:]
+    assert [tuple(int(x) for x in line.split()) for line in got.stdout.splitlines()] == want
+    assert all(rc == 0 for rc, _, _ in want)
+
+
+def test_copies_of_a_rule_do_not_need_the_original(lib):
+    """A deep copy (an averaged model's) reads its own struct, also when the original and its memory are gone."""
+    import copy
+    import gc
+    for make in (lambda: PositionBuckets(_lib.BUCKETS_CLIPPED, 19, 9, (), True),         # not kept by the factories' cache
+                 lambda: PositionBuckets(_lib.BUCKETS_LOG, 8, 30, (4,), False)):
+        for dup in (copy.deepcopy, copy.copy):
+            rule = make()
+            want = _read_rule(lib, rule)
+            kept = dup(rule)
+            size = C.sizeof(rule._struct)
+            own = C.addressof(kept._struct)
+            assert kept._address == own
+            del rule
+            gc.collect()
+            filler = [C.create_string_buffer(b"\xff" * size, size) for _ in range(64)]        # likely to land on freed memory
+            assert _read_rule(lib, kept) == want and want[0] == 0
+            assert kept.rows == want[1] and len(filler) == 64
+    module = RelativePositionBiasB200(PositionBuckets(_lib.BUCKETS_CLIPPED, 19, 9, (), True), 4)
+    twin = copy.deepcopy(module)
+    assert twin.buckets._address == C.addressof(twin.buckets._struct)
+    want = _read_rule(lib, module.buckets)
+    del module
+    gc.collect()
+    assert _read_rule(lib, twin.buckets) == want
