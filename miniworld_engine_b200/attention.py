@@ -262,7 +262,7 @@ def cross_attention_b200(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, b
     transposed view).  bf16 or fp32, the same for all; ``D`` at most 256.  ``bias``: ``[(B,) (H,) Lq, Lk]``,
     axes of size 1 shared; minus infinity masks a pair.  ``key_mask``: ``[B, Lk]``, False at keys that are
     left out, whose keys and values may hold anything, NaN included.  ``scale`` defaults to ``D ** -0.5``.
-    A row without a kept key gives zeros (and zero gradients).
+    A row without a kept key gives zeros (and zero gradients); a row whose scores hold a NaN gives NaN.
 
     bf16 with ``D`` a multiple of 8 up to 128 runs on the tensor cores, everything else (and
     ``plain_kernels=True``) on the CUDA cores in fp32 arithmetic.  Differentiable in ``q``, ``k``, ``v`` and

@@ -3,7 +3,8 @@
 //   x_ij = scale q_i . k_j + bias_ij   over the kept keys j,   p_ij = exp(x_ij - m_i) / l_i,   o_i = sum_j p_ij v_j
 //
 // with m_i the row's maximum and l_i the sum of exp(x_ij - m_i).  A row without a kept key gives o_i = 0 and zero
-// gradients.  Statistics of a row are kept as the pair (m_i, log2 l_i) rather than their sum: a mask of the type's lowest
+// gradients; it is known by l_i = 0.  The maximum does not tell: it passes over NaN, so a row of nothing but NaN also leaves
+// it at -inf, and that row's sum and result are NaN.  Statistics of a row are kept as the pair (m_i, log2 l_i) rather than their sum: a mask of the type's lowest
 // value (-3.4e38) on a whole row would swallow log l_i, and every probability would come back as 1.  For the same reason
 // x - m is formed before it is scaled to base 2 wherever a bias takes part.
 #pragma once

@@ -355,7 +355,7 @@ attn_fwd64_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     const float mm = fmaxf(m, ml.x), base = mm == -INFINITY ? 0.f : mm;
                     const float f0 = ex2f((m - base) * mul), f1 = ex2f((ml.x - base) * mul);
                     l = l * f0 + ml.y * f1;
-                    const bool nothing = mm == -INFINITY || n == 0;
+                    const bool nothing = l == 0.f;
                     const float inv = nothing ? 0.f : fp.splits > 1 ? 1.f : 1.f / l;
                     const float g0 = f0 * inv, g1 = f1 * inv;
                     const bool live = i < p.Lq;

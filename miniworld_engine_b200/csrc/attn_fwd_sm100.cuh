@@ -377,7 +377,7 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             if (n > 0 && ok) ok = warp_wait(&o_full[w], 0, lane, abort_flag, p.status, kStageIdAttnFwd, 420 + w);
             tcgen05_fence_after();
             if (ok) {
-                const bool nothing = m == -INFINITY || n == 0;
+                const bool nothing = l == 0.f;                // no kept key; NaN is none of these
                 const float inv = nothing ? 0.f : 1.f / l;
                 const bool live = i < p.Lq;
                 const long long srow = ((long long)b * p.H + h) * p.Lq + i;
@@ -462,8 +462,7 @@ attn_combine_kernel(const __grid_constant__ AttnParams p, const float* part_o, c
     for (int s = lane; s < splits; s += 32) m = fmaxf(m, __ldg(part_ml + s * rows + r).x);
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const bool nothing = m == -INFINITY;
-    const float base = nothing ? 0.f : m;
+    const float base = m == -INFINITY ? 0.f : m;
     float l = 0.f, y[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) y[k] = 0.f;
@@ -483,6 +482,7 @@ attn_combine_kernel(const __grid_constant__ AttnParams p, const float* part_o, c
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    const bool nothing = l == 0.f;
     const float inv = nothing ? 0.f : 1.f / l;
     const int i = (int)(r % p.Lq), h = (int)((r / p.Lq) % p.H), b = (int)(r / p.Lq / p.H);
     if (lane == 0 && p.stats != nullptr) p.stats[r] = nothing ? make_float2(0.f, INFINITY) : make_float2(m, log2f(l));

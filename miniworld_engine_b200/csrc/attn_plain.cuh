@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kApThreads) attn_plain_fwd_kernel(const __grid
             if (tx == 0) part_ml[row] = make_float2(m[r], l[r]);
             continue;
         }
-        const bool empty = m[r] == -INFINITY;
+        const bool empty = l[r] == 0.f;
         const float inv = empty ? 0.f : 1.f / l[r];
         T* dst = static_cast<T*>(p.o.p) + b * p.o.b + (long long)i * p.o.l + h * p.o.h;
         const long long lo = (((long long)b * p.Lq + i) * p.H + h) * p.D;
@@ -286,7 +286,8 @@ struct ApStats {
         for (int r = 0; r < kR; ++r)
 #pragma unroll
             for (int c = 0; c < kR; ++c) {
-                const float e = exp2f(fmaf(s[r][c] - st[r].x, kLog2e, -st[r].y));
+                // a masked pair has none, also in a row whose statistics are NaN
+                const float e = s[r][c] == -INFINITY ? 0.f : exp2f(fmaf(s[r][c] - st[r].x, kLog2e, -st[r].y));
                 s[r][c] = e;
                 g[r][c] = e == 0.f ? 0.f : e * (g[r][c] - delta[r]);
             }

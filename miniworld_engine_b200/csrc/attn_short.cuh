@@ -209,7 +209,7 @@ attn_short_kernel(const __grid_constant__ AttnShortParams sp) {
         }
         int h, i;
         row(r, h, i);
-        const bool nothing = mx == -INFINITY;
+        const bool nothing = sum == 0.f;
         const long long srow = ((long long)b * p.H + h) * p.Lq + i;
         if (sp.splits > 1) {
             const long long prow = (long long)split * p.B * p.H * p.Lq + srow;
