@@ -14,7 +14,8 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .functional import _dtype_code, _mask_bytes, _on_device, _require_cuda, _status, _status_words, _stream_handle
+from .functional import (_dtype_code, _mask_bytes, _on_device, _require_cuda, _require_no_tangent, _status, _status_words,
+                         _stream_handle)
 
 __all__ = ["cross_attention_b200", "cross_attention_forward_b200", "cross_attention_backward_b200", "AttentionState"]
 
@@ -266,7 +267,8 @@ def cross_attention_b200(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, b
 
     bf16 with ``D`` a multiple of 8 up to 128 runs on the tensor cores, everything else (and
     ``plain_kernels=True``) on the CUDA cores in fp32 arithmetic.  Differentiable in ``q``, ``k``, ``v`` and
-    ``bias``."""
+    ``bias``, in reverse mode; an input with a forward-mode tangent is refused."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
         return _CrossAttention.apply(q, k, v, bias, key_mask, scale, plain_kernels)
+    _require_no_tangent("cross_attention_b200", q, k, v, bias)
     return _forward(_Call(q, k, v, bias, key_mask, scale, plain_kernels), False)[0]

@@ -54,6 +54,19 @@ def _require_no_grad(what: str, *tensors) -> None:
             "inputs and parameters that do not require grad")
 
 
+_forward_ad = torch.autograd.forward_ad
+
+
+def _require_no_tangent(what: str, *tensors) -> None:
+    """Forward-mode derivatives: a dual tensor need not require a gradient, so a call that leaves autograd out when none of
+    its inputs does would drop the tangent, that is, return a zero derivative.  Raise instead (an autograd function
+    without a forward-mode rule raises by itself).  Without an open dual level no tensor carries a tangent."""
+    if getattr(_forward_ad, "_current_level", 0) < 0:
+        return
+    if any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative: an input carries a tangent")
+
+
 def _plain(t: torch.Tensor) -> torch.Tensor:
     """``t`` detached and contiguous; ``t`` itself when it already is a contiguous tensor outside autograd."""
     if t.requires_grad:

@@ -16,7 +16,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .functional import _dtype_code, _on_device, _require_cuda, _stream_handle
+from .functional import _dtype_code, _on_device, _require_cuda, _require_no_tangent, _stream_handle
 
 __all__ = ["PositionBuckets", "relative_position_bias_b200", "relative_position_bias_backward_b200",
            "RelativePositionBiasB200"]
@@ -293,10 +293,11 @@ def relative_position_bias_b200(table: torch.Tensor, buckets: PositionBuckets, q
     ``add`` where given (the pair tensor; the sum is rounded once).  The result has the dtype of
     ``add``, else ``dtype``, else that of the table.
 
-    Differentiable in ``table`` and ``add``.  ``relative_position_bias_backward_b200`` is the gradient as
-    a call of its own."""
+    Differentiable in ``table`` and ``add`` in reverse mode; an input with a forward-mode tangent is refused.
+    ``relative_position_bias_backward_b200`` is the gradient as a call of its own."""
     if torch.is_grad_enabled() and (table.requires_grad or (add is not None and add.requires_grad)):
         return _RelativePositionBias.apply(table, add, buckets, q_pos, k_pos, q_segment, k_segment, layout, dtype)
+    _require_no_tangent("relative_position_bias_b200", table, add)
     return _forward(table, buckets, q_pos, k_pos, q_segment, k_segment, layout, add, dtype)
 
 

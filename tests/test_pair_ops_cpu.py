@@ -276,3 +276,28 @@ def test_copies_of_a_rule_do_not_need_the_original(lib):
     del module
     gc.collect()
     assert _read_rule(lib, twin.buckets) == want
+
+
+@pytest.mark.parametrize("no_grad", [False, True])
+def test_forward_mode_tangents_are_refused(no_grad):
+    """A dual tensor does not require a gradient: the call must not return a result without its tangent."""
+    import contextlib
+    import torch.autograd.forward_ad as fwd
+    rule, pos = PositionBuckets.clipped(4), torch.arange(5)
+    q, k, b = torch.zeros(1, 5, 2, 8), torch.zeros(1, 5, 2, 8), torch.zeros(2, 5, 5)
+    t, add = torch.zeros(9, 4), torch.zeros(5, 5, 4)
+    f, attend = relative_position_bias_b200, cross_attention_b200
+    with fwd.dual_level(), torch.no_grad() if no_grad else contextlib.nullcontext():
+        dual = lambda x: fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: attend(dual(q), k, k), lambda: attend(q, dual(k), k), lambda: attend(q, k, dual(k)),
+                     lambda: attend(q, k, k, bias=dual(b)), lambda: f(dual(t), rule, pos),
+                     lambda: f(t, rule, pos, layout="pair", add=dual(add))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        for call in (lambda: attend(q, k, k, bias=b), lambda: f(t, rule, pos)):      # no tangent: the usual refusal on the CPU
+            with pytest.raises(RuntimeError, match="no CPU path"):
+                call()
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda x: attend(x, k, k), (q,), (q,))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        attend(q, k, k)
