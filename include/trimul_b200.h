@@ -369,7 +369,8 @@ typedef struct trimul_relpos_desc {
     int32_t  B, Lq, Lk;
     int32_t  channels;                    /* heads or channels: columns of the table                  */
     int32_t  wide_index;                  /* bit 0 q_pos, 1 k_pos, 2 q_seg, 3 k_seg: int64 instead of
-                                             int32.  Values of 2^30 and beyond are taken as 2^30 - 1   */
+                                             int32.  Positions beyond +-(2^30 - 1) are taken as that
+                                             value; segments are compared for equality as they are    */
     int32_t  reserved;
     int64_t  q_pos_b, k_pos_b, q_seg_b, k_seg_b;   /* batch strides in elements, 0 where shared       */
     int64_t  stride_b, stride_h, stride_i;         /* HEADS: of out or of the upstream gradient       */

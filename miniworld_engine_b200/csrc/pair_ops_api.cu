@@ -119,6 +119,8 @@ int run_relpos_forward(const trimul_relpos_desc* d, const trimul_buckets* b, con
                         static_cast<T*>(out), (int)per_block);
 }
 
+inline bool wide_segments(const trimul_relpos_desc* d, const trimul_buckets* b) { return b->segments != 0 && (d->wide_index & 12) != 0; }
+
 // Launch shape of the gradient: `parts` partial tables of rows * channels sums each.
 struct RelposGradPlan {
     int threads, smem, parts, lane_channels, column_blocks, parts_per_b, heads;
@@ -145,7 +147,7 @@ RelposGradPlan plan_relpos_grad(const trimul_relpos_desc* d, const trimul_bucket
         g.parts_per_b = (int)ceil_div(d->Lq, g.per_part);
         g.parts = d->B * g.parts_per_b;
         g.column_blocks = (int)ceil_div(d->channels, g.heads);
-        g.smem = sums + (int)g.per_part * 8 + lut;
+        g.smem = sums + (int)g.per_part * (wide_segments(d, b) ? 12 : 8) + lut;
         return g;
     }
     const int64_t total = (int64_t)d->B * d->Lq * d->Lk;
@@ -166,6 +168,13 @@ bool wide_lanes(const trimul_relpos_desc* d, const void* grad) {
     return (d->channels % 4) == 0 && aligned(grad, 4 * elem_size(d->dtype));
 }
 
+template <typename T, typename Seg>
+auto heads_grad_kernel(bool vec, int heads) {
+    return heads == 4 ? (vec ? relpos_heads_grad_kernel<T, true, 4, Seg> : relpos_heads_grad_kernel<T, false, 4, Seg>)
+         : heads == 2 ? (vec ? relpos_heads_grad_kernel<T, true, 2, Seg> : relpos_heads_grad_kernel<T, false, 2, Seg>)
+                      : (vec ? relpos_heads_grad_kernel<T, true, 1, Seg> : relpos_heads_grad_kernel<T, false, 1, Seg>);
+}
+
 template <typename T>
 int run_relpos_grad(const trimul_relpos_desc* d, const trimul_buckets* b, const RelposParams& p, const void* grad,
                     void* dtable, float* partial, cudaStream_t st) {
@@ -174,9 +183,7 @@ int run_relpos_grad(const trimul_relpos_desc* d, const trimul_buckets* b, const 
     const RelposGradPlan g = plan_relpos_grad(d, b, wide_lanes(d, grad));
     if (d->layout == TRIMUL_RELPOS_HEADS) {
         const bool vec = aligned(grad, 16) && (p.sB % kN) == 0 && (p.sH % kN) == 0 && (p.sI % kN) == 0;
-        auto kernel = g.heads == 4 ? (vec ? relpos_heads_grad_kernel<T, true, 4> : relpos_heads_grad_kernel<T, false, 4>)
-                    : g.heads == 2 ? (vec ? relpos_heads_grad_kernel<T, true, 2> : relpos_heads_grad_kernel<T, false, 2>)
-                                   : (vec ? relpos_heads_grad_kernel<T, true, 1> : relpos_heads_grad_kernel<T, false, 1>);
+        auto kernel = wide_segments(d, b) ? heads_grad_kernel<T, long long>(vec, g.heads) : heads_grad_kernel<T, int>(vec, g.heads);
         if (!ensure_smem(kernel, kMaxSmem)) return TRIMUL_E_CUDA;
         rc = launch_stage(kernel, dim3((unsigned)g.parts, (unsigned)g.column_blocks), g.threads, g.smem, st, true, p, *b,
                           static_cast<const T*>(grad), partial, g.parts_per_b, (int)g.per_part);

@@ -36,6 +36,10 @@ __device__ __forceinline__ int rp_load(const void* p, long long i, int is64) {
     }
     return min(max(__ldg(static_cast<const int*>(p) + i), -kRpPosLimit), kRpPosLimit);
 }
+// Segments are only compared for equality, so they are taken as they are, in full width
+__device__ __forceinline__ long long rp_segment(const void* p, long long i, int is64) {
+    return is64 ? __ldg(static_cast<const long long*>(p) + i) : (long long)__ldg(static_cast<const int*>(p) + i);
+}
 __device__ __forceinline__ float rp_table(const RelposParams& p, int u, int c) {
     const long long i = (long long)u * p.C + c;
     return p.table_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.table)[i])
@@ -145,13 +149,13 @@ relpos_heads_kernel(const __grid_constant__ RelposParams p, const __grid_constan
         const int j0 = (int)(it - row * nch) * kN;
         const int b = (int)(row / p.Lq), i = (int)(row - (long long)b * p.Lq);
         const int q = rp_load(p.q_pos, b * p.q_pos_b + i, p.q_pos64);
-        const int qs = p.q_seg != nullptr ? rp_load(p.q_seg, b * p.q_seg_b + i, p.q_seg64) : 0;
+        const long long qs = p.q_seg != nullptr ? rp_segment(p.q_seg, b * p.q_seg_b + i, p.q_seg64) : 0;
         uint4 r[kN];
 #pragma unroll
         for (int e = 0; e < kN; ++e) {
             const int j = min(j0 + e, p.Lk - 1);
             int u = rp_bucket(lut, p.M, q - rp_load(p.k_pos, b * p.k_pos_b + j, p.k_pos64));
-            if (p.q_seg != nullptr && rp_load(p.k_seg, b * p.k_seg_b + j, p.k_seg64) != qs) u = p.rows - 1;
+            if (p.q_seg != nullptr && rp_segment(p.k_seg, b * p.k_seg_b + j, p.k_seg64) != qs) u = p.rows - 1;
             r[e] = *reinterpret_cast<const uint4*>(tab + (u ^ ((u >> 3) & 7)) * kN);
         }
         rp_transpose(r);
@@ -187,7 +191,7 @@ struct RpCursor {          // position -> (batch element, row, column), stepped 
     __device__ __forceinline__ int bucket(const RelposParams& p, const uint16_t* lut) const {
         const int d = rp_load(p.q_pos, b * p.q_pos_b + i, p.q_pos64) - rp_load(p.k_pos, b * p.k_pos_b + j, p.k_pos64);
         int u = rp_bucket(lut, p.M, d);
-        if (p.q_seg != nullptr && rp_load(p.q_seg, b * p.q_seg_b + i, p.q_seg64) != rp_load(p.k_seg, b * p.k_seg_b + j, p.k_seg64))
+        if (p.q_seg != nullptr && rp_segment(p.q_seg, b * p.q_seg_b + i, p.q_seg64) != rp_segment(p.k_seg, b * p.k_seg_b + j, p.k_seg64))
             u = p.rows - 1;
         return u;
     }
@@ -277,8 +281,10 @@ relpos_pair_kernel(const __grid_constant__ RelposParams p, const __grid_constant
 // keeps kN consecutive j and walks down the rows, all kH heads at once: the bucket of a position is found once for them.
 // Where the outermost distances of a piece share a bucket (buckets are monotone on either side of zero, so everything
 // between shares it too), the piece is summed in registers; the running bucket's sums go to shared memory when it changes.
+// Seg: what holds a segment, 64 bits where either side's numbers have them: they cost registers, by which the resident
+// blocks are counted (16 x 2048^2 with three chains, forward and gradient: 129 us with 32-bit segments, 139 with 64-bit ones).
 // ---------------------------------------------------------------------------------------
-template <typename T, bool kVec, int kH>
+template <typename T, bool kVec, int kH, typename Seg>
 __global__ void __launch_bounds__(kRpThreads)
 relpos_heads_grad_kernel(const __grid_constant__ RelposParams p, const __grid_constant__ trimul_buckets rule, const T* grad,
                          float* partial, int parts_per_b, int rows_per_part) {
@@ -287,8 +293,9 @@ relpos_heads_grad_kernel(const __grid_constant__ RelposParams p, const __grid_co
     extern __shared__ __align__(16) uint8_t rp_smem[];
     float* acc = reinterpret_cast<float*>(rp_smem);                               // [rows][kH][threads]
     const int nt = blockDim.x, tid = threadIdx.x;
-    int* sq = reinterpret_cast<int*>(acc + (size_t)p.rows * kH * nt);             // the part's query positions, then segments
-    uint16_t* lut = reinterpret_cast<uint16_t*>(sq + 2 * rows_per_part);
+    Seg* sg = reinterpret_cast<Seg*>(acc + (size_t)p.rows * kH * nt);             // the part's query segments, then positions
+    int* sq = reinterpret_cast<int*>(sg + rows_per_part);
+    uint16_t* lut = reinterpret_cast<uint16_t*>(sq + rows_per_part);
     rp_build_lut(lut, rule, p.M);
     for (int u = 0; u < p.rows * kH; ++u) acc[u * nt + tid] = 0.f;
     griddep_wait();
@@ -307,7 +314,7 @@ relpos_heads_grad_kernel(const __grid_constant__ RelposParams p, const __grid_co
     for (int r = tid; r < r1; r += nt) {
         const int i = first + r * parts_per_b;
         sq[r] = rp_load(p.q_pos, b * p.q_pos_b + i, p.q_pos64);
-        sq[rows_per_part + r] = p.q_seg != nullptr ? rp_load(p.q_seg, b * p.q_seg_b + i, p.q_seg64) : 0;
+        sg[r] = p.q_seg != nullptr ? (Seg)rp_segment(p.q_seg, b * p.q_seg_b + i, p.q_seg64) : 0;
     }
     __syncthreads();
     int run = 0;
@@ -326,12 +333,13 @@ relpos_heads_grad_kernel(const __grid_constant__ RelposParams p, const __grid_co
     if (ty < side) {
         for (int c = tx; c < nch; c += tpr) {
             const int j0 = c * kN, nj = min(kN, p.Lk - j0);
-            int kp[kN], ks[kN];
+            int kp[kN];
+            Seg ks[kN];
 #pragma unroll
             for (int e = 0; e < kN; ++e) {
                 const int j = min(j0 + e, p.Lk - 1);
                 kp[e] = rp_load(p.k_pos, b * p.k_pos_b + j, p.k_pos64);
-                ks[e] = p.k_seg != nullptr ? rp_load(p.k_seg, b * p.k_seg_b + j, p.k_seg64) : 0;
+                ks[e] = p.k_seg != nullptr ? (Seg)rp_segment(p.k_seg, b * p.k_seg_b + j, p.k_seg64) : 0;
             }
             int kmin = kp[0], kmax = kp[0];
             bool one_seg = true;
@@ -366,7 +374,8 @@ relpos_heads_grad_kernel(const __grid_constant__ RelposParams p, const __grid_co
                 for (int s = 0; s < kU; ++s) {
                     const int rr = r + s * side;
                     if (rr >= r1) break;
-                    const int q = sq[rr], qs = sq[rows_per_part + rr];
+                    const int q = sq[rr];
+                    const Seg qs = sg[rr];
                     const bool apart = one_seg && ks[0] != qs;
                     const int ulo = rp_bucket(lut, p.M, q - kmax), uhi = rp_bucket(lut, p.M, q - kmin);
                     float g[kH][kN];

@@ -284,8 +284,9 @@ def relative_position_bias_b200(table: torch.Tensor, buckets: PositionBuckets, q
     """The rows of ``table`` that the position pairs' buckets select.
 
     ``table``: ``[buckets.rows, channels]``, bf16 or fp32.  ``q_pos``, ``k_pos`` (default: ``q_pos``):
-    ``[Lq]``, ``[Lk]`` or with a leading batch axis, int32 or int64; values of ``2^30`` and beyond (of either
-    sign) are taken as ``2^30 - 1``.  ``q_segment``, ``k_segment``: as the positions, for buckets with ``segments``.
+    ``[Lq]``, ``[Lk]`` or with a leading batch axis, int32 or int64; values beyond ``2^30 - 1`` of either sign are
+    taken as that value.  ``q_segment``, ``k_segment``: integers in the positions' shapes, for buckets with
+    ``segments``; only their equality counts, so they may be any numbers.
 
     ``layout="heads"``: ``[(B,) channels, Lq, Lk]``, the form that ``cross_attention_b200`` takes as its
     bias.  Rows start on 16-byte boundaries: where ``Lk`` is not a multiple of 16 bytes, the result is a

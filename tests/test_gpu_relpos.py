@@ -241,3 +241,39 @@ def test_offsets_beyond_32_bits(layout):
     # added, each addition off by 2^-24 of the sum.  A row left out would be 2^-13.6 of it
     want = (pairs.double() * 2.0 ** -10)[:, None]
     assert ((got.double() - want).abs() <= 2.0 ** -14 * want).all()
+
+
+def _far_ids(to):
+    """Segment ids that agree in what a clamp, a low word or a sign would leave of them."""
+    if to is torch.int32:
+        return [2 ** 30, 2 ** 30 + 1, 2 ** 31 - 1, -2 ** 30, -2 ** 30 - 1, -2 ** 31, 0x41414141, 0x42414141, 0, -1]
+    return [2 ** 30, 2 ** 30 + 1, 2 ** 32, 2 ** 33, 5, 2 ** 32 + 5, 2 ** 40 + 5, -2 ** 32 + 5, 2 ** 63 - 1, -2 ** 63, -1, 2 ** 32 - 1]
+
+
+@pytest.mark.parametrize("layout,channels", [("heads", 8), ("heads", 1), ("pair", 64), ("pair", 3)])
+@pytest.mark.parametrize("q_type,k_type", [(torch.int32, torch.int32), (torch.int64, torch.int64), (torch.int64, torch.int32),
+                                           (torch.int32, torch.int64)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_segments_are_told_apart_whatever_their_numbers(layout, channels, q_type, k_type, dtype):
+    from miniworld_engine_b200 import relative_position_bias_b200, relative_position_bias_backward_b200
+    gen = torch.Generator().manual_seed(9)
+    ids = lambda to: torch.tensor(_far_ids(to), dtype=torch.int64)
+    Lq, Lk = 75, 130
+    qs = ids(q_type)[torch.randint(len(ids(q_type)), (Lq,), generator=gen)]
+    ks = ids(k_type)[torch.randint(len(ids(k_type)), (Lk,), generator=gen)]
+    ks[40:80] = ids(k_type)[0]                                  # runs of one segment: the gradients add them up together
+    qs[20:60] = ids(q_type)[1]
+    q, k = torch.randint(-9, 10, (Lq,), generator=gen), torch.arange(Lk) - 60
+    u = bucket_matrix(q, k, "clip", 9, 4, qs, ks).cuda()
+    buckets = _rule("clip4", True)
+    kw = {"q_segment": qs.to(q_type).cuda(), "k_segment": ks.to(k_type).cuda(), "layout": layout}
+    assert (kw["q_segment"].cpu().long() == qs).all() and (kw["k_segment"].cpu().long() == ks).all()
+    table = torch.randn(10, channels, device="cuda")
+    want = table[u].to(dtype)
+    want = want if layout == "pair" else want.movedim(-1, 0)
+    assert torch.equal(relative_position_bias_b200(table, buckets, q.cuda(), k.cuda(), dtype=dtype, **kw), want)
+    g = torch.randint(-3, 4, want.shape, device="cuda").to(dtype)
+    flat = (g if layout == "pair" else g.movedim(0, -1)).reshape(-1, channels).double()
+    sums = torch.zeros(10, channels, dtype=torch.float64, device="cuda").index_add_(0, u.flatten(), flat)
+    got = relative_position_bias_backward_b200(g, buckets, q.cuda(), k.cuda(), **kw)
+    assert torch.equal(got.double(), sums)
