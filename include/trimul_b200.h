@@ -430,8 +430,9 @@ typedef struct trimul_attn_desc {
     void*    o_lo;                        /* bf16 only, [B, Lq, H, D] dense: the rounding of o; may be
                                              NULL in forward; backward: what forward wrote, or NULL   */
     void*    dbias;                       /* NULL, or the gradient of the bias, [bias_batch,
-                                             bias_heads, Lq, Lk]; rows start at multiples of 16 bytes
-                                             and their storage reaches to the next multiple behind Lk */
+                                             bias_heads, Lq, Lk], summed in fp32 over what shares it
+                                             and rounded once; rows start at multiples of 16 bytes and
+                                             their storage reaches to the next multiple behind Lk     */
     int64_t  dbias_b, dbias_h, dbias_i;
 } trimul_attn_desc;
 

@@ -198,7 +198,8 @@ def cross_attention_backward_b200(grad: torch.Tensor, q: torch.Tensor, k: torch.
                                   bias_grad: bool = True, plain_kernels: bool = False) -> tuple:
     """``(dq, dk, dv, dbias)`` for the upstream gradient ``grad`` of ``cross_attention_forward_b200``'s result
     with the same arguments; ``dbias`` is None without a bias or with ``bias_grad=False``, and otherwise
-    has the bias's shape (summed over the axes along which it was shared), its rows on 16-byte boundaries.
+    has the bias's shape (summed in fp32 over the axes along which it was shared, rounded once), its rows on
+    16-byte boundaries.
     No atomics: the same call gives the same bits."""
     call = _Call(q, k, v, bias, key_mask, scale, plain_kernels)
     B, Lq, Lk, H, Hk, D = call.sizes

@@ -11,7 +11,7 @@
 // What bounds it (2048 x 4096, 16 query heads on 4 key heads of 128: 243 us, 990 TFLOP/s of the seven products): a step of dq takes
 // 2700 cycles, of which its products, whose operands come from shared memory at 94 cycles per 128 x 128 x 16, take 2000 to 2200;
 // one of dk, dv 3180 with 2050 of products, since exponentials, probabilities' product and ds's product of a tile follow each other.
-// In short loops (4 x 512 x 768, 16 heads of 64: 84 us) the start and the end of a block weigh as much as its steps.
+// In short loops (4 x 512 x 768, 16 heads of 64: 81 us) the start and the end of a block weigh as much as its steps.
 //
 // Both: 384 threads (TMA producer, UMMA issuer, a helper warp, bias producer, two groups of four softmax warps that share
 // a 128 x 128 tile by halves of its columns).  p and ds go back to tensor memory as A operands of the second products,
@@ -597,7 +597,9 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
         const float delta = i < p.Lq ? __ldg(p.delta + srow) : 0.f;
         const float both = -fmaf(ml.x, kLog2e, ml.y);
         constexpr int kVec = 16 / (int)sizeof(Ds);
-        Ds* ds = p.ds != nullptr ? static_cast<Ds*>(p.ds) + b * p.ds_b + h * p.ds_h + i * p.ds_i : nullptr;
+        constexpr bool kParts = sizeof(Ds) == 4;           // ds_parts: 16 bytes are four columns of a row, the next row's after them
+        Ds* ds = p.ds != nullptr ? static_cast<Ds*>(p.ds) + b * p.ds_b + h * p.ds_h + (kParts ? 4ll * i : i * p.ds_i) : nullptr;
+        auto ds_at = [&](int col) { return reinterpret_cast<uint4*>(kParts ? ds + (long long)col * p.Lq : ds + col); };
         bool ok = true;
         int t_next = first > 0 ? tile_at(-1) + 1 : 0;      // first key tile whose ds is not written yet
         auto clear_ds = [&](int t_end) {
@@ -605,7 +607,7 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
                 for (int t = t_next; t < t_end; ++t)
                     for (int e = 0; e < 64; e += kVec)
                         if (t * kAfRows + g * 64 + e < p.Lk)
-                            *reinterpret_cast<uint4*>(ds + t * kAfRows + g * 64 + e) = make_uint4(0u, 0u, 0u, 0u);
+                            *ds_at(t * kAfRows + g * 64 + e) = make_uint4(0u, 0u, 0u, 0u);
             t_next = t_end + 1;
         };
         for (int it = 0; it < n; ++it) {
@@ -666,11 +668,12 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
                     for (int e = 0; e < 64; e += kVec)
                         if (t * kAfRows + g * 64 + e < p.Lk) {
                             if constexpr (sizeof(Ds) == 2)
-                                *reinterpret_cast<uint4*>(ds + t * kAfRows + g * 64 + e) =
+                                *ds_at(t * kAfRows + g * 64 + e) =
                                     make_uint4(pack_bf16x2(x[e], x[e + 1]), pack_bf16x2(x[e + 2], x[e + 3]),
                                                pack_bf16x2(x[e + 4], x[e + 5]), pack_bf16x2(x[e + 6], x[e + 7]));
                             else
-                                *reinterpret_cast<float4*>(ds + t * kAfRows + g * 64 + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                                *ds_at(t * kAfRows + g * 64 + e) = make_uint4(__float_as_uint(x[e]), __float_as_uint(x[e + 1]),
+                                                                              __float_as_uint(x[e + 2]), __float_as_uint(x[e + 3]));
                         }
                 }
             }

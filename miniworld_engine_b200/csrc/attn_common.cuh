@@ -34,7 +34,8 @@ struct AttnParams {
     float* delta;                          // [B][H][Lq]: sum_d dout o
     void* ds;                              // gradient of x, or null: written with the strides below
     long long ds_b, ds_h, ds_i;
-    int ds_wide;                           // ds is fp32 whatever the inputs are: it is going to be summed
+    int ds_parts;                          // it is going to be summed: fp32 whatever the inputs are, for each head in groups of
+                                           // four columns, [column / 4][Lq][4], so that a warp's rows lie side by side
     int32_t* status;
 };
 

@@ -223,13 +223,6 @@ int check_attn(const trimul_attn_desc* d) {
 inline bool sums_bias(const trimul_attn_desc* d) {
     return d->dbias != nullptr && ((d->bias_batch == 1 && d->B > 1) || (d->bias_heads == 1 && d->H > 1));
 }
-// Whether the scores' gradients of a shared bias wait for their sum in fp32 where the inputs are bf16: up to a megabyte of them, where
-// it costs nothing (4 x 1 x 312: 29.0 against 29.2 us for a training pass; 2 x 300 x 400, 8 heads 42.8 against 47.7, 4 x 512 x 768, 16
-// heads 132 against 159) and where a gradient of few elements shows the second rounding most.
-constexpr int64_t kWideDs = 1 << 20;
-bool wide_ds(const trimul_attn_desc* d) {
-    return d->dtype == TRIMUL_DTYPE_BF16 && (int64_t)d->B * d->H * d->Lq * align_up(d->Lk, 8) * 4 <= kWideDs;
-}
 inline AttnTensor tensor_of(const trimul_attn_tensor& t) { return AttnTensor{t.p, t.b, t.l, t.h}; }
 
 AttnParams attn_params(const trimul_attn_desc* d, int32_t* status) {
@@ -408,7 +401,7 @@ AttnWorkspace attn_workspace(const trimul_attn_desc* d, bool backward) {
         at = w.dv + kv;
         w.ds = at;
         w.ds_pitch = align_up(d->Lk, 8);
-        if (sums_bias(d)) at += align_up((int64_t)d->B * d->H * d->Lq * w.ds_pitch * (wide_ds(d) ? 4 : elem_size(d->dtype)), 256);
+        if (sums_bias(d)) at += align_up((int64_t)d->B * d->H * d->Lq * w.ds_pitch * 4, 256);
     }
     w.total = at;
     return w;
@@ -595,7 +588,7 @@ int run_bwd(const trimul_attn_desc* given, const AttnParams& p, const AttnWorksp
         return TRIMUL_E_CUDA;
     m[4] = m[0];
     if (d->bias != nullptr && !encode_bias(&m[4], d)) return TRIMUL_E_CUDA;
-    if (p.ds_wide) return d->D <= 64 ? launch_bwd<64, true, float>(bp, m, st) : launch_bwd<128, true, float>(bp, m, st);
+    if (p.ds_parts) return d->D <= 64 ? launch_bwd<64, true, float>(bp, m, st) : launch_bwd<128, true, float>(bp, m, st);
     if (d->D <= 64) return d->bias != nullptr ? launch_bwd<64, true>(bp, m, st) : launch_bwd<64, false>(bp, m, st);
     return d->bias != nullptr ? launch_bwd<128, true>(bp, m, st) : launch_bwd<128, false>(bp, m, st);
 }
@@ -695,8 +688,8 @@ int trimul_b200_attn_backward(const trimul_attn_desc* d, void* workspace, size_t
     if (d->dbias != nullptr) {
         if (sums_bias(d)) {
             p.ds = ws + w.ds;
-            p.ds_wide = wide_ds(d);
-            p.ds_i = w.ds_pitch; p.ds_h = w.ds_pitch * d->Lq; p.ds_b = p.ds_h * d->H;
+            p.ds_parts = 1;
+            p.ds_h = w.ds_pitch * d->Lq; p.ds_b = p.ds_h * d->H;
         } else {
             p.ds = d->dbias;
             p.ds_i = d->dbias_i; p.ds_h = d->bias_heads == 1 ? 0 : d->dbias_h; p.ds_b = d->bias_batch == 1 ? 0 : d->dbias_b;
@@ -718,17 +711,15 @@ int trimul_b200_attn_backward(const trimul_attn_desc* d, void* workspace, size_t
     if (rc == TRIMUL_OK) rc = bf16 ? run_join<__nv_bfloat16>(p, split, st) : run_join<float>(p, split, st);
     if (rc != TRIMUL_OK || !sums_bias(d)) return rc;
     const int n = 16 / elem_size(d->dtype);
-    const int64_t items = (int64_t)d->bias_batch * d->bias_heads * d->Lq * ceil_div(d->Lk, n);
-    const dim3 sgrid((unsigned)std::min<int64_t>(ceil_div(items, kApThreads), 16 * (int64_t)sm_count()));
+    const int64_t tiles = (int64_t)d->bias_batch * d->bias_heads * ceil_div(d->Lq, kApSumRows) * ceil_div(d->Lk, kApSumChunks * n);
+    const dim3 sgrid((unsigned)std::min<int64_t>(tiles, 16 * (int64_t)sm_count()));
     const int sum_b = d->bias_batch == 1, sum_h = d->bias_heads == 1;
-    auto sum = [&](auto kernel, auto* ds, auto* out) {
-        return launch_stage(kernel, sgrid, kApThreads, 0, st, true, ds, p.ds_b, p.ds_h, p.ds_i, out, (long long)d->dbias_b,
+    auto sum = [&](auto kernel, auto* out) {
+        return launch_stage(kernel, sgrid, kApThreads, 0, st, true, static_cast<const float*>(p.ds), p.ds_b, p.ds_h, out, (long long)d->dbias_b,
                             (long long)d->dbias_h, (long long)d->dbias_i, d->B, d->H, d->Lq, d->Lk, sum_b, sum_h);
     };
-    using bf = __nv_bfloat16;
-    if (!bf16) return sum(attn_bias_sum_kernel<float, float>, static_cast<const float*>(p.ds), static_cast<float*>(d->dbias));
-    if (p.ds_wide) return sum(attn_bias_sum_kernel<bf, float>, static_cast<const float*>(p.ds), static_cast<bf*>(d->dbias));
-    return sum(attn_bias_sum_kernel<bf, bf>, static_cast<const bf*>(p.ds), static_cast<bf*>(d->dbias));
+    return bf16 ? sum(attn_bias_sum_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(d->dbias))
+                : sum(attn_bias_sum_kernel<float>, static_cast<float*>(d->dbias));
 }
 
 }  // extern "C"

@@ -368,3 +368,37 @@ def test_shared_bias_gradient_of_a_small_call_is_rounded_once(Lq, D):
     delta = (g * o).sum(-1, keepdim=True)
     want, size = (p * (dp - delta)).sum(0), (p * (dp.abs() + delta.abs())).sum(0)
     assert (((got - want).abs() - 2.0 ** -8 * want.abs()) <= 2.0 ** -12 * size).all()
+
+
+@pytest.mark.parametrize("plain", [False, True])
+@pytest.mark.parametrize("B,H,Lq,Lk,D,bias", [(4, 8, 300, 400, 64, "1H"), (2, 4, 270, 514, 128, "B1"), (3, 5, 400, 333, 32, "11")])
+def test_shared_bias_gradient_of_a_large_call_is_rounded_once(B, H, Lq, Lk, D, bias, plain):
+    """As for small calls, with summands that nearly cancel: batch elements (heads) come in pairs of the same inputs, the
+    second one's upstream gradient minus 0.9 times the first one's.  Bounds as there; half a step of every summand would be
+    up to 2^-8 of 1.9 |ds| against a sum of 0.1 |ds|."""
+    from miniworld_engine_b200 import cross_attention_backward_b200, cross_attention_forward_b200
+    q, k, v, g, b, _ = _inputs(B, Lq, Lk, H, H, D, bias, None, BF16, seed=B)
+    for t in (q, k, v):
+        if bias != "B1":
+            t[1] = t[0]
+        else:
+            t[:, :, 1] = t[:, :, 0]
+    if bias != "B1":
+        g[1] = -0.9 * g[0]
+        g[2:] *= 0.01                        # and little beside the pair
+    else:
+        g[:, :, 1] = -0.9 * g[:, :, 0]
+        g[:, :, 2:] *= 0.01
+    out, state = cross_attention_forward_b200(q, k, v, bias=b, plain_kernels=plain)
+    got = cross_attention_backward_b200(g, q, k, v, out, state, bias=b, plain_kernels=plain)[3].double()
+    o = out.double() + state.rounding.double()
+    q, k, v, g, o = (t.double().transpose(1, 2) for t in (q, k, v, g, o))
+    p = (q @ k.mT * D ** -0.5 + b.double()).softmax(-1)
+    dp = g @ v.mT
+    delta = (g * o).sum(-1, keepdim=True)
+    want, size = p * (dp - delta), p * (dp.abs() + delta.abs())
+    for axis in (0, 1):
+        if b.shape[axis] == 1:
+            want, size = want.sum(axis, keepdim=True), size.sum(axis, keepdim=True)
+    assert got.shape == want.shape
+    assert (((got - want).abs() - 2.0 ** -8 * want.abs()) <= 2.0 ** -12 * size).all()
