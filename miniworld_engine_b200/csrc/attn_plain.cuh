@@ -286,8 +286,7 @@ struct ApStats {
         for (int r = 0; r < kR; ++r)
 #pragma unroll
             for (int c = 0; c < kR; ++c) {
-                // a masked pair has none, also in a row whose statistics are NaN
-                const float e = s[r][c] == -INFINITY ? 0.f : exp2f(fmaf(s[r][c] - st[r].x, kLog2e, -st[r].y));
+                const float e = exp2f(fmaf(s[r][c] - st[r].x, kLog2e, -st[r].y));
                 s[r][c] = e;
                 g[r][c] = e == 0.f ? 0.f : e * (g[r][c] - delta[r]);
             }
@@ -349,8 +348,9 @@ __device__ __forceinline__ void ap_dq_block(const AttnParams& p, const AttnBwdSp
                 P[(ty * kR + r) * pp + tx + 16 * c] = g[r][c];
                 if (p.ds != nullptr && i < p.Lq && j < p.Lk) {
                     const long long head = b * p.ds_b + h * p.ds_h;
-                    if (p.ds_parts) static_cast<float*>(p.ds)[head + ((long long)(j >> 2) * p.Lq + i) * 4 + (j & 3)] = g[r][c];
-                    else at_store(static_cast<T*>(p.ds) + head + i * p.ds_i + j, g[r][c]);
+                    const float ds = bias.kept[c] ? g[r][c] : 0.f;         // zero also in a row whose statistics are NaN
+                    if (p.ds_parts) static_cast<float*>(p.ds)[head + ((long long)(j >> 2) * p.Lq + i) * 4 + (j & 3)] = ds;
+                    else at_store(static_cast<T*>(p.ds) + head + i * p.ds_i + j, ds);
                 }
             }
         }
