@@ -81,6 +81,8 @@ class PositionBuckets:
             want = near ** (shared - k) * max_distance ** k
             while t ** shared < want:
                 t += 1
+                if t > _lib.MAX_LUT:
+                    raise NotImplementedError(f"distances beyond {_lib.MAX_LUT} must share a bucket")
             thresholds.append(t)
         kind = _lib.BUCKETS_LOG if bidirectional else _lib.BUCKETS_CAUSAL
         return PositionBuckets(kind, num_buckets, max_distance, tuple(thresholds), segments)

@@ -301,3 +301,22 @@ def test_forward_mode_tangents_are_refused(no_grad):
         torch.func.jvp(lambda x: attend(x, k, k), (q,), (q,))
     with pytest.raises(RuntimeError, match="no CPU path"):
         attend(q, k, k)
+
+
+@pytest.mark.parametrize("count,top", [(32, 10 ** 9), (32, 10 ** 15), (4, 10 ** 18), (64, 2 ** 62)])
+@pytest.mark.parametrize("bidirectional", [False, True])
+def test_far_distances_are_refused_at_once(count, top, bidirectional):
+    """A border beyond the look-up table is refused without counting up to it."""
+    import signal
+
+    def late(signum, frame):
+        raise TimeoutError("still counting")
+
+    before = signal.signal(signal.SIGALRM, late)
+    signal.setitimer(signal.ITIMER_REAL, 10)
+    try:
+        with pytest.raises(NotImplementedError, match="must share a bucket"):
+            PositionBuckets.logarithmic(count, top, bidirectional=bidirectional)
+    finally:
+        signal.setitimer(signal.ITIMER_REAL, 0)
+        signal.signal(signal.SIGALRM, before)
