@@ -264,7 +264,8 @@ def relative_position_bias_backward_b200(grad: torch.Tensor, buckets: PositionBu
 class _RelativePositionBias(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, add, buckets, q_pos, k_pos, q_segment, k_segment, layout, dtype):
-        ctx.save_for_backward(q_pos, k_pos, q_segment, k_segment)
+        # positions given twice are saved once: saved-tensor hooks may hand the backward pass two objects for them
+        ctx.save_for_backward(q_pos, None if k_pos is q_pos else k_pos, q_segment, k_segment)
         ctx.buckets, ctx.layout, ctx.table_dtype = buckets, layout, table.dtype
         return _forward(table, buckets, q_pos, k_pos, q_segment, k_segment, layout, add, dtype)
 

@@ -320,3 +320,25 @@ def test_far_distances_are_refused_at_once(count, top, bidirectional):
     finally:
         signal.setitimer(signal.ITIMER_REAL, 0)
         signal.signal(signal.SIGALRM, before)
+
+
+@pytest.mark.parametrize("same", [False, True])
+def test_positions_that_come_back_as_another_object(monkeypatch, same):
+    """Saved-tensor hooks (checkpointing, offload) hand the backward pass copies: positions given once as queries' and keys'
+    are still one set of positions there."""
+    from miniworld_engine_b200 import relpos
+    buckets, pos, seg = PositionBuckets.clipped(4, segments=True), torch.arange(5), torch.zeros(5, dtype=torch.int32)
+    seen = []
+
+    def backward(grad, rule, q_pos, k_pos=None, *, q_segment, k_segment, layout, dtype):
+        call = relpos._Call(rule, q_pos, k_pos, q_segment, k_segment, layout, 1, 1, 4, q_pos.device)
+        seen.append((call.lq, call.lk, call.keep[1] is call.keep[0], call.keep[3] is call.keep[2]))
+        return torch.zeros(10, 4)
+
+    monkeypatch.setattr(relpos, "_forward", lambda table, *args: torch.zeros(4, 5, 5))
+    monkeypatch.setattr(relpos, "relative_position_bias_backward_b200", backward)
+    table = torch.zeros(10, 4, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t):
+        out = relative_position_bias_b200(table, buckets, pos, pos if same else None, q_segment=seg)
+    out.sum().backward()
+    assert seen == [(5, 5, True, True)]
