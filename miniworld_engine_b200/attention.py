@@ -8,7 +8,6 @@ the state between them themselves (a captured training step, a framework without
 from __future__ import annotations
 
 import ctypes as C
-import math
 from typing import NamedTuple
 
 import torch
@@ -45,6 +44,7 @@ def _laid_out(t: torch.Tensor, tensor_cores: bool) -> torch.Tensor:
 
 
 _NONE = (0, 0, 0, 0)
+_MAX_SCALE = torch.finfo(torch.float32).max
 _workspace_sizes: dict = {}      # of the library's answers, by what they depend on
 
 
@@ -84,8 +84,8 @@ class _Call:
         self.sizes = (B, Lq, Lk, H, Hk, D)
         self.empty = B == 0 or Lq == 0 or H == 0
         scale = D ** -0.5 if scale is None else float(scale)
-        if not math.isfinite(scale):
-            raise ValueError(f"scale must be finite, got {scale}")
+        if not abs(scale) <= _MAX_SCALE:
+            raise ValueError(f"scale must be finite (in 32 bits), got {scale}")
         flags = _lib.ATTN_FLAG_PLAIN if plain_kernels else 0
         self.bias = self.bias_shape = self.mask = None
         self.bias_args, self.mask_args = (0, 0, 0, 0, 0, 0), (0, 0)

@@ -342,3 +342,15 @@ def test_positions_that_come_back_as_another_object(monkeypatch, same):
         out = relative_position_bias_b200(table, buckets, pos, pos if same else None, q_segment=seg)
     out.sum().backward()
     assert seen == [(5, 5, True, True)]
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e300, 3.5e38])
+def test_scales_beyond_32_bits_are_refused(monkeypatch, scale):
+    from miniworld_engine_b200 import attention
+    monkeypatch.setattr(attention, "_require_cuda", lambda t, name: None)
+    q, k = torch.zeros(2, 3, 4, 8), torch.zeros(2, 5, 2, 8)
+    with pytest.raises(ValueError, match="scale must be finite"):
+        cross_attention_b200(q, k, k, scale=scale)
+    with pytest.raises(ValueError, match="scale must be finite"):
+        cross_attention_b200(q[:0], k[:0], k[:0], scale=scale)          # also where nothing is computed
+    assert attention._Call(q, k, k, None, None, torch.finfo(torch.float32).max, False).pack((0, 0, 0, 0), 0, 0)
