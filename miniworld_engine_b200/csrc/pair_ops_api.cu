@@ -329,8 +329,11 @@ int plain_splits(const trimul_attn_desc* d) {
 // block slot's share of all steps: few queries against many keys leave dq to a few long loops, many queries against few keys dk and dv.
 // Tensor cores, 8 heads, us whole / split: 61 x 4096 of 64 41 / 20, of 128 46 / 29, 100 x 1024 of 64 13.8 / 10.8, 2048 x 100 of
 // 128 37 / 22; a loop just over twice the share (700 x 1400, 4 heads of 128) 21.6 / 24.2, hence `margin`; shares of four steps at
-// least instead of two 100 x 1024 12.2, 2048 x 100 25.1.  CUDA cores, where a step takes longer and two blocks fit on an SM: 2 x
-// 60 x 1000, 4 heads of 96 208 / 75, 500 x 60, 4 heads of 64 128 / 25, 188 x 169, 8 heads of 128 69 / 59.
+// least instead of two 100 x 1024 12.2, 2048 x 100 25.1.  CUDA cores: 2 x 60 x 1000, 4 heads of 96 208 / 75, 500 x 60, 4 heads of
+// 64 128 / 25, 188 x 169, 8 heads of 128 69 / 59.  There, too, one block fits on an SM (156 to 255 registers of 256 threads), but a
+// step takes longer, so the shares are half an SM's and the last blocks end closer together.  A training pass in fp32 by half / whole
+// shares: 1030 x 1700, a head of 40 152 / 182, 300 x 300, 8 heads of 64 109 / 131, 188 x 169, 8 heads of 128 115 / 125; the other way
+// round 4 x 100 x 100, 8 heads of 64 86 / 80, 3 x 333 x 77, 4 heads of 24 51 / 49; no difference at 2 x 512 x 1024, 8 heads of 64.
 AttnBwdSplit backward_split(const trimul_attn_desc* d, int rows, int least, int margin, int slots) {
     const int64_t nq = ceil_div(d->Lq, rows), nk = ceil_div(d->Lk, rows), q = nq * d->H * d->B, kv = nk * d->Hk * d->B;
     const int64_t kv_loop = nq * (d->H / d->Hk), share = std::max<int64_t>(least, ceil_div(q * nk + kv * kv_loop, slots));
