@@ -277,3 +277,31 @@ def test_segments_are_told_apart_whatever_their_numbers(layout, channels, q_type
     sums = torch.zeros(10, channels, dtype=torch.float64, device="cuda").index_add_(0, u.flatten(), flat)
     got = relative_position_bias_backward_b200(g, buckets, q.cuda(), k.cuda(), **kw)
     assert torch.equal(got.double(), sums)
+
+
+@pytest.mark.parametrize("layout,channels", [("heads", 1), ("heads", 2), ("heads", 16), ("pair", 128), ("pair", 5)])
+@pytest.mark.parametrize("rule", ["clip32", "log32", "clip300"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("chains", [False, True])
+def test_runs_of_one_bucket_add_up_exactly(layout, channels, rule, dtype, chains):
+    """Residue numbers in order: most of a row shares a bucket, whose elements are summed in registers.  Upstream values of
+    1 to 3 make every sum a whole number below 3 * 1100^2 < 2^24, exact in fp32 in any order; an element left out or taken
+    twice shows."""
+    from miniworld_engine_b200 import relative_position_bias_backward_b200
+    n = 1100 if layout == "heads" else 420
+    i = torch.arange(n, device="cuda", dtype=torch.int32)
+    pos, seg = i - (i >= 400).int() * 400, (i >= 400).int() + (i >= 405).int()
+    kw = {"q_segment": seg} if chains else {}
+    kind, count, top = RULES[rule]
+    u = bucket_matrix(pos, pos, kind, count, top, seg if chains else None, seg if chains else None).cuda()
+    buckets = _rule(rule, chains)
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    g = torch.randint(1, 4, (n, n, channels), generator=gen, device="cuda").to(dtype)
+    want = torch.zeros(buckets.rows, channels, dtype=torch.float64, device="cuda")
+    want.index_add_(0, u.flatten(), g.reshape(-1, channels).double())
+    # the fullest bucket is full: at least the 120 * 121 / 2 = 7260 pairs of 420 that lie 300 or more apart, of mean 2
+    assert want.max() > 7260 and want.max() < 2 ** 24
+    g = g if layout == "pair" else g.movedim(-1, 0)
+    for grad in (g, g.contiguous()):
+        got = relative_position_bias_backward_b200(grad, buckets, pos, layout=layout, **kw)
+        assert torch.equal(got.double(), want)
