@@ -267,7 +267,9 @@ def cross_attention_b200(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, b
     A row without a kept key gives zeros (and zero gradients); a row whose scores hold a NaN gives NaN.
 
     bf16 with ``D`` a multiple of 8 up to 128 runs on the tensor cores, everything else (and
-    ``plain_kernels=True``) on the CUDA cores in fp32 arithmetic.  Differentiable in ``q``, ``k``, ``v`` and
+    ``plain_kernels=True``) on the CUDA cores in fp32 arithmetic.  The tensor-core kernels round the probabilities, and
+    in the backward pass the scores' gradients, to bf16 on their way into a product (half a step each, beside the
+    rounding of the result); ``plain_kernels=True`` keeps them in fp32.  Differentiable in ``q``, ``k``, ``v`` and
     ``bias``, in reverse mode; an input with a forward-mode tangent is refused."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
         return _CrossAttention.apply(q, k, v, bias, key_mask, scale, plain_kernels)

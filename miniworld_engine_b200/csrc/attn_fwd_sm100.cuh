@@ -18,7 +18,8 @@
 // P is handed over in halves of 64 keys, so that its product starts while the rest is exponentiated.
 // What bounds it: softmax, product and next scores of a query tile wait for each other (3500 cycles a round for both tiles, of
 // which the tensor cores work 2100 and the exponentials 2048), and blocks of 256 queries: 4096 x 8192 with 16 heads of 128 is
-// 256 blocks for 148 SMs.  1058 TFLOP/s there (0.64 of the measured GEMM rate).  Softmax by two warps per row (each half the keys) measured the same.
+// 256 blocks for 148 SMs.  268 us there in a call by itself, 1026 TFLOP/s (0.62 of the measured GEMM rate); 281 in a row of calls.
+// Softmax by two warps per row (each half the keys) measured the same.
 // Head dimensions below 128 are filled with zeros by the TMA loads.
 #pragma once
 

@@ -307,7 +307,8 @@ relpos_heads_grad_kernel(const __grid_constant__ RelposParams p, const __grid_co
     const int ty = tid / tpr, tx = tid % tpr;
     const int b = blockIdx.x / parts_per_b;
     // row r of the part is query first + r parts_per_b: near pairs, whose pieces have several buckets and cost most, then come
-    // to all threads alike as r goes on (with consecutive rows a few warps had them all: 64 us instead of 38 for 134 MB)
+    // to all threads alike as r goes on (with consecutive rows a few warps had them all: 95 us instead of 82 for forward and
+    // gradient of 16 x 2048^2 with logarithmic buckets, 111 instead of 88 with 65 clipped ones)
     const int first = blockIdx.x - b * parts_per_b, r1 = (p.Lq - first + parts_per_b - 1) / parts_per_b;
     const long long row_stride = p.sI * parts_per_b;
     const T* gb = grad + b * p.sB + h0 * p.sH + first * p.sI;
