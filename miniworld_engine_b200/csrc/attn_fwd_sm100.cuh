@@ -5,7 +5,10 @@
 // tensor memory, P goes back to tensor memory as the A operand of the second product and never touches shared memory.
 // A block owns two tiles of 128 queries of one head.  While the softmax warps of one tile exponentiate, the tensor cores
 // work for the other.  384 threads:
-//   warp 0      TMA producer: queries once, then key and value tiles of 128 rows through one ring of slots
+//   warp 0      TMA producer: queries once, then key and value tiles of 128 rows through one ring of slots.  What tells that a
+//               tile has come belongs to the tile, not to its slot: the ring is odd, so a slot holds keys and values in turn,
+//               and a warp that waits for the values alone would miss a phase of a slot's barrier.  Where the key tile before
+//               them came late, it would take the open phase's predecessor for the one that it waits for
 //   warp 1      UMMA issuer (a second one, a warp per query tile, made it 15 % slower)
 //   warp 2      with a key mask: zeroes the value rows of masked keys in shared memory, whose probabilities are zero but
 //               which may hold infinities or NaN
@@ -30,7 +33,7 @@ namespace trimul {
 constexpr int kAfThreads = 384;
 constexpr int kAfRows = 128;                     // rows of a query or key tile
 constexpr int kAfSub = 128 * 128;                // 128 rows x 64 bf16, swizzled
-constexpr int kAfClean = 4;                      // at least the value tiles that the ring holds at once
+constexpr int kAfClean = 4;                      // at least the key (the value) tiles that the ring holds at once
 constexpr int kStageIdAttnFwd = 11;
 constexpr int kAfD = 128;                        // columns of head dimension
 constexpr float kAfSlack = 8.f;                  // log2 of what a row's maximum may grow without a rescale
@@ -44,7 +47,7 @@ struct AfLayout {
     static constexpr int kOffRing = kOffBias + (kBias ? 2 * 2 * kAfSub : 0);
     static constexpr int kOffBars = kOffRing + kStages * kTile;
     static constexpr int kSmem = kOffBars + 256;
-    static_assert((14 + 2 * kStages + kAfClean) * 8 + 8 <= 256, "barriers");
+    static_assert((14 + kStages + 3 * kAfClean) * 8 + 8 <= 256, "barriers");
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -88,9 +91,10 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     uint64_t* o_full = p_full + 4;             // [2] last product complete
     uint64_t* b_full = o_full + 2;             // [2]
     uint64_t* b_empty = b_full + 2;            // [2]
-    uint64_t* full = b_empty + 2;        // [kSt]
-    uint64_t* empty = full + kSt;              // [kSt]
-    uint64_t* v_ok = empty + kSt;              // [kAfClean] masked value rows zeroed, value tile j at j % kAfClean
+    uint64_t* empty = b_empty + 2;             // [kSt]
+    uint64_t* k_full = empty + kSt;            // [kAfClean] key tile j at j % kAfClean, and so
+    uint64_t* v_full = k_full + kAfClean;      // [kAfClean] value tile j
+    uint64_t* v_ok = v_full + kAfClean;        // [kAfClean] its masked rows zeroed
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_ok + kAfClean);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -111,11 +115,12 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             mbar_init(&b_full[s], 1);
             mbar_init(&b_empty[s], 4);
         }
-        for (int s = 0; s < kSt; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+        for (int s = 0; s < kSt; ++s) mbar_init(&empty[s], 1);
+        for (int s = 0; s < kAfClean; ++s) {
+            mbar_init(&k_full[s], 1);
+            mbar_init(&v_full[s], 1);
+            mbar_init(&v_ok[s], 1);
         }
-        for (int s = 0; s < kAfClean; ++s) mbar_init(&v_ok[s], 1);
         *abort_flag = 0;
         fence_mbarrier_init();
         tma_prefetch_desc(&tmQ);
@@ -153,11 +158,12 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             for (int it = 0; it < 2 * n; ++it) {
                 const int s = it % kSt;
                 if (!mbar_wait<true>(&empty[s], ((it / kSt) & 1) ^ 1, abort_flag, p.status, kStageIdAttnFwd, 100 + s)) break;
-                mbar_arrive_expect_tx(&full[s], L::kTile);
+                uint64_t* full = ((it & 1) ? v_full : k_full) + (it >> 1) % kAfClean;
+                mbar_arrive_expect_tx(full, L::kTile);
                 const int j0 = tile_at(it >> 1) * kAfRows;
 #pragma unroll
                 for (int u = 0; u < kD / 64; ++u)
-                    tma_load_4d(ring + s * L::kTile + u * kAfSub, (it & 1) ? &tmV : &tmK, &full[s], u * 64, j0, hk, b);
+                    tma_load_4d(ring + s * L::kTile + u * kAfSub, (it & 1) ? &tmV : &tmK, full, u * 64, j0, hk, b);
                 if (it == 0 && two) load_q(1);
             }
         }
@@ -193,21 +199,20 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             };
             // ring position of the key tile that is next, and of the value tile
             int sk = 0, sv = 1 % kSt;
-            uint32_t phk = 0, phv = 0;
-            auto step = [&](int& slot, uint32_t& ph) {
+            auto step = [&](int& slot) {
                 slot += 2;
-                if (slot >= kSt) { slot -= kSt; ph ^= 1u; }
+                if (slot >= kSt) slot -= kSt;
             };
-            if (wait(&full[0], 0, 300)) {
+            if (wait(&k_full[0], 0, 300)) {
                 for (int w = 0; ok && w < tiles; ++w)
                     if (wait(&q_full[w], 0, 310 + w)) scores(w, 0);
                 umma_commit_warp(&empty[0]);
             }
-            step(sk, phk);
+            step(sk);
+            uint64_t* v_ready = fp.words != nullptr ? v_ok : v_full;
             for (int j = 0; ok && j < n; ++j) {
                 const bool more = j + 1 < n;
-                if (fp.words != nullptr) wait(&v_ok[j % kAfClean], (j / kAfClean) & 1, 320);
-                else wait(&full[sv], phv, 321);
+                wait(&v_ready[j % kAfClean], (j / kAfClean) & 1, 320);
                 for (int w = 0; ok && w < tiles; ++w) {
                     for (int half = 0; half < 2; ++half)
                         if (wait(&p_full[2 * w + half], j & 1, 330 + w)) mix(w, sv, half, j > 0);
@@ -215,13 +220,13 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
                     if (!more) umma_commit_warp(&o_full[w]);
                     if (w == tiles - 1) umma_commit_warp(&empty[sv]);
                     if (more) {
-                        if (w == 0 && !wait(&full[sk], phk, 340)) break;
+                        if (w == 0 && !wait(&k_full[(j + 1) % kAfClean], ((j + 1) / kAfClean) & 1, 340)) break;
                         scores(w, sk);
                         if (w == tiles - 1) umma_commit_warp(&empty[sk]);
                     }
                 }
-                step(sk, phk);
-                step(sv, phv);
+                step(sk);
+                step(sv);
             }
         }
     } else if (warp == 2) {
@@ -229,7 +234,7 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             for (int j = 0; j < n; ++j) {
                 const int s = (2 * j + 1) % kSt, t = tile_at(j);
                 const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(fp.words) + (long long)b * fp.n_tiles + t);
-                if (!warp_wait(&full[s], ((2 * j + 1) / kSt) & 1, lane, abort_flag, p.status, kStageIdAttnFwd, 500 + s)) break;
+                if (!warp_wait(&v_full[j % kAfClean], (j / kAfClean) & 1, lane, abort_flag, p.status, kStageIdAttnFwd, 500 + s)) break;
                 if ((w4.x & w4.y & w4.z & w4.w) != 0xffffffffu) {
                     const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
                     uint8_t* v = ring + s * L::kTile;

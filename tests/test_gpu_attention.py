@@ -402,3 +402,27 @@ def test_shared_bias_gradient_of_a_large_call_is_rounded_once(B, H, Lq, Lk, D, b
             want, size = want.sum(axis, keepdim=True), size.sum(axis, keepdim=True)
     assert got.shape == want.shape
     assert (((got - want).abs() - 2.0 ** -8 * want.abs()) <= 2.0 ** -12 * size).all()
+
+
+@pytest.mark.parametrize("D", [128, 96, 64])
+@pytest.mark.parametrize("bias", [None, "11"])
+def test_first_calls_on_cold_inputs(D, bias):
+    """Keys and values that come late and in any order: fresh inputs, nothing of them in the L2, a mask with holes or a
+    tail.  The call is right, and the same bits come again when the inputs are warm."""
+    from miniworld_engine_b200 import cross_attention_b200, read_status
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    r = lambda *s: torch.randn(s, generator=gen, device="cuda").bfloat16()
+    for step in range(40):
+        Lq = (5, 129, 300)[step % 3]
+        q, k, v = r(5, Lq, 4, D), r(5, 4100, 4, D), r(5, 4100, 4, D)
+        b = None if bias is None else r(1, 1, Lq, 4100)
+        m = (torch.rand(5, 4100, generator=gen, device="cuda") > 0.4 if step % 2 else
+             torch.arange(4100, device="cuda")[None] < torch.randint(1, 4101, (5, 1), generator=gen, device="cuda"))
+        flush.zero_()
+        first = cross_attention_b200(q, k, v, bias=b, key_mask=m)
+        again = cross_attention_b200(q, k, v, bias=b, key_mask=m)
+        assert torch.equal(first, again), step
+        if step < 6:
+            check(first, attention64(q, k, v, b, m)["out"], "out")
+    assert read_status()[0] == 0
