@@ -224,7 +224,7 @@ __device__ __forceinline__ void attn_dkv_block(const CUtensorMap& tmQ, const CUt
     griddep_wait();
     griddep_launch_dependents();
 
-    const uint4 w4 = bp.words != nullptr ? __ldg(reinterpret_cast<const uint4*>(bp.words) + (long long)b * bp.n_tiles + tile)
+    const uint4 w4 = bp.words != nullptr ? at_load(reinterpret_cast<const uint4*>(bp.words) + (long long)b * bp.n_tiles + tile)
                                          : make_uint4(~0u, ~0u, ~0u, ~0u);
     const int first = split * bp.w.kv_share;             // of the query tiles, head after head
     const int n = warp_uniform((w4.x | w4.y | w4.z | w4.w) != 0u ? max(0, min(bp.w.kv_share, group * nq - first)) : 0);
@@ -300,8 +300,8 @@ __device__ __forceinline__ void attn_dkv_block(const CUtensorMap& tmQ, const CUt
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = i0 + 32 * e + lane;
-                ml[e] = i < p.Lq ? __ldg(p.stats + base + i) : make_float2(0.f, INFINITY);
-                dl[e] = i < p.Lq ? __ldg(p.delta + base + i) : 0.f;
+                ml[e] = i < p.Lq ? at_load(p.stats + base + i) : make_float2(0.f, INFINITY);
+                dl[e] = i < p.Lq ? at_load(p.delta + base + i) : 0.f;
             }
             if (!warp_wait(&st_empty[s], ((it / L::kStats) & 1) ^ 1, lane, abort_flag, p.status, kStageIdAttnDkv, 500 + s)) break;
             float* d = stat + s * 384 + lane;
@@ -501,7 +501,7 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
     // of the listed key tiles a block takes its share
     const int listed = warp_uniform(list != nullptr ? list[0] : bp.n_tiles), share = (listed + bp.w.q_splits - 1) / bp.w.q_splits;
     const int first = min(split * share, listed), n = min(share, listed - first);
-    auto tile_at = [&](int it) { return list != nullptr ? __ldg(list + 1 + first + it) : first + it; };
+    auto tile_at = [&](int it) { return list != nullptr ? at_load(list + 1 + first + it) : first + it; };
 
     if (warp == 0) {
         if (lane == 0 && n > 0) {
@@ -557,7 +557,7 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
         if (bp.words != nullptr) {
             for (int it = 0; it < n; ++it) {
                 const int s = it % kKSt, t = tile_at(it);
-                const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(bp.words) + (long long)b * bp.n_tiles + t);
+                const uint4 w4 = at_load(reinterpret_cast<const uint4*>(bp.words) + (long long)b * bp.n_tiles + t);
                 if (!warp_wait(&k_full[s], (it / kKSt) & 1, lane, abort_flag, p.status, kStageIdAttnDq, 500 + s)) break;
                 if ((w4.x & w4.y & w4.z & w4.w) != 0xffffffffu) {
                     const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
@@ -593,8 +593,8 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
         const uint32_t lane_off = (uint32_t)(q * 32) << 16;
         const float c2 = p.scale * kLog2e;
         const long long srow = ((long long)b * p.H + h) * p.Lq + i;
-        const float2 ml = i < p.Lq ? __ldg(p.stats + srow) : make_float2(0.f, INFINITY);
-        const float delta = i < p.Lq ? __ldg(p.delta + srow) : 0.f;
+        const float2 ml = i < p.Lq ? at_load(p.stats + srow) : make_float2(0.f, INFINITY);
+        const float delta = i < p.Lq ? at_load(p.delta + srow) : 0.f;
         const float both = -fmaf(ml.x, kLog2e, ml.y);
         constexpr int kVec = 16 / (int)sizeof(Ds);
         constexpr bool kParts = sizeof(Ds) == 4;           // ds_parts: 16 bytes are four columns of a row, the next row's after them
@@ -613,7 +613,7 @@ __device__ __forceinline__ void attn_dq_block(const CUtensorMap& tmQ, const CUte
         for (int it = 0; it < n; ++it) {
             const int t = tile_at(it);
             uint4 w4 = make_uint4(~0u, ~0u, ~0u, ~0u);
-            if (bp.words != nullptr) w4 = __ldg(reinterpret_cast<const uint4*>(bp.words) + (long long)b * bp.n_tiles + t);
+            if (bp.words != nullptr) w4 = at_load(reinterpret_cast<const uint4*>(bp.words) + (long long)b * bp.n_tiles + t);
             else if ((t + 1) * kAfRows > p.Lk) w4 = tail_words(p.Lk - t * kAfRows);
             const uint32_t w[2] = {g == 0 ? w4.x : w4.z, g == 0 ? w4.y : w4.w};
             if (!(ok = warp_wait(s_full, it & 1, lane, abort_flag, p.status, kStageIdAttnDq, 400))) break;

@@ -114,7 +114,7 @@ attn_fwd64_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     const int kept = warp_uniform(list != nullptr ? list[0] : fp.n_tiles);
     const int t_first = split * fp.tiles_per_split;
     const int n = max(0, min(fp.tiles_per_split, kept - t_first));
-    auto tile_at = [&](int j) { return list != nullptr ? __ldg(list + 1 + t_first + j) : t_first + j; };
+    auto tile_at = [&](int j) { return list != nullptr ? at_load(list + 1 + t_first + j) : t_first + j; };
 
     if (warp == 0) {
         if (lane == 0 && n > 0) {
@@ -207,7 +207,7 @@ attn_fwd64_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         if (fp.words != nullptr) {
             for (int j = 0; j < n; ++j) {
                 const int s = (2 * j + 1) % kSt, t = tile_at(j);
-                const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(fp.words) + (long long)b * fp.n_tiles + t);
+                const uint4 w4 = at_load(reinterpret_cast<const uint4*>(fp.words) + (long long)b * fp.n_tiles + t);
                 if (!warp_wait(&full[s], ((2 * j + 1) / kSt) & 1, lane, abort_flag, p.status, kStageIdAttnFwd64, 500 + s)) break;
                 if ((w4.x & w4.y & w4.z & w4.w) != 0xffffffffu) {
                     const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
@@ -240,7 +240,7 @@ attn_fwd64_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 const int t = tile_at(j);
                 uint32_t keep[2] = {~0u, ~0u};
                 if (fp.words != nullptr) {
-                    const uint2 w2 = __ldg(reinterpret_cast<const uint2*>(fp.words) + ((long long)b * fp.n_tiles + t) * 2 + half);
+                    const uint2 w2 = at_load(reinterpret_cast<const uint2*>(fp.words) + ((long long)b * fp.n_tiles + t) * 2 + half);
                     keep[0] = w2.x;
                     keep[1] = w2.y;
                 } else if ((t + 1) * kAfRows > p.Lk) {

@@ -144,7 +144,7 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     const int kept = warp_uniform(list != nullptr ? list[0] : fp.n_tiles);
     const int t_first = split * fp.tiles_per_split;
     const int n = max(0, min(fp.tiles_per_split, kept - t_first));
-    auto tile_at = [&](int j) { return list != nullptr ? __ldg(list + 1 + t_first + j) : t_first + j; };
+    auto tile_at = [&](int j) { return list != nullptr ? at_load(list + 1 + t_first + j) : t_first + j; };
 
     if (warp == 0) {
         if (lane == 0 && n > 0) {
@@ -233,7 +233,7 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         if (fp.words != nullptr) {
             for (int j = 0; j < n; ++j) {
                 const int s = (2 * j + 1) % kSt, t = tile_at(j);
-                const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(fp.words) + (long long)b * fp.n_tiles + t);
+                const uint4 w4 = at_load(reinterpret_cast<const uint4*>(fp.words) + (long long)b * fp.n_tiles + t);
                 if (!warp_wait(&v_full[j % kAfClean], (j / kAfClean) & 1, lane, abort_flag, p.status, kStageIdAttnFwd, 500 + s)) break;
                 if ((w4.x & w4.y & w4.z & w4.w) != 0xffffffffu) {
                     const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
@@ -288,7 +288,7 @@ attn_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             for (int j = 0; j < n; ++j) {
                 const int t = tile_at(j);
                 uint4 w4 = make_uint4(~0u, ~0u, ~0u, ~0u);
-                if (fp.words != nullptr) w4 = __ldg(reinterpret_cast<const uint4*>(fp.words) + (long long)b * fp.n_tiles + t);
+                if (fp.words != nullptr) w4 = at_load(reinterpret_cast<const uint4*>(fp.words) + (long long)b * fp.n_tiles + t);
                 else if ((t + 1) * kAfRows > p.Lk) w4 = tail_words(p.Lk - t * kAfRows);
                 if (!(ok = warp_wait(&s_full[w], j & 1, lane, abort_flag, p.status, kStageIdAttnFwd, 400 + w))) break;
                 tcgen05_fence_after();
@@ -465,7 +465,7 @@ attn_combine_kernel(const __grid_constant__ AttnParams p, const float* part_o, c
     if (r >= rows) return;
     const int lane = threadIdx.x & 31;
     float m = -INFINITY;
-    for (int s = lane; s < splits; s += 32) m = fmaxf(m, __ldg(part_ml + s * rows + r).x);
+    for (int s = lane; s < splits; s += 32) m = fmaxf(m, at_load(part_ml + s * rows + r).x);
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float base = m == -INFINITY ? 0.f : m;
@@ -473,7 +473,7 @@ attn_combine_kernel(const __grid_constant__ AttnParams p, const float* part_o, c
 #pragma unroll
     for (int k = 0; k < 8; ++k) y[k] = 0.f;
     for (int s0 = 0; s0 < splits; s0 += 32) {
-        const float2 ml = s0 + lane < splits ? __ldg(part_ml + (s0 + lane) * rows + r) : make_float2(-INFINITY, 0.f);
+        const float2 ml = s0 + lane < splits ? at_load(part_ml + (s0 + lane) * rows + r) : make_float2(-INFINITY, 0.f);
         const float w = ex2f((ml.x - base) * kLog2e);
         l = fmaf(ml.y, w, l);
         const int n = min(32, splits - s0);
@@ -483,7 +483,7 @@ attn_combine_kernel(const __grid_constant__ AttnParams p, const float* part_o, c
             if (32 * k >= p.D) break;
             const float* o = part_o + (s0 * rows + r) * p.D + min(d, p.D - 1);
 #pragma unroll 8
-            for (int s = 0; s < n; ++s) y[k] = fmaf(__ldg(o + s * rows * p.D), __shfl_sync(0xffffffffu, w, s), y[k]);
+            for (int s = 0; s < n; ++s) y[k] = fmaf(at_load(o + s * rows * p.D), __shfl_sync(0xffffffffu, w, s), y[k]);
         }
     }
 #pragma unroll

@@ -532,7 +532,7 @@ attn_bias_sum_kernel(const float* ds, long long ds_b, long long ds_h, T* out, lo
                 const float4* src = reinterpret_cast<const float4*>(ds + b * ds_b + h * ds_h) + (long long)c * kLoads * Lq + i;
 #pragma unroll
                 for (int l = 0; l < kLoads; ++l) {
-                    const float4 v = __ldg(src + (long long)l * Lq);
+                    const float4 v = at_load(src + (long long)l * Lq);
                     acc[4 * l] += v.x;
                     acc[4 * l + 1] += v.y;
                     acc[4 * l + 2] += v.z;

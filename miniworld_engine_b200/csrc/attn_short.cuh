@@ -94,7 +94,7 @@ attn_short_kernel(const __grid_constant__ AttnShortParams sp) {
 #pragma unroll
         for (int u = 0; u < kAsLoads; ++u) {
             const int j = j0 + u * kKeys + sub;
-            bits |= (uint32_t)(j < k_end && (mask == nullptr || __ldg(mask + j) != 0)) << u;
+            bits |= (uint32_t)(j < k_end && (mask == nullptr || at_load(mask + j) != 0)) << u;
         }
         return bits;
     };
@@ -109,12 +109,12 @@ attn_short_kernel(const __grid_constant__ AttnShortParams sp) {
         for (int u = 0; u < kAsLoads; ++u) {
             const int j = j0 + u * kKeys + sub;
             kv[u] = vv[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (in && ((keep >> u) & 1u)) kv[u] = __ldg(reinterpret_cast<const uint4*>(k + (long long)j * p.k.l));
+            if (in && ((keep >> u) & 1u)) kv[u] = at_load(reinterpret_cast<const uint4*>(k + (long long)j * p.k.l));
         }
 #pragma unroll
         for (int u = 0; u < kAsLoads; ++u) {
             const int j = j0 + u * kKeys + sub;
-            if (in && ((keep >> u) & 1u)) vv[u] = __ldg(reinterpret_cast<const uint4*>(v + (long long)j * p.v.l));
+            if (in && ((keep >> u) & 1u)) vv[u] = at_load(reinterpret_cast<const uint4*>(v + (long long)j * p.v.l));
         }
         float s[kAsLoads][kR];
 #pragma unroll

@@ -354,3 +354,14 @@ def test_scales_beyond_32_bits_are_refused(monkeypatch, scale):
     with pytest.raises(ValueError, match="scale must be finite"):
         cross_attention_b200(q[:0], k[:0], k[:0], scale=scale)          # also where nothing is computed
     assert attention._Call(q, k, k, None, None, torch.finfo(torch.float32).max, False).pack((0, 0, 0, 0), 0, 0)
+
+
+def test_attention_kernels_load_nothing_through_the_non_coherent_path():
+    """They run while the kernel before them still writes; that path is for memory that is not written meanwhile."""
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(_lib.__file__), "csrc")
+    for name in sorted(os.listdir(csrc)):
+        if name.startswith("attn_"):
+            code = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, name)).read())
+            assert not re.search(r"__ldg|ld\.global\.nc|__restrict__", code), name
